@@ -350,6 +350,83 @@ int32_t omni_qattn_decode_host(const void* q_host, int32_t q_dtype, void* q_stag
                                int32_t n_splits, void* workspace, size_t workspace_bytes,
                                int32_t* status_word);
 
+/* ---- prompts: the way into the cache -------------------------------------------------------------------------
+ * Per-head norm of queries and keys and their position rotation in one pass (no counterpart in the reference, whose
+ * inputs are already rotated projections).  x[0] queries, x[1] keys (heads[1] == 0: none), rows of `dtype` at element
+ * strides xs[.][users, heads, tokens]; y[.] contiguous [B][heads][T][128].
+ *   normalize   y = x * rsqrt(mean(x^2) + eps) * weight (weight[.] [128] of weight_dtype[.], NULL = ones)
+ *   n_pairs     P <= 64 pairs are rotated by position * inv_freq[pair], (i, i + P) or, interleaved, (2i, 2i + 1); the
+ *               dims behind 2P pass through.  The angle is formed and reduced in fp64.
+ *   n_axes      pairs [axis_end[a-1], axis_end[a]) follow the positions of axis a (axis_end[n_axes-1] == P)
+ *   positions   int32, or int64 when positions64, at strides ps[axes, users, tokens]; inv_freq fp32, or fp64 when
+ *               inv_freq64, [P]
+ * Rows must start on 16-byte boundaries.  fp32 inside, one rounding at the store. */
+#define OMNI_MAX_AXES 4
+typedef struct omni_norm_rope_t {
+    const void* x[2]; void* y[2]; const void* weight[2];
+    const void* positions; const void* inv_freq;
+    int64_t xs[2][3];
+    int64_t ps[3];
+    int64_t B, T;
+    int32_t heads[2];
+    int32_t weight_dtype[2];
+    int32_t axis_end[OMNI_MAX_AXES];
+    int32_t dtype, n_axes, n_pairs, positions64, inv_freq64, interleaved, normalize;
+    float   eps;
+} omni_norm_rope_t;
+int32_t omni_qk_norm_rope(const omni_norm_rope_t* call, void* stream);
+
+/* Attention of whole prompts over themselves, before their keys are packed: out[b,h,i] = sum_j softmax_j(scale q[b,h,i].
+ * k[b,h / (Hq / Hkv),j]) v[b,..,j] over the keys j of the same prompt, j <= i when causal.
+ *   q, k, v      rows of `dtype` at element strides [users, heads, tokens], starting on 16-byte boundaries
+ *   cu_seqlens   device int32 [n_seqs + 1], ascending: prompt i is rows cu[i] .. cu[i+1]-1 of the one user (B == 1) whose T
+ *                rows hold all prompts; rows of no prompt get zeros.  NULL: every user is one prompt (n_seqs == B)
+ *   seq_lens     device int32 [B] or NULL (T): without cu_seqlens, rows of a user at and behind its length get zeros
+ *   out          contiguous [B][Hq][T][128] of `dtype`
+ * Values of masked keys never reach a row, whatever they hold (infinities and NaN included).  Scores, softmax statistics and
+ * sums are fp32; for bf16 and fp16 the weights are rounded to that type for the second product.
+ *   status_word  device int32 or NULL, as in omni_qattn_decode */
+int32_t omni_prompt_attn(const void* q, const void* k, const void* v, int32_t dtype,
+                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         const int32_t* cu_seqlens, int64_t n_seqs, const int32_t* seq_lens,
+                         int64_t B, int32_t Hq, int32_t Hkv, int64_t T, float scale, int32_t causal,
+                         void* out, int32_t* status_word, void* stream);
+
+/* ---- eviction: keeping the cache small -----------------------------------------------------------------------
+ * The softmax weight that every cached key receives from T queries of its kv head's group (what omni_qattn_decode weighs
+ * V with), summed over the queries: sums[b,h,s] = sum_{g,t} softmax_s(scale q[b,h*G+g,t].k^[b,h,s]), fp32 [B][Hkv][S].
+ *   causal       the T queries are those of the cache's last T tokens: query t sees the keys s <= len - T + t (a query
+ *                without keys adds nothing); 0: every query sees all keys below the length
+ *   accumulate   0: every entry is written, zeros at and behind the length; 1: added to what sums holds, entries at and
+ *                behind the length stay as they are
+ * Cache arguments as in omni_qattn_decode ([B][Hkv][S] rows, contiguous).  Sums are formed in a fixed order: the same call
+ * gives the same bits.  `workspace`: omni_attn_weight_sums_workspace_bytes(...) bytes of device scratch. */
+size_t  omni_attn_weight_sums_workspace_bytes(int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S);
+int32_t omni_attn_weight_sums(const void* q, int32_t q_dtype, const uint8_t* k_nib, const uint8_t* k_qjl,
+                              const float* k_norms, const float* codebooks, int32_t cb_per_head,
+                              const int32_t* user_ids, int32_t user_id, const int32_t* seq_lens,
+                              int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S, float scale, int32_t with_qjl,
+                              int32_t rotate_q, int32_t causal, int32_t accumulate, void* workspace,
+                              size_t workspace_bytes, float* sums, void* stream);
+
+/* Eviction by accumulated weight: of every (user, head) with more than `budget` keys the `recent` last ones and the
+ * budget - recent others with the largest sums stay (equal sums: the lower position; NaN counts as the largest), in their
+ * order, gathered into the *_out arrays [B][H][capacity], capacity >= budget.  Users with at most `budget` keys keep all.
+ * Rows at and behind the new length are zeros.  index[b,h,i] is the old position of the i-th kept key, -1 behind the new
+ * length; new_lens[b] = min(length, budget).  v_qjl and v_norms may both be NULL.  v_paired: V's nibble rows are in the pair
+ * layout of omni_v_pair_groups for the old lengths and leave in that of the new ones. */
+typedef struct omni_evict_t {
+    const float* sums; const int32_t* seq_lens;              /* [B][H][S]; [B] or NULL (S) */
+    const uint8_t* k_nib; const uint8_t* k_qjl; const float* k_norms; const uint8_t* v_nib; const uint8_t* v_qjl; const float* v_norms;
+    float* sums_out;
+    uint8_t* k_nib_out; uint8_t* k_qjl_out; float* k_norms_out; uint8_t* v_nib_out; uint8_t* v_qjl_out; float* v_norms_out;
+    int32_t* index;                                          /* [B][H][budget] */
+    int32_t* new_lens;                                       /* [B] */
+    int64_t B, S, budget, recent, capacity;
+    int32_t H, v_paired;
+} omni_evict_t;
+int32_t omni_evict_keys(const omni_evict_t* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

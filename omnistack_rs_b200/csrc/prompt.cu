@@ -1,0 +1,248 @@
+// Attention of whole prompts over themselves: entry point and the fp32 kernel.
+//
+//   s_ij = scale q_i . k_j (j of the same prompt, j <= i when causal),  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
+//
+// One pass over the keys with the running maximum m and sum of each row.  64 x 64 tiles of scores on the FP32 units: 256
+// threads, 4 x 4 scores and 4 x 8 outputs each; K and V share one buffer so that two CTAs fit an SM.
+#include "prompt.cuh"
+
+namespace omni {
+
+constexpr int kPfM = 64, kPfN = 64;                // rows (token, head) and keys of a tile
+constexpr int kPfThreads = 256;
+constexpr int kPfStride = kHeadDim + 4;            // floats: a warp's sixteen key rows start in different banks
+constexpr int kPfPStride = kPfN + 4;
+constexpr int kPfSmem = (2 * kPfM * kPfStride + kPfM * kPfPStride) * 4;
+constexpr float kPfLog2e = 1.4426950408889634f;
+
+// rows [r0, r0 + 64) of a strided head into shared memory as fp32, zeros from row `end` on
+template <int DT>
+__device__ __forceinline__ void pf_load_tile(float* dst, const void* src, int64_t base, int64_t stride, int r0, int end) {
+#pragma unroll
+    for (int i = 0; i < kPfN * 32 / kPfThreads; ++i) {
+        const int at = i * kPfThreads + threadIdx.x, row = at >> 5, c = (at & 31) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (r0 + row < end) Elem<DT>::load4(src, base + (int64_t)(r0 + row) * stride + c, v);
+        *reinterpret_cast<float4*>(dst + row * kPfStride + c) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid_constant__ PromptArgs a) {
+    extern __shared__ __align__(16) float pf_smem[];
+    float* Qs = pf_smem;
+    float* Ks = Qs + kPfM * kPfStride;                                   // keys, then the values of the same tile
+    float* Ps = Ks + kPfN * kPfStride;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int64_t slot = (int64_t)gridDim.x - 1 - blockIdx.x;            // a prompt's last tiles have the most keys: first
+    const PromptTile w = prompt_tile(a, slot, tid & 31);
+    const int hg = blockIdx.y % a.n_hg, hkv = blockIdx.y / a.n_hg;
+    const int G = a.Hq / a.Hkv, head0 = hkv * G + hg * a.gp;
+    typename Elem<DT>::T* out = reinterpret_cast<typename Elem<DT>::T*>(a.out);
+
+    // ---- rows that belong to no prompt -----------------------------------------------------------------------------
+    {
+        int64_t z0 = slot * a.tpt, zb = 0;                               // packed: this CTA looks after rows z0 .. z0 + tpt - 1
+        int64_t live0 = 0, live1 = 0;
+        if (a.cu) {
+            live0 = __ldg(a.cu);
+            live1 = __ldg(a.cu + a.n_seqs);
+        } else {
+            z0 = w.t0; zb = w.b; live1 = w.len;
+        }
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        if (z0 < a.T && (z0 < live0 || z0 + a.tpt > live1)) {
+            for (int at = tid; at < a.tpt * a.gp * 32; at += kPfThreads) {
+                const int64_t t = z0 + (at >> 5) % a.tpt;
+                const int head = head0 + (at >> 5) / a.tpt;
+                if (t < a.T && (t < live0 || t >= live1)) Elem<DT>::store4(out, ((zb * a.Hq + head) * a.T + t) * kHeadDim + 4 * (at & 31), zero);
+            }
+        }
+    }
+    if (w.t0 >= w.len) return;
+
+    // ---- queries, scaled for exponents of two --------------------------------------------------------------------------
+    const float qs = a.scale * kPfLog2e;
+    for (int at = tid; at < kPfM * 32; at += kPfThreads) {
+        const int row = at >> 5, c = (at & 31) * 4;
+        const int t = w.t0 + row % a.tpt, g = row / a.tpt;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (g < a.gp && t < w.len) Elem<DT>::load4(a.q, w.b * a.qs[0] + (int64_t)(head0 + g) * a.qs[1] + (w.row0 + t) * a.qs[2] + c, v);
+        *reinterpret_cast<float4*>(Qs + row * kPfStride + c) = make_float4(v[0] * qs, v[1] * qs, v[2] * qs, v[3] * qs);
+    }
+    int lim[4];                                                          // newest key of this thread's rows (-1: no row)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 4 * ty + i, t = w.t0 + row % a.tpt;
+        lim[i] = row / a.tpt < a.gp && t < w.len ? (a.causal ? t : w.len - 1) : -1;
+    }
+    const int t_last = w.t0 + a.tpt - 1 < w.len ? w.t0 + a.tpt - 1 : w.len - 1;
+    const int n_keys = a.causal ? t_last + 1 : w.len;
+    const int n_free = a.causal ? w.t0 + 1 : w.len;                      // keys below this are open to every row of the tile
+    const int64_t kbase = w.b * a.ks[0] + (int64_t)hkv * a.ks[1] + w.row0 * a.ks[2];
+    const int64_t vbase = w.b * a.vs[0] + (int64_t)hkv * a.vs[1] + w.row0 * a.vs[2];
+    float m[4], l[4], o[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m[i] = -INFINITY; l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[i][c] = 0.f;
+    }
+
+    for (int j0 = 0; j0 < n_keys; j0 += kPfN) {
+        const bool masked = j0 + kPfN > n_free;
+        __syncthreads();                                                 // the previous tile's values are no longer read
+        pf_load_tile<DT>(Ks, a.k, kbase, a.ks[2], j0, n_keys);
+        __syncthreads();
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < kHeadDim; d += 4) {
+            float4 qv[4], kv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(Qs + (4 * ty + i) * kPfStride + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * kPfStride + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[i][j] = fmaf(qv[i].x, kv[j].x, s[i][j]);
+                    s[i][j] = fmaf(qv[i].y, kv[j].y, s[i][j]);
+                    s[i][j] = fmaf(qv[i].z, kv[j].z, s[i][j]);
+                    s[i][j] = fmaf(qv[i].w, kv[j].w, s[i][j]);
+                }
+        }
+        __syncthreads();                                                 // the keys have been read
+        pf_load_tile<DT>(Ks, a.v, vbase, a.vs[2], j0, n_keys);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j0 + tx + 16 * j > lim[i]) s[i][j] = -INFINITY;
+            }
+            float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+#pragma unroll
+            for (int x = 8; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, x));
+            const float m_new = fmaxf(m[i], mx);
+            const float ref = m_new == -INFINITY ? 0.f : m_new;          // no open key so far: every weight below is zero
+            const float alpha = exp2f(m[i] - ref);
+            m[i] = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2f(s[i][j] - ref);
+                sum += p;
+                Ps[(4 * ty + i) * kPfPStride + tx + 16 * j] = p;
+            }
+#pragma unroll
+            for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(kFullMask, sum, x);
+            l[i] = fmaf(l[i], alpha, sum);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[i][c] *= alpha;
+        }
+        __syncthreads();
+        if (!masked) {
+#pragma unroll 2
+            for (int j = 0; j < kPfN; j += 4) {
+                float4 pv[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(Ps + (4 * ty + i) * kPfPStride + j);
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const float4 va = *reinterpret_cast<const float4*>(Ks + (j + jj) * kPfStride + 4 * tx);
+                    const float4 vb = *reinterpret_cast<const float4*>(Ks + (j + jj) * kPfStride + 64 + 4 * tx);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = jj == 0 ? pv[i].x : jj == 1 ? pv[i].y : jj == 2 ? pv[i].z : pv[i].w;
+                        o[i][0] = fmaf(p, va.x, o[i][0]); o[i][1] = fmaf(p, va.y, o[i][1]);
+                        o[i][2] = fmaf(p, va.z, o[i][2]); o[i][3] = fmaf(p, va.w, o[i][3]);
+                        o[i][4] = fmaf(p, vb.x, o[i][4]); o[i][5] = fmaf(p, vb.y, o[i][5]);
+                        o[i][6] = fmaf(p, vb.z, o[i][6]); o[i][7] = fmaf(p, vb.w, o[i][7]);
+                    }
+                }
+            }
+        } else {                                                         // zero weights must not meet a masked key's infinities
+            for (int j = 0; j < kPfN && j0 + j < n_keys; ++j) {
+                const float4 va = *reinterpret_cast<const float4*>(Ks + j * kPfStride + 4 * tx);
+                const float4 vb = *reinterpret_cast<const float4*>(Ks + j * kPfStride + 64 + 4 * tx);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (j0 + j > lim[i]) continue;
+                    const float p = Ps[(4 * ty + i) * kPfPStride + j];
+                    o[i][0] = fmaf(p, va.x, o[i][0]); o[i][1] = fmaf(p, va.y, o[i][1]);
+                    o[i][2] = fmaf(p, va.z, o[i][2]); o[i][3] = fmaf(p, va.w, o[i][3]);
+                    o[i][4] = fmaf(p, vb.x, o[i][4]); o[i][5] = fmaf(p, vb.y, o[i][5]);
+                    o[i][6] = fmaf(p, vb.z, o[i][6]); o[i][7] = fmaf(p, vb.w, o[i][7]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 4 * ty + i, t = w.t0 + row % a.tpt;
+        if (lim[i] < 0) continue;
+        const float inv = 1.f / l[i];
+        const int64_t at = ((w.b * a.Hq + head0 + row / a.tpt) * a.T + w.row0 + t) * kHeadDim;
+        const float lo[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
+        const float hi[4] = {o[i][4] * inv, o[i][5] * inv, o[i][6] * inv, o[i][7] * inv};
+        Elem<DT>::store4(out, at + 4 * tx, lo);
+        Elem<DT>::store4(out, at + 64 + 4 * tx, hi);
+    }
+}
+
+template <int DT>
+static int32_t launch_prompt_fp32(PromptArgs a, cudaStream_t st) {
+    a.tpt = kPfM / a.gp;
+    a.slots = a.cu ? a.T / a.tpt + a.n_seqs : a.B * ((a.T + a.tpt - 1) / a.tpt);
+    OMNI_REQUIRE(a.slots <= 0x7fffffffLL && (int64_t)a.Hkv * a.n_hg <= 65535, OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: too many tiles");
+    OMNI_CUDA(cudaFuncSetAttribute(prompt_fp32_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmem));
+    prompt_fp32_kernel<DT><<<dim3((unsigned)a.slots, (unsigned)(a.Hkv * a.n_hg)), kPfThreads, kPfSmem, st>>>(a);
+    return check_cuda(cudaGetLastError(), "prompt_fp32_kernel launch");
+}
+
+}  // namespace omni
+
+using namespace omni;
+
+extern "C" int32_t omni_prompt_attn(const void* q, const void* k, const void* v, int32_t dtype,
+                                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                    const int32_t* cu_seqlens, int64_t n_seqs, const int32_t* seq_lens,
+                                    int64_t B, int32_t Hq, int32_t Hkv, int64_t T, float scale, int32_t causal,
+                                    void* out, int32_t* status_word, void* stream) {
+    OMNI_REQUIRE(B >= 0 && T >= 0 && Hq > 0 && Hkv > 0 && n_seqs >= 0, OMNI_ERR_ARG, "omni_prompt_attn: bad extent");
+    OMNI_REQUIRE(Hq % Hkv == 0, OMNI_ERR_ARG, "omni_prompt_attn: Hq=%d is not a multiple of Hkv=%d", Hq, Hkv);
+    OMNI_REQUIRE(dtype >= 0 && dtype <= 2, OMNI_ERR_ARG, "omni_prompt_attn: unknown dtype code %d", dtype);
+    OMNI_REQUIRE(T <= 0x3fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: more than 2^30 rows per user");
+    OMNI_REQUIRE(cu_seqlens ? B == 1 && !seq_lens : n_seqs == B, OMNI_ERR_ARG, "omni_prompt_attn: packed prompts are the rows of one user; otherwise every user is one prompt");
+    if (B == 0 || T == 0) return OMNI_OK;
+    OMNI_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides, OMNI_ERR_ARG, "omni_prompt_attn: NULL buffer");
+    const int64_t unit = dtype == OMNI_F32 ? 4 : 8;
+    OMNI_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");
+    PromptArgs a{};
+    for (int i = 0; i < 3; ++i) {
+        OMNI_REQUIRE(q_strides[i] % unit == 0 && k_strides[i] % unit == 0 && v_strides[i] % unit == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");
+        a.qs[i] = q_strides[i]; a.ks[i] = k_strides[i]; a.vs[i] = v_strides[i];
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    if (n_seqs == 0) {
+        OMNI_CUDA(cudaMemsetAsync(out, 0, (size_t)(B * Hq * T) * kHeadDim * (dtype == OMNI_F32 ? 4 : 2), st));
+        return OMNI_OK;
+    }
+    a.q = q; a.k = k; a.v = v; a.out = out; a.cu = cu_seqlens; a.seq_lens = seq_lens;
+    a.B = B; a.T = T; a.n_seqs = n_seqs; a.Hq = Hq; a.Hkv = Hkv; a.scale = scale; a.causal = causal; a.status = status_word;
+    // heads per tile: the largest divisor of the group up to sixteen
+    const int G = Hq / Hkv;
+    a.gp = 1;
+    for (int g = 2; g <= 16; ++g) if (G % g == 0) a.gp = g;
+    a.n_hg = G / a.gp;
+    switch (dtype) {
+        case OMNI_F32:  return launch_prompt_fp32<OMNI_F32>(a, st);
+        case OMNI_BF16: return launch_prompt_fp32<OMNI_BF16>(a, st);
+        default:        return launch_prompt_fp32<OMNI_F16>(a, st);
+    }
+}

@@ -1,0 +1,71 @@
+// Declarations shared by the prompt-attention translation units.
+#pragma once
+#include "common.cuh"
+
+namespace omni {
+
+// Attention of whole prompts over themselves.  Rows of q / k / v are (b, h, t) with element strides; a prompt is a run of rows
+// of one b:  packed:  b = 0, rows cu[i] .. cu[i + 1] - 1;   padded:  b = i, rows 0 .. seq_lens[i] - 1 (or T - 1).
+// A tile holds `gp` query heads of one kv head next to each other (row r = head r / tpt of the group, token t0 + r % tpt), so
+// that short prompts still fill it and every key is read once for all of them.
+struct PromptArgs {
+    const void* q; const void* k; const void* v; void* out;
+    int64_t qs[3], ks[3], vs[3];                   // element strides of (b, h, t)
+    const int32_t* cu; const int32_t* seq_lens;
+    int64_t B, T, n_seqs;
+    int Hq, Hkv, gp, n_hg;                         // gp heads per tile, n_hg = Hq / Hkv / gp tiles of heads per kv head
+    int tpt;                                       // tokens per tile
+    int64_t slots;                                 // tile slots per head group (an upper bound where lengths are on the device)
+    float scale;
+    int causal;
+    int32_t* status;
+};
+
+struct PromptTile {
+    int64_t b, row0;                               // first row of the prompt
+    int len, t0;                                   // its length; first token of the tile (>= len: nothing to do)
+};
+
+// The prompt and tile behind a slot.  Padded: slots are (b, tile).  Packed: prompt i owns the slots from cu[i] / tpt + i up to
+// those of prompt i + 1, which are at least ceil(len / tpt) of them; a warp finds the prompt with 32 probes a step.
+// All 32 lanes of a warp call this together.
+__device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& a, int64_t slot, int lane) {
+    PromptTile r;
+    if (!a.cu) {
+        const int64_t per = a.slots / a.n_seqs;
+        r.b = slot / per;
+        r.row0 = 0;
+        int64_t len = a.seq_lens ? (int64_t)__ldg(a.seq_lens + r.b) : a.T;
+        r.len = (int)(len < 0 ? 0 : (len > a.T ? a.T : len));
+        r.t0 = (int)(slot % per) * a.tpt;
+        return r;
+    }
+    // the last prompt whose first slot is at or below `slot` (first slots ascend strictly; that of prompt 0 counts as 0)
+    int64_t lo = 0, n = a.n_seqs;                  // the answer lies in [lo, lo + n)
+    while (n > 1) {
+        const int64_t step = (n + 31) / 32;
+        const int64_t i = lo + lane * step;
+        bool below = lane == 0;
+        if (lane > 0 && i < lo + n) {
+            int64_t c = __ldg(a.cu + i);
+            c = c < 0 ? 0 : (c > a.T ? a.T : c);
+            below = c / a.tpt + i <= slot;
+        }
+        const int hit = 31 - __clz((int)__ballot_sync(kFullMask, below));
+        const int64_t next = lo + hit * step;
+        n = lo + n - next < step ? lo + n - next : step;
+        lo = next;
+    }
+    int64_t c0 = __ldg(a.cu + lo), c1 = __ldg(a.cu + lo + 1);
+    c0 = c0 < 0 ? 0 : (c0 > a.T ? a.T : c0);
+    c1 = c1 < c0 ? c0 : (c1 > a.T ? a.T : c1);
+    r.b = 0;
+    r.row0 = c0;
+    r.len = (int)(c1 - c0);
+    const int64_t first = c0 / a.tpt + lo;
+    const int64_t t0 = (slot - first) * a.tpt;
+    r.t0 = slot < first || t0 > r.len ? r.len : (int)t0;
+    return r;
+}
+
+}  // namespace omni

@@ -1,0 +1,84 @@
+"""Attention of whole prompts over themselves on the GPU: what runs before a prompt's keys and values are packed.
+
+The reference computes it with ``reference_attn`` (omnistack_rs/attention/reference.py:72) over dense tensors and an additive
+mask; here a prompt's bounds and the causal order are arguments, and prompts of different lengths share a call.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+import torch
+
+from .. import _lib
+from .hadamard import HEAD_DIM
+from .position import _rows, _strides
+
+
+def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
+                seq_lens: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None) -> torch.Tensor:
+    """``softmax(scale q k^T) v`` within every prompt; returns a new contiguous tensor of ``q``'s shape and dtype.
+
+    ``q`` (B, n_heads, T, 128), ``k`` and ``v`` (B, n_kv_heads, T, 128), float32, bfloat16 or float16, any strides over users,
+    heads and tokens; n_heads is a multiple of n_kv_heads.  Query t sees the keys up to t (``causal``) or all keys of its
+    prompt.  ``scale`` defaults to 1/sqrt(128).
+
+    Padded prompts: user b's prompt is its first ``seq_lens[b]`` rows (all T without ``seq_lens``).
+    Packed prompts: B is 1 and ``cu_seqlens`` (n + 1,) gives the row at which each prompt begins, and the end of the last.
+    Lengths held on the host are checked here; lengths on the device are taken as they are, cut to the T rows there are.
+    Rows that belong to no prompt are zeros in the result, and what they hold in ``k`` and ``v`` reaches no other row, nor do
+    the keys and values behind a query's own position (infinities and NaN included).
+
+    Scores, softmax statistics and sums are float32.  For bfloat16 and float16 the tensor cores multiply the weights, rounded
+    to that type, with the values; float32 stays float32 throughout."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k and v must be (B, n_heads, T, 128)")
+    B, Hq, T, D = q.shape
+    if D != HEAD_DIM:
+        raise ValueError(f"attention requires last dim = {HEAD_DIM} (head_dim), got {D}")
+    Hkv = k.shape[1]
+    if k.shape != (B, Hkv, T, HEAD_DIM) or v.shape != k.shape:
+        raise ValueError(f"k and v must be ({B}, n_kv_heads, {T}, {HEAD_DIM}) like q, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if Hkv == 0 or Hq % Hkv or Hq == 0:
+        raise ValueError(f"n_heads={Hq} is not a multiple of n_kv_heads={Hkv}")
+    if q.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {q.dtype}; use float32, bfloat16 or float16")
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise TypeError(f"q, k and v have different dtypes: {q.dtype}, {k.dtype} and {v.dtype}")
+    lengths = None
+    if cu_seqlens is not None:
+        if seq_lens is not None:
+            raise ValueError("give cu_seqlens (packed prompts) or seq_lens (padded ones), not both")
+        if B != 1:
+            raise ValueError(f"packed prompts are the rows of one user (B = 1), got B = {B}")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError(f"cu_seqlens must have shape (n_prompts + 1,), got {tuple(cu_seqlens.shape)}")
+        lengths, name = cu_seqlens, "cu_seqlens"
+    elif seq_lens is not None:
+        if seq_lens.shape != (B,):
+            raise ValueError(f"seq_lens must have shape ({B},), got {tuple(seq_lens.shape)}")
+        lengths, name = seq_lens, "seq_lens"
+    if lengths is not None:
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name} must be int32 or int64, got {lengths.dtype}")
+        if lengths.device.type == "cpu" and lengths.numel():
+            if int(lengths.min()) < 0 or int(lengths.max()) > T:
+                raise ValueError(f"{name} must lie in [0, {T}]")
+            if cu_seqlens is not None and bool((lengths[1:] < lengths[:-1]).any()):
+                raise ValueError("cu_seqlens must ascend")
+    dev = _lib.require_cuda(q, k, v)
+    lib = _lib.load()
+    if lengths is not None:
+        lengths = _lib.as_device(lengths, dev, torch.int32)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty(B, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
+    i64 = C.c_int64 * 3
+    packed = cu_seqlens is not None
+    with _lib.on_device(dev):
+        _lib.check(lib.omni_prompt_attn(
+            _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.DTYPE_CODE[q.dtype], i64(*_strides(q)), i64(*_strides(k)), i64(*_strides(v)),
+            _lib.ptr(lengths) if packed else None, lengths.numel() - 1 if packed else B, None if packed else _lib.ptr(lengths),
+            B, Hq, Hkv, T, float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale), int(bool(causal)),
+            _lib.ptr(out), _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr(dev)))
+    return out

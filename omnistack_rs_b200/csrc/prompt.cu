@@ -40,25 +40,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
     const int G = a.Hq / a.Hkv, head0 = hkv * G + hg * a.gp;
     typename Elem<DT>::T* out = reinterpret_cast<typename Elem<DT>::T*>(a.out);
 
-    // ---- rows that belong to no prompt -----------------------------------------------------------------------------
-    {
-        int64_t z0 = slot * a.tpt, zb = 0;                               // packed: this CTA looks after rows z0 .. z0 + tpt - 1
-        int64_t live0 = 0, live1 = 0;
-        if (a.cu) {
-            live0 = __ldg(a.cu);
-            live1 = __ldg(a.cu + a.n_seqs);
-        } else {
-            z0 = w.t0; zb = w.b; live1 = w.len;
-        }
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        if (z0 < a.T && (z0 < live0 || z0 + a.tpt > live1)) {
-            for (int at = tid; at < a.tpt * a.gp * 32; at += kPfThreads) {
-                const int64_t t = z0 + (at >> 5) % a.tpt;
-                const int head = head0 + (at >> 5) / a.tpt;
-                if (t < a.T && (t < live0 || t >= live1)) Elem<DT>::store4(out, ((zb * a.Hq + head) * a.T + t) * kHeadDim + 4 * (at & 31), zero);
-            }
-        }
-    }
+    prompt_zero_rows<DT>(a, w, slot, head0, tid, kPfThreads);
     if (w.t0 >= w.len) return;
 
     // ---- queries, scaled for exponents of two --------------------------------------------------------------------------
@@ -240,6 +222,8 @@ extern "C" int32_t omni_prompt_attn(const void* q, const void* k, const void* v,
     a.gp = 1;
     for (int g = 2; g <= 16; ++g) if (G % g == 0) a.gp = g;
     a.n_hg = G / a.gp;
+    // The tensor-core kernel takes its running maximum over unscaled scores, which needs a positive scale.
+    if (dtype != OMNI_F32 && scale > 0.f) return launch_prompt_umma(a, dtype, st);
     switch (dtype) {
         case OMNI_F32:  return launch_prompt_fp32<OMNI_F32>(a, st);
         case OMNI_BF16: return launch_prompt_fp32<OMNI_BF16>(a, st);

@@ -68,4 +68,28 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& a, int64_t s
     return r;
 }
 
+// Zeros in the rows that belong to no prompt.  Padded: the rows of the slot's tokens at and behind the length.  Packed: slot i
+// looks after rows i * tpt .. (i + 1) * tpt - 1 of the one user (there are more slots than such runs).
+template <int DT>
+__device__ __forceinline__ void prompt_zero_rows(const PromptArgs& a, const PromptTile& w, int64_t slot, int head0, int tid, int threads) {
+    int64_t z0 = slot * a.tpt, zb = 0, live0 = 0, live1 = 0;
+    if (a.cu) {
+        live0 = __ldg(a.cu);
+        live1 = __ldg(a.cu + a.n_seqs);
+    } else {
+        z0 = w.t0; zb = w.b; live1 = w.len;
+    }
+    if (z0 >= a.T || (z0 >= live0 && z0 + a.tpt <= live1)) return;
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int at = tid; at < a.tpt * a.gp * 32; at += threads) {
+        const int64_t t = z0 + (at >> 5) % a.tpt;
+        const int head = head0 + (at >> 5) / a.tpt;
+        if (t < a.T && (t < live0 || t >= live1))
+            Elem<DT>::store4(a.out, ((zb * a.Hq + head) * a.T + t) * kHeadDim + 4 * (at & 31), zero);
+    }
+}
+
+// Tensor-core kernel for bf16 and fp16 (prompt_umma.cu)
+int32_t launch_prompt_umma(PromptArgs a, int dtype, cudaStream_t st);
+
 }  // namespace omni

@@ -1,0 +1,455 @@
+// Attention of whole prompts over themselves on the fifth-generation tensor cores, bf16 and fp16.
+//
+// One CTA takes two tiles of 128 rows (row = token and query head of one kv head's group) and walks over the keys of their
+// prompt in blocks of 128:   S_t = Q_t K^T  ->  P_t = exp2(c S_t - m)  ->  O_t += P_t V     (t = 0, 1;  c = scale * log2 e)
+// Q, K and V tiles come by TMA (128-byte swizzle); S, P and O live in tensor memory (512 columns: S0 S1 O0 O1, each P in the
+// columns of its S, which the softmax threads have read by then).  Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1,
+// thread = row; warp 8 issues every product; warp 9 every copy.  While the softmax of one tile runs, the products of the
+// other do.
+//
+// A block's maximum only replaces the running one when it exceeds it by 2^slack, so O is rescaled rarely; the softmax threads
+// do it themselves: S_t of a block is issued behind P_t V of the block before, so its arrival says that O_t is complete.
+//
+// A zero weight times an infinite or NaN value of a masked key would be NaN.  Rows that come out NaN are therefore formed
+// again from global memory over their own keys alone (prompt_row_again), which settles NaN that belong there too.
+#include "prompt.cuh"
+#include <cuda.h>
+#include <mutex>
+
+namespace omni {
+
+constexpr int kPuThreads = 384;                    // warps 10 and 11 only complete the third warpgroup
+// Registers: 384 threads are launched with 168 each (64,512); the softmax warpgroups go up to 232, the third down to 40
+// (256 * 232 + 128 * 40 = 64,512).
+constexpr int kPuSoftmaxRegs = 232, kPuOtherRegs = 40;
+constexpr int kPuStages = 5;                       // ring of K and V tiles, 32 KiB each, in the order K0 V0 K1 V1 ...
+constexpr uint32_t kPuTile = 128 * 128 * 2;        // bytes of a 128-row tile: two halves of 64 dims, 128 bytes a row
+constexpr uint32_t kPuHalf = kPuTile / 2;
+constexpr uint32_t kPuOffK = 2 * kPuTile;
+constexpr uint32_t kPuOffBar = kPuOffK + kPuStages * kPuTile;
+constexpr uint32_t kPuSmem = kPuOffBar + 256 + 1024;       // barriers, and room to start on a 1,024-byte boundary
+constexpr uint32_t kPuColS = 0, kPuColO = 256, kPuTmemCols = 512;
+constexpr uint32_t kPuWaitLimit = 1u << 20;
+constexpr float kPuLog2e = 1.4426950408889634f;
+
+// ---- PTX wrappers --------------------------------------------------------------------------------
+__device__ __forceinline__ void pu_bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" :: "r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void pu_bar_arrive(uint32_t bar) {
+    asm volatile("{\n .reg .b64 t;\n mbarrier.arrive.shared::cta.b64 t, [%0];\n}\n" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void pu_bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n .reg .b64 t;\n mbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n}\n" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool pu_bar_wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kPuWaitLimit; ++i) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+// by all lanes of a warp, with one answer
+__device__ __forceinline__ bool pu_bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(kFullMask, pu_bar_wait(bar, parity)); }
+__device__ __forceinline__ void pu_tma_load(uint32_t dst, const CUtensorMap* map, int d, int t, int h, int b, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
+                 :: "r"(dst), "l"(map), "r"(d), "r"(t), "r"(h), "r"(b), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void pu_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void pu_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void pu_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void pu_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void pu_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool pu_elect() {
+    uint32_t is;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
+    return is != 0;
+}
+// Shared-memory matrix descriptors, 128-byte swizzle.  Low word: start address (>> 4) and, for an MN-major operand, the distance
+// (>> 4) between its runs of 64 elements along MN.  High word: 1,024 bytes between groups of eight rows, version, swizzle mode.
+constexpr uint32_t kPuDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t pu_desc(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void pu_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n"
+                 :: "r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kPuDescHi) : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void pu_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n"
+                 :: "r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kPuDescHi) : "memory");
+}
+__device__ __forceinline__ void pu_ld32(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void pu_st32(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
+                 :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                    "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+                    "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+                    "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+template <int DT>
+__device__ __forceinline__ constexpr uint32_t pu_idesc(bool b_mn_major) {
+    return (1u << 4) | (DT == OMNI_BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? (1u << 16) : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ float pu_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int DT> __device__ __forceinline__ uint32_t pu_pack(float lo, float hi) {
+    uint32_t r;
+    if constexpr (DT == OMNI_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// One output row over its own keys alone, by a warp (lane l has dims 4l .. 4l + 3), fp32 throughout.
+template <int DT>
+__device__ __forceinline__ void prompt_row_again(const PromptArgs& a, int64_t b, int64_t row0, int t, int newest, int head, int lane) {
+    const int hkv = head / (a.Hq / a.Hkv);
+    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+    Elem<DT>::load4(a.q, b * a.qs[0] + (int64_t)head * a.qs[1] + (row0 + t) * a.qs[2] + 4 * lane, q);
+    const int64_t kb = b * a.ks[0] + (int64_t)hkv * a.ks[1] + row0 * a.ks[2] + 4 * lane;
+    const int64_t vb = b * a.vs[0] + (int64_t)hkv * a.vs[1] + row0 * a.vs[2] + 4 * lane;
+    const float c = a.scale * kPuLog2e;
+    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j <= newest; ++j) {
+        float k[4], v[4];
+        Elem<DT>::load4(a.k, kb + (int64_t)j * a.ks[2], k);
+        Elem<DT>::load4(a.v, vb + (int64_t)j * a.vs[2], v);
+        float s = fmaf(q[0], k[0], fmaf(q[1], k[1], fmaf(q[2], k[2], q[3] * k[3])));
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(kFullMask, s, x);
+        s *= c;
+        const float m_new = fmaxf(m, s);
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2f(m - ref), p = exp2f(s - ref);
+        m = m_new;
+        l = fmaf(l, alpha, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(o[i], alpha, p * v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] /= l;
+    Elem<DT>::store4(a.out, ((b * a.Hq + head) * a.T + row0 + t) * kHeadDim + 4 * lane, o);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kPuThreads, 1)
+prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v) {
+    extern __shared__ unsigned char pu_smem[];
+    // fp16 weights carry 2^bias: the type ends at 2^-24, and weights far below the row's largest would lose their bits there
+    constexpr float kBias = DT == OMNI_F16 ? 8.f : 0.f, kSlack = DT == OMNI_F16 ? 7.f : 8.f;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t slot = (int64_t)gridDim.x - 1 - blockIdx.x;            // a prompt's last tiles have the most keys: first
+    const PromptTile w = prompt_tile(a, slot, lane);
+    const int hg = blockIdx.y % a.n_hg, hkv = blockIdx.y / a.n_hg;
+    const int head0 = hkv * (a.Hq / a.Hkv) + hg * a.gp;
+    prompt_zero_rows<DT>(a, w, slot, head0, tid, kPuThreads);
+    if (w.t0 >= w.len) return;
+
+    const int tt = a.tpt / 2;                                            // tokens of one tile
+    int n_blocks[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int first = w.t0 + x * tt, last = first + tt - 1 < w.len ? first + tt - 1 : w.len - 1;
+        n_blocks[x] = first >= w.len ? 0 : ((a.causal ? last + 1 : w.len) + 127) / 128;
+    }
+    const int n_all = n_blocks[0] > n_blocks[1] ? n_blocks[0] : n_blocks[1];
+
+    const uint32_t base = ((uint32_t)__cvta_generic_to_shared(pu_smem) + 1023u) & ~1023u;
+    const uint32_t sQ = base, sKV = base + kPuOffK, bars = base + kPuOffBar;
+    const uint32_t bar_q = bars, bar_full = bars + 16, bar_empty = bar_full + 8 * kPuStages, bar_s = bar_empty + 8 * kPuStages, bar_p = bar_s + 16,
+                   bar_o = bar_p + 16, tmem_at = bar_o + 16;
+    if (tid == 0) {
+        for (int x = 0; x < 2; ++x) {
+            pu_bar_init(bar_q + 8 * x, 1);
+            pu_bar_init(bar_s + 8 * x, 1);
+            pu_bar_init(bar_p + 8 * x, 4);
+            pu_bar_init(bar_o + 8 * x, 1);
+        }
+        for (int i = 0; i < kPuStages; ++i) {
+            pu_bar_init(bar_full + 8 * i, 1);
+            pu_bar_init(bar_empty + 8 * i, 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" :: "r"(tmem_at), "r"(kPuTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    pu_fence_before();
+    __syncthreads();
+    pu_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(tmem) : "r"(tmem_at));
+    bool ok = true;                                                      // false once a bounded wait has run out
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" :: "n"(kPuOtherRegs));
+        if (warp == 9) {
+            // ---- copies -----------------------------------------------------------------------------------------------
+            if (lane == 0) {
+                const uint32_t q_bytes = (uint32_t)(tt * a.gp) * 256u;
+                for (int x = 0; x < 2; ++x) {
+                    if (n_blocks[x] == 0) continue;
+                    pu_bar_expect(bar_q + 8 * x, q_bytes);
+                    for (int h = 0; h < 2; ++h)
+                        pu_tma_load(sQ + x * kPuTile + h * kPuHalf, &map_q, 64 * h, (int)w.row0 + w.t0 + x * tt, head0, (int)w.b, bar_q + 8 * x);
+                }
+                int i = 0;
+                for (; i < 2 * n_all; ++i) {                                 // tile i: K of block i / 2, or V when odd
+                    const int st = i % kPuStages, round = i / kPuStages;
+                    if (round > 0 && !pu_bar_wait(bar_empty + 8 * st, (round - 1) & 1)) { ok = false; break; }
+                    const uint32_t dst = sKV + st * kPuTile, bar = bar_full + 8 * st;
+                    pu_bar_expect(bar, kPuTile);
+                    const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
+                    for (int h = 0; h < 2; ++h) pu_tma_load(dst + h * kPuHalf, map, 64 * h, (int)w.row0 + 128 * (i >> 1), hkv, (int)w.b, bar);
+                }
+                // no copy may still be under way when the CTA ends (they all are complete unless a wait ran out)
+                if (!ok)
+                    for (int k = i < kPuStages ? 0 : i - kPuStages; k < i; ++k) pu_bar_wait(bar_full + 8 * (k % kPuStages), (k / kPuStages) & 1);
+            }
+        } else if (warp == 8) {
+            // ---- products: the whole warp waits, one thread issues ----------------------------------------------------------
+            auto issue_s = [&](int x, uint32_t sK) {
+                if (pu_elect()) {
+                    const uint32_t da = pu_desc(sQ + x * kPuTile, 16), db = pu_desc(sK, 16);
+    #pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t off = ((ks >> 2) * kPuHalf + (ks & 3) * 32) >> 4;
+                        pu_mma_ss(tmem + kPuColS + 128 * x, da + off, db + off, pu_idesc<DT>(false), ks > 0);
+                    }
+                    pu_commit(bar_s + 8 * x);
+                }
+                __syncwarp();
+            };
+            ok = pu_bar_wait_warp(bar_full, 0);
+            for (int x = 0; ok && x < 2; ++x) {
+                if (n_blocks[x] == 0) continue;
+                ok = pu_bar_wait_warp(bar_q + 8 * x, 0);
+                if (ok) { pu_fence_after(); issue_s(x, sKV); }
+            }
+            if (ok && pu_elect()) pu_commit(bar_empty);
+            int st = 0;                                                      // ring stage of K_j, and the parity of its round
+            uint32_t ph = 0;
+            for (int j = 0; ok && j < n_all; ++j) {
+                if (++st == kPuStages) { st = 0; ph ^= 1u; }                 // V_j
+                const int stv = st;
+                ok = pu_bar_wait_warp(bar_full + 8 * st, ph);
+                if (++st == kPuStages) { st = 0; ph ^= 1u; }                 // K_{j+1}
+                if (ok && j + 1 < n_all) ok = pu_bar_wait_warp(bar_full + 8 * st, ph);
+                const uint32_t sV = sKV + stv * kPuTile, sK = sKV + st * kPuTile;
+    #pragma unroll 1
+                for (int x = 0; ok && x < 2; ++x) {
+                    if (j >= n_blocks[x]) continue;
+                    ok = pu_bar_wait_warp(bar_p + 8 * x, j & 1);
+                    if (!ok) break;
+                    pu_fence_after();
+                    if (pu_elect()) {
+                        const uint32_t db = pu_desc(sV, kPuHalf), dd = tmem + kPuColO + 128 * x, da = tmem + kPuColS + 128 * x;
+    #pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) pu_mma_ts(dd, da + 8 * ks, db + ks * (2048 >> 4), pu_idesc<DT>(true), (j > 0 || ks > 0) ? 1u : 0u);
+                        if (j + 1 >= n_blocks[x]) pu_commit(bar_o + 8 * x);
+                    }
+                    __syncwarp();
+                    if (j + 1 < n_blocks[x]) issue_s(x, sK);
+                }
+                if (ok && pu_elect()) {
+                    pu_commit(bar_empty + 8 * stv);
+                    if (j + 1 < n_all) pu_commit(bar_empty + 8 * st);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" :: "n"(kPuSoftmaxRegs));
+        // ---- softmax of tile x, thread = row ------------------------------------------------------------------------
+        const int x = warp >> 2, row = tid & 127;
+        const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t t_s = t_lane + kPuColS + 128 * x, t_o = t_lane + kPuColO + 128 * x;
+        const int g = row / tt, t = w.t0 + x * tt + row % tt;
+        const bool live = g < a.gp && t < w.len;
+        // newest key of the row; rows without a query go through the motions on whatever their operands hold
+        const int lim = live ? (a.causal ? t : w.len - 1) : w.len - 1;
+        const int n_free = a.causal ? w.t0 + x * tt + 1 : w.len;         // keys below this are open to every row of the tile
+        const float c = a.scale * kPuLog2e;
+        float m = -INFINITY, l = 0.f;                                    // m: in units of c * score
+        for (int j = 0; j < n_blocks[x]; ++j) {
+            ok = pu_bar_wait_warp(bar_s + 8 * x, j & 1);
+            if (!ok) break;
+            pu_fence_after();
+            uint32_t s[128];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pu_ld32(t_s + 32 * i, s + 32 * i);
+            pu_wait_ld();
+            if (128 * j + 128 > n_free) {
+                const int open = lim - 128 * j;                          // columns 0 .. open of the block are seen
+#pragma unroll
+                for (int i = 0; i < 128; ++i) s[i] = i <= open ? s[i] : 0xff800000u;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 128; i += 4) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(s[i + k]));
+            }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+            const bool raise = top > m + kSlack;
+            if (__any_sync(kFullMask, raise)) {
+                const float m_new = raise ? top : m;
+                const float alpha = raise ? pu_ex2(m - m_new) : 1.f;
+                m = m_new;
+                l *= alpha;
+                if (j > 0) {
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t o[32];
+                        pu_ld32(t_o + 32 * i, o);
+                        pu_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                        pu_st32(t_o + 32 * i, o);
+                    }
+                }
+            }
+            const float neg = kBias - m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float p0 = pu_ex2(fmaf(__uint_as_float(s[64 * h + 2 * i]), c, neg));
+                    const float p1 = pu_ex2(fmaf(__uint_as_float(s[64 * h + 2 * i + 1]), c, neg));
+                    sum[(2 * i) & 3] += p0;
+                    sum[(2 * i + 1) & 3] += p1;
+                    p[i] = pu_pack<DT>(p0, p1);
+                }
+                pu_st32(t_s + 32 * h, p);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            pu_wait_st();
+            pu_fence_before();
+            __syncwarp();
+            if (lane == 0) pu_bar_arrive(bar_p + 8 * x);
+        }
+        // ---- result rows ---------------------------------------------------------------------------------------------
+        if (n_blocks[x] > 0) {
+            if (ok) ok = pu_bar_wait_warp(bar_o + 8 * x, 0);
+            if (ok) {
+                pu_fence_after();
+                const float inv = 1.f / l;
+                uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) +
+                                                      ((w.b * a.Hq + head0 + (live ? g : 0)) * a.T + w.row0 + (live ? t : w.t0)) * kHeadDim);
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t o[32];
+                    pu_ld32(t_o + 32 * i, o);
+                    pu_wait_ld();
+                    uint32_t r[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float u = __uint_as_float(o[2 * k]) * inv, v = __uint_as_float(o[2 * k + 1]) * inv;
+                        bad = bad || u != u || v != v;
+                        r[k] = pu_pack<DT>(u, v);
+                    }
+                    if (live) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) dst[4 * i + k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+                    }
+                }
+                uint32_t again = __ballot_sync(kFullMask, live && bad);
+                while (again) {
+                    const int src = __ffs(again) - 1;
+                    again &= again - 1;
+                    prompt_row_again<DT>(a, w.b, w.row0, __shfl_sync(kFullMask, t, src), __shfl_sync(kFullMask, lim, src),
+                                         head0 + __shfl_sync(kFullMask, g, src), lane);
+                }
+            }
+        }
+    }
+    if (!ok && a.status) atomicExch(a.status, OMNI_STATUS_WAIT_EXPIRED);
+    __syncwarp();
+    pu_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        pu_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" :: "r"(tmem), "r"(kPuTmemCols) : "memory");
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------
+typedef CUresult (*PuEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static PuEncodeFn pu_encode_fn() {
+    static std::mutex mu;
+    static PuEncodeFn fn = nullptr;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PuEncodeFn>(p);
+    }
+    return fn;
+}
+
+// view (dims, tokens, heads, users) of 16-bit rows, boxes of 64 dims x `tokens` x `heads`
+static int32_t pu_map(CUtensorMap* map, const void* base, int dtype, const int64_t* strides, int64_t T, int64_t H, int64_t B, int tokens, int heads) {
+    PuEncodeFn fn = pu_encode_fn();
+    OMNI_REQUIRE(fn != nullptr, OMNI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
+    cuuint64_t st[3];
+    const int64_t by[3] = {strides[2], strides[1], strides[0]}, n[3] = {T, H, B};
+    for (int i = 0; i < 3; ++i) {
+        st[i] = n[i] > 1 ? (cuuint64_t)(2 * by[i]) : (cuuint64_t)(2 * kHeadDim);          // an extent of one is never stepped over
+        OMNI_REQUIRE(st[i] > 0 && st[i] % 16 == 0 && st[i] < (1ull << 40), OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: stride of %lld elements", (long long)by[i]);
+    }
+    const cuuint32_t box[4] = {64u, (cuuint32_t)tokens, (cuuint32_t)heads, 1u}, one[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = fn(map, dtype == OMNI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, st,
+                          box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    OMNI_REQUIRE(r == CUDA_SUCCESS, OMNI_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return OMNI_OK;
+}
+
+template <int DT>
+static int32_t launch_prompt_umma_t(const PromptArgs& a, cudaStream_t st) {
+    CUtensorMap mq, mk, mv;
+    int32_t rc = pu_map(&mq, a.q, DT, a.qs, a.T, a.Hq, a.B, a.tpt / 2, a.gp);
+    if (rc == OMNI_OK) rc = pu_map(&mk, a.k, DT, a.ks, a.T, a.Hkv, a.B, 128, 1);
+    if (rc == OMNI_OK) rc = pu_map(&mv, a.v, DT, a.vs, a.T, a.Hkv, a.B, 128, 1);
+    if (rc != OMNI_OK) return rc;
+    OMNI_CUDA(cudaFuncSetAttribute(prompt_umma_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPuSmem));
+    prompt_umma_kernel<DT><<<dim3((unsigned)a.slots, (unsigned)(a.Hkv * a.n_hg)), kPuThreads, kPuSmem, st>>>(a, mq, mk, mv);
+    return check_cuda(cudaGetLastError(), "prompt_umma_kernel launch");
+}
+
+int32_t launch_prompt_umma(PromptArgs a, int dtype, cudaStream_t st) {
+    a.tpt = 2 * (128 / a.gp);
+    a.slots = a.cu ? a.T / a.tpt + a.n_seqs : a.B * ((a.T + a.tpt - 1) / a.tpt);
+    OMNI_REQUIRE(a.slots <= 0x7fffffffLL && (int64_t)a.Hkv * a.n_hg <= 65535, OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: too many tiles");
+    return dtype == OMNI_BF16 ? launch_prompt_umma_t<OMNI_BF16>(a, st) : launch_prompt_umma_t<OMNI_F16>(a, st);
+}
+
+}  // namespace omni

@@ -16,6 +16,12 @@ from .hadamard import HEAD_DIM
 from .position import _rows, _strides
 
 
+def _tiles(x: torch.Tensor) -> torch.Tensor:
+    """``x`` itself when a kernel can copy boxes of its rows, else a contiguous copy (tensor maps have no stride of 0)."""
+    x = _rows(x)
+    return x.contiguous() if any(st == 0 and n > 1 for st, n in zip(x.stride()[:3], x.shape[:3])) else x
+
+
 def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
                 seq_lens: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None) -> torch.Tensor:
     """``softmax(scale q k^T) v`` within every prompt; returns a new contiguous tensor of ``q``'s shape and dtype.
@@ -71,7 +77,7 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens
     lib = _lib.load()
     if lengths is not None:
         lengths = _lib.as_device(lengths, dev, torch.int32)
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    q, k, v = _tiles(q), _tiles(k), _tiles(v)
     out = torch.empty(B, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
     i64 = C.c_int64 * 3
     packed = cu_seqlens is not None

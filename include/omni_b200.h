@@ -400,14 +400,15 @@ int32_t omni_prompt_attn(const void* q, const void* k, const void* v, int32_t dt
  *   accumulate   0: every entry is written, zeros at and behind the length; 1: added to what sums holds, entries at and
  *                behind the length stay as they are
  * Cache arguments as in omni_qattn_decode ([B][Hkv][S] rows, contiguous).  Sums are formed in a fixed order: the same call
- * gives the same bits.  `workspace`: omni_attn_weight_sums_workspace_bytes(...) bytes of device scratch. */
+ * gives the same bits.  `workspace`: omni_attn_weight_sums_workspace_bytes(...) bytes of device scratch.
+ *   status_word  device int32 or NULL, as in omni_qattn_decode */
 size_t  omni_attn_weight_sums_workspace_bytes(int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S);
 int32_t omni_attn_weight_sums(const void* q, int32_t q_dtype, const uint8_t* k_nib, const uint8_t* k_qjl,
                               const float* k_norms, const float* codebooks, int32_t cb_per_head,
                               const int32_t* user_ids, int32_t user_id, const int32_t* seq_lens,
                               int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S, float scale, int32_t with_qjl,
                               int32_t rotate_q, int32_t causal, int32_t accumulate, void* workspace,
-                              size_t workspace_bytes, float* sums, void* stream);
+                              size_t workspace_bytes, float* sums, int32_t* status_word, void* stream);
 
 /* Eviction by accumulated weight: of every (user, head) with more than `budget` keys the `recent` last ones and the
  * budget - recent others with the largest sums stay (equal sums: the lower position; NaN counts as the largest), in their

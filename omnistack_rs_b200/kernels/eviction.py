@@ -100,7 +100,7 @@ def attn_weight_sums(q: torch.Tensor, k_nibbles: torch.Tensor, k_qjl: torch.Tens
             _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], _lib.ptr(k_nibbles), _lib.ptr(k_qjl), _lib.ptr(k_norms), _lib.ptr(cb), per_head,
             _lib.ptr(ids), uid, _lib.ptr(lens), B, Hq, Hkv, T, S, float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale),
             int(bool(with_qjl)), int(bool(rotate_q)), int(bool(causal)), int(into is not None), _lib.ptr(scratch), nbytes,
-            _lib.ptr(sums), _lib.stream_ptr(dev)))
+            _lib.ptr(sums), _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr(dev)))
     return sums
 
 

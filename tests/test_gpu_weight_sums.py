@@ -32,7 +32,8 @@ def check(got, q, rows, cb, ids, lens, with_qjl, causal, scale=SCALE, extra=0.0)
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("B,Hq,Hkv,T,S,lens", [(1, 1, 1, 1, 1, None), (2, 8, 2, 1, 300, [300, 17]), (3, 6, 3, 4, 140, [0, 2, 140]), (1, 4, 1, 9, 129, None),
-                                               (2, 10, 2, 1, 1025, [1025, 513]), (1, 3, 1, 32, 70, [33]), (2, 16, 1, 1, 64, None)])
+                                               (2, 10, 2, 1, 1025, [1025, 513]), (1, 3, 1, 32, 70, [33]), (2, 16, 1, 1, 64, None),
+                                               (1, 8, 1, 40, 700, [690]), (1, 4, 2, 20, 1300, None)])
 def test_against_definition(dtype, B, Hq, Hkv, T, S, lens):
     from omnistack_rs_b200.kernels.eviction import attn_weight_sums
     nib, qjl, norms, cb = packed(B, Hkv, S, seed=S + T)

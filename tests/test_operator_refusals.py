@@ -109,7 +109,7 @@ def test_c_entries_refuse_bad_arguments(lib):
     assert prompt(T=1 << 31) == _lib.ERR_UNSUPPORTED and prompt(T=0) == _lib.OK
     assert lib.omni_attn_weight_sums_workspace_bytes(0, 4, 2, 1, 100) == 0
     sums = lambda q=one, Hq=4, Hkv=2, S=64, ws=0: lib.omni_attn_weight_sums(  # noqa: E731
-        q, 1, one, one, one, one, 0, None, 0, None, 1, Hq, Hkv, 1, S, 1.0, 1, 0, 1, 0, one, ws, one, None)
+        q, 1, one, one, one, one, 0, None, 0, None, 1, Hq, Hkv, 1, S, 1.0, 1, 0, 1, 0, one, ws, one, None, None)
     assert sums(q=None) == sums(Hq=3) == sums(ws=0) == _lib.ERR_ARG and sums(S=0) == _lib.OK
     assert sums(Hq=2048, Hkv=2048) == _lib.ERR_UNSUPPORTED
     assert lib.omni_evict_keys(None, None) == _lib.ERR_ARG

@@ -126,6 +126,29 @@ template <> struct Elem<OMNI_F16> {
     static __device__ __forceinline__ float round(float x) { return __half2float(__float2half_rn(x)); }
 };
 
+// Load 8 consecutive elements of a row as fp32 (16-byte loads).
+template <int DT> __device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+    if constexpr (DT == OMNI_F32) {
+        const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+        const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (DT == OMNI_BF16) {
+                v[2 * k] = __uint_as_float(w[k] << 16);
+                v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+                v[2 * k] = f.x;
+                v[2 * k + 1] = f.y;
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ int seed_of(int32_t user_id, int head) { return ((user_id & 1023) ^ head) & 1023; }
 
 }  // namespace omni

@@ -16,28 +16,6 @@ constexpr int kPosThreads = 256;
 constexpr int kPosRows = kPosThreads / 16;         // sixteen-lane units per CTA
 constexpr int kPosUnroll = 4;                      // rows a unit has in flight
 
-template <int DT> __device__ __forceinline__ void pos_load8(const void* p, int64_t i, float (&v)[8]) {
-    if constexpr (DT == OMNI_F32) {
-        const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
-        const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if constexpr (DT == OMNI_BF16) {
-                v[2 * k] = __uint_as_float(w[k] << 16);
-                v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-            } else {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-                v[2 * k] = f.x;
-                v[2 * k + 1] = f.y;
-            }
-        }
-    }
-}
-
 template <int DT> __device__ __forceinline__ void pos_store8(void* p, int64_t i, const float (&v)[8]) {
     if constexpr (DT == OMNI_F32) {
         float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
@@ -64,11 +42,11 @@ __device__ __forceinline__ void pos_weight8(const void* w, int dtype, int i, flo
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = 1.f;
     } else if (dtype == OMNI_F32) {
-        pos_load8<OMNI_F32>(w, i, v);
+        load8<OMNI_F32>(w, i, v);
     } else if (dtype == OMNI_BF16) {
-        pos_load8<OMNI_BF16>(w, i, v);
+        load8<OMNI_BF16>(w, i, v);
     } else {
-        pos_load8<OMNI_F16>(w, i, v);
+        load8<OMNI_F16>(w, i, v);
     }
 }
 
@@ -135,7 +113,7 @@ __global__ void __launch_bounds__(kPosThreads) norm_rope_kernel(const __grid_con
         for (int r = 0; r < kPosUnroll; ++r) {
             const int h = h0 + r < h_end ? h0 + r : h_end - 1;
             const int s = h >= H0;
-            pos_load8<DT>(a.x[s], b * a.xs[s][0] + (int64_t)(h - (s ? H0 : 0)) * a.xs[s][1] + t * a.xs[s][2] + 8 * lane, v[r]);
+            load8<DT>(a.x[s], b * a.xs[s][0] + (int64_t)(h - (s ? H0 : 0)) * a.xs[s][1] + t * a.xs[s][2] + 8 * lane, v[r]);
         }
 #pragma unroll
         for (int r = 0; r < kPosUnroll; ++r) {

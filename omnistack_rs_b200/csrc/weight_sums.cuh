@@ -19,6 +19,8 @@ struct WeightArgs {
     float2* partial;                               // [B * Hkv][chunks][columns] maximum (base 2) and sum
     float* scores;                                 // warp-level kernel: [B * Hkv][S][columns, rounded up to even]
     int64_t chunk_keys, chunks;
+    int32_t* tiles_before;                         // tcgen05 kernel: [B + 1] tiles of one kv head in front of every user
+    void* prepared;                                // tcgen05 kernel: the columns, ready for tensor memory
     float* sums;
 };
 
@@ -32,13 +34,13 @@ __device__ __forceinline__ float ws_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// power of two that brings `top` into [8192, 16384); 1 for zero, infinite and NaN
+// power of two that brings `top` into [8192, 16384) (2^60 at most: products of two of them stay finite); 1 for zero, infinite, NaN
 __device__ __forceinline__ float ws_pow2(float top) {
     if (!(top > 0.f) || !(top < INFINITY)) return 1.f;
     int e;
     frexpf(top, &e);
     e = 14 - e;
-    return exp2f((float)(e > 120 ? 120 : e));
+    return exp2f((float)(e > 60 ? 60 : e));
 }
 __device__ __forceinline__ uint32_t ws_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);

@@ -1,23 +1,37 @@
 // Key weights of many columns (a prompt's last tokens): tcgen05 products in two passes over the keys.
 //
-// Query columns are the rows of the product (128 at a time), keys its columns:  S[col, key] = Q'[col, :] . K'[key, :].  Q' lives
-// in tensor memory for the whole CTA, K' is dequantised tile by tile (128 keys) into shared memory, twice: values and what they
+// Query columns are the rows of the product (128 at a time), keys its columns:  S[col, key] = Q'[col, :] . K'[key, :].  Q' is made
+// once by a launch of its own (rotation, scaling, G . q, fp16 values and remainders) and lives in tensor memory for a whole CTA, K' is dequantised tile by tile (128 keys) into shared memory, twice: values and what they
 // leave of the centroids, plus the signs.  Two accumulators, since a key's norm multiplies the sign product alone and would have to
 // be split as well to ride in it:   A = Qhi Khi + Qhi Klo (+ Qlo Khi),   B = Chi sign + Clo sign,   s = f_A A + f_B norm B.
 //
-// Pass 1: thread = column, running maximum and sum over the chunk's keys, one pair per (chunk, column) into the workspace.
+// The tiles of all (user, head) lie in one row, cut into equal shares, one per CTA: lengths differ, and only the device knows
+// them.  A run of tiles of one head inside a share is a span; span (head, CTA) is number head + CTA, which no other span has.
+// Pass 1: thread = column, running maximum and sum over a span's keys, one pair per (span, column) into the workspace.
 // Pass 2: the same scores again (cheaper than 4 bytes per key and column written and read), weights 2^(s - lse), and their sum over
 // the columns: a halving exchange between the lanes of a warp, then the four warps' parts in order.
 //
-// Warps 0-3: scores (thread = column).  Warps 4-7: dequantisation (thread = key), two buffers ahead of the products.  Warp 8
-// issues the products.  Shared memory is what bounds a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the
-// products' reads of K', about 1,900 cycles against 1,536 of the tensor pipe.
+// Warps 0-7: scores, two threads per column with 64 of a tile's keys each.  Warps 8-15: dequantisation, two threads per key, up to
+// two buffers ahead of the products.  Warp 16 issues the products.  (One thread per column and key left each scheduler two warps,
+// which issued an instruction every third cycle: 135 us for a pass of 16 users x 8,192 keys x 128 columns.)  Shared memory bounds
+// a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the products' reads of K', about 1,900 cycles against 1,536
+// of the tensor pipe.
 #include "weight_sums.cuh"
 
 namespace omni {
 
-constexpr int kWwThreads = 288;
 constexpr int kWwTile = 128;                       // keys per tile, columns per CTA
+constexpr int kWwThreads = 640;                    // warps 17-19 only complete the last warpgroup
+// Registers: launched with 96 per thread (61,440); scores go up to 144, dequantisation down to 72, the rest to 48
+// (256 * 144 + 256 * 72 + 128 * 48 = 61,440).
+constexpr int kWwScoreRegs = 144, kWwKeyRegs = 72, kWwOtherRegs = 48;
+// Prepared columns: per (head, 128 columns) 48 rows of 128 16-byte pieces -- 16 of Q' values, 16 of what they leave, 8 of G . q values,
+// 8 of what those leave -- and the columns' 128 score factors.
+constexpr int kWwPrepRows = 48;
+constexpr size_t kWwPrepBytes = (size_t)kWwPrepRows * kWwTile * 16 + kWwTile * 4;
+// G . q is at most 128 times the query's scaled maximum (below 2^14), so 2^-7 keeps it inside fp16, and the same factor for every
+// column lets it ride, with the coefficient and the table's factor, in the keys' norms.
+constexpr float kWwProjMul = 1.f / 128.f;
 constexpr uint32_t kWwLbo = 128;                   // K-major operands: bytes between the two 8-element chunks of a k-step
 constexpr uint32_t kWwSbo = 16 * 128, kWwSboSign = 8 * 128;         // ... and between groups of eight keys
 constexpr uint32_t kWwBytesV = 128 * 128 * 2, kWwBytesSign = 128 * 64 * 2;
@@ -63,7 +77,7 @@ __device__ __forceinline__ void ww_mma(uint32_t d, uint32_t a, uint32_t b, uint3
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
                  :: "r"(d), "r"(a), "l"(desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void ww_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+__device__ __forceinline__ void ww_ld32(uint32_t taddr, uint32_t* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
                  "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
@@ -81,6 +95,33 @@ __device__ __forceinline__ void ww_st32(uint32_t taddr, const uint32_t (&v)[32])
                     "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
                  : "memory");
 }
+__device__ __forceinline__ void ww_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+                 :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                    "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t ww_pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 ww_unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t ww_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t ww_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ void ww_sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" :: "r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -91,55 +132,160 @@ __device__ __forceinline__ uint2 ww_lut(uint32_t lut_lane, uint32_t w, int byte)
     return v;
 }
 
-template <int DT, bool QLO, int PASS>
+// A warp per column: rotation, power-of-two scaling, G . q, and all of it as fp16 values and remainders.
+constexpr int kWpWarps = 8;
+template <int DT>
+__global__ void __launch_bounds__(kWpWarps * 32) weight_prepare_kernel(const __grid_constant__ WeightArgs a, int64_t col_groups) {
+    __shared__ __align__(16) float q_s[kWpWarps][kHeadDim];
+    __shared__ uint4 g_s[kQjlDim];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (blockIdx.x == gridDim.x - 1) {                                   // tiles of one kv head in front of every user
+        __shared__ int part[kWpWarps];
+        int before = 0;
+        for (int64_t b0 = 0; b0 <= a.B; b0 += kWpWarps * 32) {
+            const int64_t b = b0 + tid;
+            const int n = b < a.B ? (ws_len(a, b) + kWwTile - 1) / kWwTile : 0;
+            int upto = n;
+#pragma unroll
+            for (int x = 1; x < 32; x <<= 1) {
+                const int o = __shfl_up_sync(kFullMask, upto, x);
+                if (lane >= x) upto += o;
+            }
+            if (lane == 31) part[warp] = upto;
+            __syncthreads();
+            int total = 0;
+#pragma unroll
+            for (int w = 0; w < kWpWarps; ++w) {
+                if (w < warp) upto += part[w];
+                total += part[w];
+            }
+            if (b <= a.B) a.tiles_before[b] = before + upto - n;
+            before += total;
+            __syncthreads();
+        }
+        return;
+    }
+    const int64_t bh = blockIdx.x / col_groups, b = bh / a.Hkv;
+    const int h = (int)(bh % a.Hkv), G = a.Hq / a.Hkv, cols = G * a.T;
+    const int col = (int)(blockIdx.x % col_groups) * kWpWarps + warp;
+    if (tid < kQjlDim && a.with_qjl) {
+        const int32_t uid = a.user_ids ? __ldg(a.user_ids + b) : a.user_id;
+        g_s[tid] = __ldg(reinterpret_cast<const uint4*>(a.g_rows + ((size_t)seed_of(uid, h) * kQjlDim + tid) * 4));
+    }
+    float q[4] = {0.f, 0.f, 0.f, 0.f};
+    if (col < cols) Elem<DT>::load4(a.q, ((b * a.Hq + (int64_t)h * G + col / a.T) * a.T + col % a.T) * kHeadDim + 4 * lane, q);
+    if (a.rotate_q) wht128_warp(q, lane);
+    float top = fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3])));
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, x));
+    // a negative scale goes into the queries, so that the largest product is the largest score
+    const float q_mul = copysignf(ws_pow2(top), a.scale);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { q[k] *= q_mul; q_s[warp][4 * lane + k] = q[k]; }
+    __syncthreads();
+    if (col >= cols) return;
+    unsigned char* out = reinterpret_cast<unsigned char*>(a.prepared) + (bh * ((cols + kWwTile - 1) / kWwTile) + col / kWwTile) * kWwPrepBytes;
+    const int c = col % kWwTile;
+    {
+        const uint32_t v0 = ws_half2(q[0], q[1]), v1 = ws_half2(q[2], q[3]);
+        const int piece = lane >> 1, at = (lane & 1) * 8;                 // two lanes fill a piece of eight halves
+        *reinterpret_cast<uint2*>(out + ((size_t)piece * kWwTile + c) * 16 + at) = make_uint2(v0, v1);
+        *reinterpret_cast<uint2*>(out + ((size_t)(16 + piece) * kWwTile + c) * 16 + at) = make_uint2(ws_rest2(q[0], q[1], v0), ws_rest2(q[2], q[3], v1));
+    }
+    if (a.with_qjl) {                                                    // projections 2 lane and 2 lane + 1
+        float p[2] = {0.f, 0.f};
+        const uint4 ga = g_s[2 * lane], gb = g_s[2 * lane + 1];
+        const uint32_t wa[4] = {ga.x, ga.y, ga.z, ga.w}, wb[4] = {gb.x, gb.y, gb.z, gb.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(&q_s[warp][32 * w + d]);
+                const float e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    p[0] += __uint_as_float(__float_as_uint(e[k]) ^ (((~wa[w] >> (d + k)) & 1u) << 31));
+                    p[1] += __uint_as_float(__float_as_uint(e[k]) ^ (((~wb[w] >> (d + k)) & 1u) << 31));
+                }
+            }
+        }
+        const float x = p[0] * kWwProjMul, y = p[1] * kWwProjMul;
+        const uint32_t v = ws_half2(x, y);
+        const int piece = 32 + (lane >> 2), at = (lane & 3) * 4;
+        *reinterpret_cast<uint32_t*>(out + ((size_t)piece * kWwTile + c) * 16 + at) = v;
+        *reinterpret_cast<uint32_t*>(out + ((size_t)(8 + piece) * kWwTile + c) * 16 + at) = ws_rest2(x, y, v);
+    }
+    if (lane == 0) {
+        float cb_top = 0.f;
+        const float* cb = a.codebooks + (a.cb_per_head ? h * 16 : 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) cb_top = fmaxf(cb_top, fabsf(__ldg(cb + i)));
+        // never zero: zero times a masked score's -inf is NaN
+        reinterpret_cast<float*>(out + (size_t)kWwPrepRows * kWwTile * 16)[c] = fmaxf(a.scale * kWsLog2e / q_mul / ws_pow2(cb_top), 1e-30f);
+    }
+}
+
+// Position in the row of tiles: user, kv head, tile of that head.  Users without keys have no place in it.
+struct WwPlace {
+    int b, h, tile, len, n_tiles;                     // the user's length and its tiles per head
+    __device__ __forceinline__ void user(const WeightArgs& a) { len = ws_len(a, b); n_tiles = (len + kWwTile - 1) / kWwTile; }
+    // the place of tile x, by a warp
+    __device__ __forceinline__ void find(const WeightArgs& a, int64_t x, int lane) {
+        int64_t lo = 0, n = a.B;                   // the last user with at most x tiles in front of it lies in [lo, lo + n)
+        while (n > 1) {
+            const int64_t step = (n + 31) / 32, i = lo + lane * step;
+            const bool below = lane == 0 || (i < lo + n && (int64_t)__ldg(a.tiles_before + i) * a.Hkv <= x);
+            const int64_t next = lo + (31 - __clz((int)__ballot_sync(kFullMask, below))) * step;
+            n = lo + n - next < step ? lo + n - next : step;
+            lo = next;
+        }
+        b = (int)lo;
+        user(a);
+        const int64_t in = x - (int64_t)__ldg(a.tiles_before + b) * a.Hkv;
+        h = (int)(in / n_tiles);
+        tile = (int)(in % n_tiles);
+    }
+    // behind the last tile of this head
+    __device__ __forceinline__ void next_head(const WeightArgs& a) {
+        tile = 0;
+        if (++h < a.Hkv) return;
+        h = 0;
+        do { ++b; user(a); } while (n_tiles == 0);
+    }
+};
+
+template <bool QLO, int PASS>
 __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __grid_constant__ WeightArgs a, int col0, int32_t* status) {
     extern __shared__ __align__(1024) unsigned char ww_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t bh = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, b = bh / a.Hkv;
-    const int h = (int)(bh % a.Hkv), G = a.Hq / a.Hkv, cols = G * a.T;
-    const int len = ws_len(a, b);
-    const int64_t k_begin64 = chunk * a.chunk_keys;
-    float* sums = a.sums + bh * a.S;
-    if (k_begin64 >= len) {                                              // nothing but zeros, if anything
-        if (PASS == 2 && !a.accumulate && col0 == 0)
-            for (int64_t s = k_begin64 + tid; s < a.S && s < k_begin64 + a.chunk_keys; s += kWwThreads) sums[s] = 0.f;
-        return;
+    const int cols = a.Hq / a.Hkv * a.T;
+    if (PASS == 2 && !a.accumulate && col0 == 0) {                       // zeros behind the lengths
+        for (int64_t bh = blockIdx.x; bh < a.B * a.Hkv; bh += gridDim.x)
+            for (int64_t s = ws_len(a, bh / a.Hkv) + tid; s < a.S; s += kWwThreads) a.sums[bh * a.S + s] = 0.f;
     }
-    const int k_begin = (int)k_begin64;
-    const int k_end = len - k_begin < a.chunk_keys ? len : k_begin + (int)a.chunk_keys;
-    const int n_tiles = (k_end - k_begin + kWwTile - 1) / kWwTile;
+    const int64_t all = (int64_t)__ldg(a.tiles_before + a.B) * a.Hkv;    // this CTA's share: tiles x0 .. x1 - 1
+    const int64_t x0 = blockIdx.x * all / gridDim.x, x1 = (blockIdx.x + 1) * all / gridDim.x;
+    const int n_share = (int)(x1 - x0);
+    if (n_share <= 0) return;
+    WwPlace at;
+    at.find(a, x0, lane);
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(ww_smem);
     float* norm_s = reinterpret_cast<float*>(ww_smem + kWwOffNorm);      // ring of four tiles' norms
     float* red_s = reinterpret_cast<float*>(ww_smem + kWwOffRed);
-    const uint32_t bar_full = base + kWwOffBar, bar_empty = bar_full + 16, bar_s = bar_empty + 16, bar_free = bar_s + 8, tmem_at = bar_free + 8;
+    const uint32_t bar_full = base + kWwOffBar, bar_empty = bar_full + 16, bar_s = bar_empty + 16, bar_free = bar_s + 16, bar_q = bar_free + 16, tmem_at = bar_q + 8;
     if (tid == 0) {
+        ww_bar_init(bar_q, 8);
         for (int i = 0; i < 2; ++i) {
-            ww_bar_init(bar_full + 8 * i, 4);
+            ww_bar_init(bar_full + 8 * i, 8);
             ww_bar_init(bar_empty + 8 * i, 1);
+            ww_bar_init(bar_s + 8 * i, 1);                               // scores of keys 0-63 and 64-127 of a tile: by halves, so that the
+            ww_bar_init(bar_free + 8 * i, 4);                            // products of one go on while the other's are taken out
         }
-        ww_bar_init(bar_s, 1);
-        ww_bar_init(bar_free, 4);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" :: "r"(tmem_at), "r"(kWwTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
-    }
-    const float cb_mul = ws_build_lut(ww_smem + kWwOffLut, a.codebooks + (a.cb_per_head ? h * 16 : 0), tid);
-    if (a.with_qjl && warp >= 4 && warp < 8) {                           // G as +-1, [64 projections][128 dims], where the first values will go
-        const int32_t uid = a.user_ids ? __ldg(a.user_ids + b) : a.user_id;
-        const int pi = (tid - 128) >> 1, half = tid & 1;                 // projection, and which 64 of its 128 dims
-        const uint32_t* gr = a.g_rows + ((size_t)seed_of(uid, h) * kQjlDim + pi) * 4 + 2 * half;
-        const uint32_t row = base + (uint32_t)(pi >> 3) * kWwSbo + (uint32_t)(pi & 7) * 16 + (uint32_t)half * 8 * kWwLbo;
-#pragma unroll
-        for (int wd = 0; wd < 2; ++wd) {
-            const uint32_t bits = __ldg(gr + wd);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                ww_sts16(row + (uint32_t)(4 * wd + k) * kWwLbo, ws_signs2(bits >> (8 * k)), ws_signs2(bits >> (8 * k + 2)), ws_signs2(bits >> (8 * k + 4)),
-                         ws_signs2(bits >> (8 * k + 6)));
-        }
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     }
     ww_fence_before();
     __syncthreads();
@@ -147,153 +293,84 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(tmem) : "r"(tmem_at));
     const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const int col = col0 + tid;                                          // of warps 0-3
-    const bool col_on = warp < 4 && col < cols;
-    float q_mul = 1.f, p_mul = 1.f;
-
-    // ---- Q' into tensor memory -----------------------------------------------------------------------------------------
-    if (warp < 4) {
-        float q[128];
-        const int64_t qrow = col_on ? (b * a.Hq + (int64_t)h * G + col / a.T) * a.T + col % a.T : 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (col_on) Elem<DT>::load4(a.q, qrow * kHeadDim + 4 * i, v);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) q[4 * i + k] = v[k];
-        }
-        if (a.rotate_q) {                                                // Walsh-Hadamard, stages in order, one rounding each
-#pragma unroll
-            for (int s = 1; s < 128; s <<= 1) {
-#pragma unroll
-                for (int i = 0; i < 128; ++i) {
-                    if ((i & s) == 0) {
-                        const float x = q[i], y = q[i | s];
-                        q[i] = __fadd_rn(x, y);
-                        q[i | s] = __fsub_rn(x, y);
-                    }
-                }
-            }
-            const float s = __uint_as_float(OMNI_WHT_SCALE_BITS);
-#pragma unroll
-            for (int i = 0; i < 128; ++i) q[i] = __fmul_rn(q[i], s);
-        }
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) top = fmaxf(top, fabsf(q[i]));
-        q_mul = ws_pow2(top);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            uint32_t v[32], r[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float x = q[64 * j + 2 * i] * q_mul, y = q[64 * j + 2 * i + 1] * q_mul;
-                v[i] = ws_half2(x, y);
-                if (QLO) r[i] = ws_rest2(x, y, v[i]);
-            }
-            ww_st32(t_lane + kWwColQhi + 32 * j, v);
-            if (QLO) ww_st32(t_lane + kWwColQlo + 32 * j, r);
-        }
-        ww_wait_st();
-        ww_fence_before();
-    }
+    const int half = (warp >> 2) & 1;                                    // which half of a column's keys, of a key's dims
+    const int row = tid & 127;
     bool ok = true;
-    uint32_t ph_s = 0;                                                   // parity of the next completion of bar_s
-    if (a.with_qjl) {                                                    // C = G . q, then split like the centroids
-        __syncthreads();
-        if (warp == 8) {
-            ww_fence_after();
-            if (ww_elect()) {
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tmem + kWwColQhi + 8 * ks, base + ks * 2 * kWwLbo, kWwSbo, 64, ks > 0);
-                if (QLO) {
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tmem + kWwColQlo + 8 * ks, base + ks * 2 * kWwLbo, kWwSbo, 64, 1);
-                }
-                ww_commit(bar_s);
-            }
-            __syncwarp();
-        }
-        ok = ww_bar_wait(bar_s, 0);                                      // G's buffer may be overwritten from here on
-        ph_s = 1;
-        if (ok && warp < 4) {
-            ww_fence_after();
-            uint32_t p[2][32], v[32], r[32];
-            ww_ld32(t_lane + kWwColA, p[0]);
-            ww_ld32(t_lane + kWwColA + 32, p[1]);
-            ww_wait_ld();
-            float top = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(p[0][i])), fabsf(__uint_as_float(p[1][i]))));
-            p_mul = ws_pow2(top);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float x = __uint_as_float(p[i >> 4][2 * (i & 15)]) * p_mul, y = __uint_as_float(p[i >> 4][2 * (i & 15) + 1]) * p_mul;
-                v[i] = ws_half2(x, y);
-                r[i] = ws_rest2(x, y, v[i]);
-            }
-            ww_st32(t_lane + kWwColChi, v);
-            ww_st32(t_lane + kWwColClo, r);
-            ww_wait_st();
-            ww_fence_before();
-        }
-    }
-    ok = __syncthreads_and(ok) != 0;                                     // Q' and C are complete
 
-    if (ok && warp == 8) {
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" :: "n"(kWwOtherRegs));
         // ---- products ---------------------------------------------------------------------------------------------------
-        ww_fence_after();
-        for (int t = 0; ok && t < n_tiles; ++t) {
+        int span_end = 0, spans = 0;
+        for (int t = 0; warp == 16 && ok && t < n_share; ++t) {
+            if (t == span_end) {                                         // another head's columns
+                ok = ww_bar_wait(bar_q, spans++ & 1);
+                if (!ok) break;
+                span_end += at.n_tiles - at.tile;
+                if (span_end < n_share) at.next_head(a);
+            }
             const uint32_t kv = base + (t & 1) * kWwBuf;
             ok = ww_bar_wait(bar_full + 8 * (t & 1), (t >> 1) & 1);
-            if (ok && t > 0) ok = ww_bar_wait(bar_free, (t - 1) & 1);
-            if (!ok) break;
-            ww_fence_after();
-            if (ww_elect()) {
+#pragma unroll 1
+            for (int x = 0; ok && x < 2; ++x) {
+                if (t > 0) ok = ww_bar_wait(bar_free + 8 * x, (t - 1) & 1);
+                if (!ok) break;
+                ww_fence_after();
+                if (ww_elect()) {
+                    const uint32_t kx = kv + x * 8 * kWwSbo, sx = kv + 2 * kWwBytesV + x * 8 * kWwSboSign, da = tmem + kWwColA + 64 * x, db = tmem + kWwColB + 64 * x;
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tmem + kWwColQhi + 8 * ks, kv + ks * 2 * kWwLbo, kWwSbo, 128, ks > 0);
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, ks > 0);
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tmem + kWwColQhi + 8 * ks, kv + kWwBytesV + ks * 2 * kWwLbo, kWwSbo, 128, 1);
-                if (QLO) {
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + kWwBytesV + ks * 2 * kWwLbo, kWwSbo, 64, 1);
+                    if (QLO) {
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tmem + kWwColQlo + 8 * ks, kv + ks * 2 * kWwLbo, kWwSbo, 128, 1);
+                        for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQlo + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, 1);
+                    }
+                    if (a.with_qjl) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColChi + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, ks > 0);
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColClo + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, 1);
+                    }
+                    if (x == 1) ww_commit(bar_empty + 8 * (t & 1));
+                    ww_commit(bar_s + 8 * x);
                 }
-                if (a.with_qjl) {
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) ww_mma(tmem + kWwColB, tmem + kWwColChi + 8 * ks, kv + 2 * kWwBytesV + ks * 2 * kWwLbo, kWwSboSign, 128, ks > 0);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) ww_mma(tmem + kWwColB, tmem + kWwColClo + 8 * ks, kv + 2 * kWwBytesV + ks * 2 * kWwLbo, kWwSboSign, 128, 1);
-                }
-                ww_commit(bar_empty + 8 * (t & 1));
-                ww_commit(bar_s);
+                __syncwarp();
             }
-            __syncwarp();
         }
-    } else if (ok && warp >= 4) {
-        // ---- dequantisation: thread = key ---------------------------------------------------------------------------------
-        const int x = tid - 128;
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" :: "n"(kWwKeyRegs));
+        // ---- dequantisation: 64 dims of key x and 32 of its signs per thread --------------------------------------------------
+        const int x = row;
         const uint32_t lut_lane = base + kWwOffLut + 8 * (lane & 15);
-        const uint32_t at = (uint32_t)(x >> 3) * kWwSbo + (uint32_t)(x & 7) * 16, at_sign = 2 * kWwBytesV + (uint32_t)(x >> 3) * kWwSboSign + (uint32_t)(x & 7) * 16;
-        uint4 nib[4];
-        uint2 sign = make_uint2(0u, 0u);
+        const uint32_t row_at = (uint32_t)(x >> 3) * kWwSbo + (uint32_t)(x & 7) * 16 + 8 * half * kWwLbo;
+        const uint32_t sign_at = 2 * kWwBytesV + (uint32_t)(x >> 3) * kWwSboSign + (uint32_t)(x & 7) * 16 + 4 * half * kWwLbo;
+        float norm_mul = 1.f;                                            // the sign product in units of the value product
+        uint4 nib[2];
+        uint32_t sign = 0;
         float norm = 0.f;
-        auto fetch = [&](int t) {                                        // keys past the end repeat the last one
-            const int k = k_begin + t * kWwTile + x;
-            const int64_t row = bh * a.S + (k < k_end ? k : k_end - 1);
+        auto fetch = [&]() {                                             // keys past the end repeat the last one
+            const int k = at.tile * kWwTile + x;
+            const int64_t r = ((int64_t)at.b * a.Hkv + at.h) * a.S + (k < at.len ? k : at.len - 1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) nib[i] = __ldg(reinterpret_cast<const uint4*>(a.k_nib + row * kNibBytes) + i);
+            for (int i = 0; i < 2; ++i) nib[i] = __ldg(reinterpret_cast<const uint4*>(a.k_nib + r * kNibBytes) + 2 * half + i);
             if (a.with_qjl) {
-                sign = __ldg(reinterpret_cast<const uint2*>(a.k_qjl + row * kQjlBytes));
-                norm = __ldg(a.k_norms + row);
+                sign = __ldg(reinterpret_cast<const uint32_t*>(a.k_qjl + r * kQjlBytes) + half);
+                norm = __ldg(a.k_norms + r);
             }
         };
-        fetch(0);
-        for (int t = 0; t < n_tiles; ++t) {
-            if (t > 1) ok = ww_bar_wait(bar_empty + 8 * (t & 1), ((t >> 1) - 1) & 1);
-            if (!ok) break;
+        fetch();
+        bool new_table = true;
+        for (int t = 0; t < n_share; ++t) {
+            if (new_table) {                                             // no lookup of the previous table is still to come
+                asm volatile("bar.sync 2, 256;\n" ::: "memory");
+                norm_mul = kQjlCoef / kWwProjMul * ws_build_lut(ww_smem + kWwOffLut, a.codebooks + (a.cb_per_head ? at.h * 16 : 0), tid - 256);
+                asm volatile("bar.sync 2, 256;\n" ::: "memory");
+            }
+            if (ok && t > 1) ok = ww_bar_wait(bar_empty + 8 * (t & 1), ((t >> 1) - 1) & 1);
+            // (a warp whose wait ran out stays for the barriers of the others and leaves behind the loop)
             const uint32_t kv = base + (t & 1) * kWwBuf;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {                                // sixteen lookups, then their eight stores
+            for (int i = 0; i < 2; ++i) {                                // sixteen lookups, then their eight stores
                 const uint32_t w[4] = {nib[i].x, nib[i].y, nib[i].z, nib[i].w};
                 uint2 v[4][4];
 #pragma unroll
@@ -303,143 +380,227 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    ww_sts16(kv + at + (uint32_t)(4 * i + j) * kWwLbo, v[j][0].x, v[j][1].x, v[j][2].x, v[j][3].x);
-                    ww_sts16(kv + kWwBytesV + at + (uint32_t)(4 * i + j) * kWwLbo, v[j][0].y, v[j][1].y, v[j][2].y, v[j][3].y);
+                    ww_sts16(kv + row_at + (uint32_t)(4 * i + j) * kWwLbo, v[j][0].x, v[j][1].x, v[j][2].x, v[j][3].x);
+                    ww_sts16(kv + kWwBytesV + row_at + (uint32_t)(4 * i + j) * kWwLbo, v[j][0].y, v[j][1].y, v[j][2].y, v[j][3].y);
                 }
             }
             if (a.with_qjl) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t bits = (i < 4 ? sign.x : sign.y) >> (8 * (i & 3));
-                    ww_sts16(kv + at_sign + (uint32_t)i * kWwLbo, ws_signs2(bits), ws_signs2(bits >> 2), ws_signs2(bits >> 4), ws_signs2(bits >> 6));
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t bits = sign >> (8 * i);
+                    ww_sts16(kv + sign_at + (uint32_t)i * kWwLbo, ws_signs2(bits), ws_signs2(bits >> 2), ws_signs2(bits >> 4), ws_signs2(bits >> 6));
                 }
             }
-            norm_s[(t & 3) * kWwTile + x] = norm;
-            if (t + 1 < n_tiles) fetch(t + 1);
+            if (half == 0) norm_s[(t & 3) * kWwTile + x] = norm * norm_mul;
+            if (t + 1 < n_share) {
+                const int h = at.h;
+                if (++at.tile == at.n_tiles) at.next_head(a);
+                new_table = a.cb_per_head && at.h != h;
+                fetch();
+            }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) ww_bar_arrive(bar_full + 8 * (t & 1));
         }
-    } else if (ok) {
-        // ---- scores: thread = column ------------------------------------------------------------------------------------
-        const float f_a = a.scale * kWsLog2e / q_mul / cb_mul, f_b = a.with_qjl ? a.scale * kWsLog2e * kQjlCoef / q_mul / p_mul : 0.f;
-        const int last = col_on ? (a.causal ? len - a.T + col % a.T : len - 1) : -1;    // newest key of the column
-        const int open_to = a.causal ? len - a.T : len - 1;              // newest key that every column sees
-        float m = -INFINITY, l = 0.f, lse = 0.f;
-        if (PASS == 2 && col_on) {
-            const int n = (int)((len + a.chunk_keys - 1) / a.chunk_keys);
-            const float2* p = a.partial + bh * a.chunks * cols + col;
-            for (int i = 0; i < n; ++i) m = fmaxf(m, p[(int64_t)i * cols].x);
-            const float ref = m == -INFINITY ? 0.f : m;
-            for (int i = 0; i < n; ++i) l += p[(int64_t)i * cols].y * exp2f(p[(int64_t)i * cols].x - ref);
-            lse = m == -INFINITY && l == 0.f ? 0.f : ref + log2f(l);     // no open key: its scores are -inf
-        }
-        for (int t = 0; t < n_tiles; ++t) {
-            // after a wait that ran out the warp still goes through the barriers it shares with the others, storing nothing
-            if (ok) ok = ww_bar_wait(bar_s, (ph_s + t) & 1);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" :: "n"(kWwScoreRegs));
+        // ---- scores: 64 keys of a tile per thread -----------------------------------------------------------------------------
+        const int col = col0 + row;
+        const bool col_on = col < cols;
+        int done = 0;                                                    // tiles behind this one
+        while (done < n_share) {
+            const int64_t bh = (int64_t)at.b * a.Hkv + at.h;
+            const int len = at.len;
+            const int n_span = at.n_tiles - at.tile < n_share - done ? at.n_tiles - at.tile : n_share - done;
+            float* sums = a.sums + bh * a.S;
+            const unsigned char* prep = reinterpret_cast<const unsigned char*>(a.prepared) + (bh * ((cols + kWwTile - 1) / kWwTile) + col0 / kWwTile) * kWwPrepBytes;
+            const float f = col_on ? __ldg(reinterpret_cast<const float*>(prep + (size_t)kWwPrepRows * kWwTile * 16) + row) : 1.f;
+            // Q' of the columns into tensor memory, half of each part per thread, once no product of the previous span reads it
+            if (ok && done > 0) ok = ww_bar_wait(bar_empty + 8 * ((done - 1) & 1), ((done - 1) >> 1) & 1);
             ww_fence_after();
-            const float* nrm = norm_s + (t & 3) * kWwTile;
-            float s[128];
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(prep) + row;
+                auto piece = [&](int r, uint32_t* dst) {
+                    const uint4 x = col_on ? __ldg(src + (size_t)r * kWwTile) : make_uint4(0u, 0u, 0u, 0u);
+                    dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w;
+                };
+                uint32_t v[32], r[32], p[16], o[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t u[32], v[32];
-                ww_ld32(t_lane + kWwColA + 32 * j, u);
-                if (a.with_qjl) ww_ld32(t_lane + kWwColB + 32 * j, v);
-                ww_wait_ld();
+                for (int i = 0; i < 8; ++i) piece(8 * half + i, v + 4 * i);
+                if (QLO) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[32 * j + i] = __uint_as_float(u[i]) * f_a;
+                    for (int i = 0; i < 8; ++i) piece(16 + 8 * half + i, r + 4 * i);
+                }
                 if (a.with_qjl) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 n4 = *reinterpret_cast<const float4*>(nrm + 32 * j + i);
-                        s[32 * j + i] = fmaf(__uint_as_float(v[i]) * f_b, n4.x, s[32 * j + i]);
-                        s[32 * j + i + 1] = fmaf(__uint_as_float(v[i + 1]) * f_b, n4.y, s[32 * j + i + 1]);
-                        s[32 * j + i + 2] = fmaf(__uint_as_float(v[i + 2]) * f_b, n4.z, s[32 * j + i + 2]);
-                        s[32 * j + i + 3] = fmaf(__uint_as_float(v[i + 3]) * f_b, n4.w, s[32 * j + i + 3]);
-                    }
+                    for (int i = 0; i < 4; ++i) { piece(32 + 4 * half + i, p + 4 * i); piece(40 + 4 * half + i, o + 4 * i); }
                 }
+                ww_st32(t_lane + kWwColQhi + 32 * half, v);
+                if (QLO) ww_st32(t_lane + kWwColQlo + 32 * half, r);
+                if (a.with_qjl) {
+                    ww_st16(t_lane + kWwColChi + 16 * half, p);
+                    ww_st16(t_lane + kWwColClo + 16 * half, o);
+                }
+                ww_wait_st();
+                ww_fence_before();
+                __syncwarp();
+                if (lane == 0) ww_bar_arrive(bar_q);
             }
-            ww_fence_before();
-            __syncwarp();
-            if (lane == 0) ww_bar_arrive(bar_free);                      // the accumulators may be overwritten
-            const int k0 = k_begin + t * kWwTile;
-            if (k0 + kWwTile - 1 > open_to || k0 + kWwTile > k_end || cols - col0 < kWwTile) {
-                const int lim = (last < k_end - 1 ? last : k_end - 1) - k0;
-#pragma unroll
-                for (int i = 0; i < 128; ++i) s[i] = i <= lim ? s[i] : -INFINITY;
+            const int last = col_on ? (a.causal ? len - a.T + col % a.T : len - 1) : -1;    // newest key of the column
+            const int open_to = a.causal ? len - a.T : len - 1;          // newest key that every column sees
+            float m = -INFINITY, l = 0.f, lse = 0.f;
+            if (PASS == 2 && col_on) {
+                // the head's spans: the CTAs whose shares hold its first and its last tile, and those between
+                const int64_t first = ((int64_t)__ldg(a.tiles_before + at.b)) * a.Hkv + (int64_t)at.h * at.n_tiles;
+                const int64_t c0 = ((first + 1) * gridDim.x + all - 1) / all - 1, c1 = ((first + at.n_tiles) * gridDim.x + all - 1) / all - 1;
+                const float2* p = a.partial + (bh + c0) * cols + col;
+                for (int64_t i = 0; i <= c1 - c0; ++i) m = fmaxf(m, p[i * cols].x);
+                const float ref = m == -INFINITY ? 0.f : m;
+                for (int64_t i = 0; i <= c1 - c0; ++i) l += p[i * cols].y * exp2f(p[i * cols].x - ref);
+                lse = m == -INFINITY && l == 0.f ? 0.f : ref + log2f(l); // no open key: its scores are -inf
             }
-            if (PASS == 1) {
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int t = done; t < done + n_span; ++t) {
+                // after a wait that ran out the warp still goes through the barriers it shares with the others, storing nothing
+                if (ok) ok = ww_bar_wait(bar_s + 8 * half, t & 1);
+                ww_fence_after();
+                uint32_t s[64];                                          // products of the values, then the scores / f
+                ww_ld32(t_lane + kWwColA + 64 * half, s);
+                ww_ld32(t_lane + kWwColA + 64 * half + 32, s + 32);
+                if (a.with_qjl) {
+                    const float* nrm = norm_s + (t & 3) * kWwTile + 64 * half;
 #pragma unroll
-                for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-                const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-                const float ref = m_new == -INFINITY ? 0.f : m_new;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t v[32];                                  // products of the signs
+                        ww_ld32(t_lane + kWwColB + 64 * half + 32 * j, v);
+                        ww_wait_ld();
+                        if (j == 1) {
+                            ww_fence_before();
+                            __syncwarp();
+                            if (lane == 0) ww_bar_arrive(bar_free + 8 * half);   // the accumulators may be overwritten
+                        }
 #pragma unroll
-                for (int i = 0; i < 128; ++i) sum[i & 3] += ws_ex2(s[i] - ref);
-                l = fmaf(l, ws_ex2(m - ref), (sum[0] + sum[1]) + (sum[2] + sum[3]));
-                m = m_new;
-            } else {
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 n4 = *reinterpret_cast<const float4*>(nrm + 32 * j + i);
 #pragma unroll
-                for (int i = 0; i < 128; ++i) s[i] = ws_ex2(s[i] - lse);
-                // sum over the warp's 32 columns: lanes trade halves of their keys until each has the total of four
-#pragma unroll
-                for (int n = 64, x = 16; n >= 4; n >>= 1, x >>= 1) {
-                    const bool up = (lane & x) != 0;
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        if (i < n) {
-                            const float mine = up ? s[i + n] : s[i], other = up ? s[i] : s[i + n];
-                            s[i] = mine + __shfl_xor_sync(kFullMask, other, x);
+                            for (int k = 0; k < 4; k += 2) {
+                                uint32_t* d = s + 32 * j + i + k;
+                                const float2 r = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(v[i + k]), __uint_as_float(v[i + k + 1])),
+                                                                    k ? ww_pack2(n4.z, n4.w) : ww_pack2(n4.x, n4.y),
+                                                                    ww_pack2(__uint_as_float(d[0]), __uint_as_float(d[1]))));
+                                d[0] = __float_as_uint(r.x);
+                                d[1] = __float_as_uint(r.y);
+                            }
                         }
                     }
+                } else {
+                    ww_wait_ld();
+                    ww_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ww_bar_arrive(bar_free + 8 * half);
                 }
-                *reinterpret_cast<float4*>(red_s + warp * kWwTile + 4 * lane) = make_float4(s[0], s[1], s[2], s[3]);
-                asm volatile("bar.sync 1, 128;\n" ::: "memory");
-                const float total = (red_s[tid] + red_s[kWwTile + tid]) + (red_s[2 * kWwTile + tid] + red_s[3 * kWwTile + tid]);
-                if (ok && k0 + tid < k_end) {
-                    if (a.accumulate || col0 > 0) sums[k0 + tid] += total;
-                    else sums[k0 + tid] = total;
+                const int k0 = (at.tile + t - done) * kWwTile;
+                if (k0 + kWwTile - 1 > open_to || k0 + kWwTile > len || cols - col0 < kWwTile) {
+                    const int lim = (last < len - 1 ? last : len - 1) - k0 - 64 * half;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) s[i] = i <= lim ? s[i] : 0xff800000u;
                 }
-                asm volatile("bar.sync 1, 128;\n" ::: "memory");
+                if (PASS == 1) {
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const float m_new = fmaxf(m, top * f);
+                    const float ref = m_new == -INFINITY ? 0.f : m_new;
+                    const uint64_t f2 = ww_pack2(f, f), r2 = ww_pack2(-ref, -ref);
+                    uint64_t sum[2] = {ww_pack2(0.f, 0.f), ww_pack2(0.f, 0.f)};
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, r2));
+                        sum[(i >> 1) & 1] = ww_add2(sum[(i >> 1) & 1], ww_pack2(ws_ex2(e.x), ws_ex2(e.y)));
+                    }
+                    const float2 total = ww_unpack2(ww_add2(sum[0], sum[1]));
+                    l = fmaf(l, ws_ex2(m - ref), total.x + total.y);
+                    m = m_new;
+                } else {
+                    float p[64];
+                    const uint64_t f2 = ww_pack2(f, f), r2 = ww_pack2(-lse, -lse);
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, r2));
+                        p[i] = ws_ex2(e.x);
+                        p[i + 1] = ws_ex2(e.y);
+                    }
+                    // sum over the warp's 32 columns: lanes trade halves of their keys until each has the totals of two
+#pragma unroll
+                    for (int n = 32, x = 16; n >= 2; n >>= 1, x >>= 1) {
+                        const bool up = (lane & x) != 0;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (i < n) {
+                                const float mine = up ? p[i + n] : p[i], other = up ? p[i] : p[i + n];
+                                p[i] = mine + __shfl_xor_sync(kFullMask, other, x);
+                            }
+                        }
+                    }
+                    float* red = red_s + 64 * half;                          // [four warps of a half][128 keys]
+                    *reinterpret_cast<float2*>(red + (warp & 3) * kWwTile + 2 * lane) = make_float2(p[0], p[1]);
+                    asm volatile("bar.sync 1, 256;\n" ::: "memory");
+                    if (tid < kWwTile) {
+                        const float total = (red_s[tid] + red_s[kWwTile + tid]) + (red_s[2 * kWwTile + tid] + red_s[3 * kWwTile + tid]);
+                        if (ok && k0 + tid < len) {
+                            if (a.accumulate || col0 > 0) sums[k0 + tid] += total;
+                            else sums[k0 + tid] = total;
+                        }
+                    }
+                    asm volatile("bar.sync 1, 256;\n" ::: "memory");
+                }
             }
+            if (PASS == 1) {                                             // the column's halves
+                float2* hand = reinterpret_cast<float2*>(red_s);
+                if (half == 1) hand[row] = make_float2(m, l);
+                asm volatile("bar.sync 1, 256;\n" ::: "memory");
+                if (half == 0 && ok && col_on) {
+                    const float2 o = hand[row];
+                    const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.f : top;
+                    a.partial[(bh + blockIdx.x) * cols + col] = make_float2(top, l * ws_ex2(m - ref) + o.y * ws_ex2(o.x - ref));
+                }
+                asm volatile("bar.sync 1, 256;\n" ::: "memory");
+            }
+            done += n_span;
+            if (done < n_share) at.next_head(a);
         }
-        if (PASS == 1 && ok && col_on) a.partial[(bh * a.chunks + chunk) * cols + col] = make_float2(m, l);
-        if (PASS == 2 && !a.accumulate && col0 == 0)                     // the rest of the chunk lies behind the length
-            for (int64_t s = k_end + tid; s < a.S && s < k_begin64 + a.chunk_keys; s += 128) sums[s] = 0.f;
     }
     if (!ok && status) atomicExch(status, OMNI_STATUS_WAIT_EXPIRED);
     __syncwarp();
     ww_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         ww_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" :: "r"(tmem), "r"(kWwTmemCols) : "memory");
     }
 }
 
-// Keys of a chunk: about three rounds of one CTA per SM, at least 512 (a CTA's prologue costs about as much as two tiles)
-static int64_t ww_chunk_keys(int64_t heads, int64_t S) {
-    const int64_t per = (heads * S + 148 * 3 - 1) / (148 * 3);
-    const int64_t keys = per < 512 ? 512 : (per > 8192 ? 8192 : per);
-    return (keys + kWwTile - 1) / kWwTile * kWwTile;
+// The CTAs of a call: one per SM, or one per tile where there are fewer
+static int64_t ww_ctas(int64_t heads, int64_t S) {
+    const int64_t tiles = heads * ((S + kWwTile - 1) / kWwTile);
+    return tiles < 148 ? tiles : 148;
 }
+static size_t ww_before_bytes(int64_t B) { return ((size_t)(B + 1) * 4 + 15) & ~(size_t)15; }
 
 size_t weight_window_workspace(int64_t B, int Hq, int Hkv, int T, int64_t S) {
-    const int64_t keys = ww_chunk_keys(B * Hkv, S);
-    return (size_t)B * Hq * T * ((S + keys - 1) / keys) * sizeof(float2);
+    const int64_t heads = B * Hkv, cols = (int64_t)(Hq / Hkv) * T, col_tiles = (cols + kWwTile - 1) / kWwTile;
+    return (size_t)(heads * col_tiles) * kWwPrepBytes + ww_before_bytes(B) + (size_t)(heads + ww_ctas(heads, S)) * cols * sizeof(float2);
 }
 
-template <int DT, bool QLO>
-static int32_t launch_weight_window_t(const WeightArgs& a, int32_t* status, cudaStream_t st) {
+template <bool QLO>
+static int32_t launch_weight_window_t(const WeightArgs& a, unsigned grid, int32_t* status, cudaStream_t st) {
     const int cols = a.Hq / a.Hkv * a.T;
-    const unsigned grid = (unsigned)(a.B * a.Hkv * a.chunks);
-    OMNI_CUDA(cudaFuncSetAttribute(weight_window_kernel<DT, QLO, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWwSmem));
-    OMNI_CUDA(cudaFuncSetAttribute(weight_window_kernel<DT, QLO, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWwSmem));
+    OMNI_CUDA(cudaFuncSetAttribute(weight_window_kernel<QLO, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWwSmem));
+    OMNI_CUDA(cudaFuncSetAttribute(weight_window_kernel<QLO, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWwSmem));
     for (int pass = 1; pass <= 2; ++pass) {
         for (int col0 = 0; col0 < cols; col0 += kWwTile) {
-            if (pass == 1) weight_window_kernel<DT, QLO, 1><<<grid, kWwThreads, kWwSmem, st>>>(a, col0, status);
-            else weight_window_kernel<DT, QLO, 2><<<grid, kWwThreads, kWwSmem, st>>>(a, col0, status);
+            if (pass == 1) weight_window_kernel<QLO, 1><<<grid, kWwThreads, kWwSmem, st>>>(a, col0, status);
+            else weight_window_kernel<QLO, 2><<<grid, kWwThreads, kWwSmem, st>>>(a, col0, status);
             OMNI_CUDA(cudaGetLastError());
         }
     }
@@ -447,14 +608,23 @@ static int32_t launch_weight_window_t(const WeightArgs& a, int32_t* status, cuda
 }
 
 int32_t launch_weight_window(WeightArgs a, int q_dtype, int32_t* status, cudaStream_t st) {
-    a.chunk_keys = ww_chunk_keys(a.B * a.Hkv, a.S);
-    a.chunks = (a.S + a.chunk_keys - 1) / a.chunk_keys;
-    OMNI_REQUIRE(a.B * a.Hkv * a.chunks <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_attn_weight_sums: too many keys");
+    const int64_t heads = a.B * a.Hkv, cols = (int64_t)(a.Hq / a.Hkv) * a.T, col_groups = (cols + kWpWarps - 1) / kWpWarps;
+    const int64_t ctas = ww_ctas(heads, a.S);
+    OMNI_REQUIRE(heads * col_groups < 0x7fffffffLL && a.B * ((a.S + kWwTile - 1) / kWwTile) <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_attn_weight_sums: too many keys");
+    unsigned char* ws = reinterpret_cast<unsigned char*>(a.partial);     // prepared columns, tiles in front of every user, the spans' partial states
+    a.prepared = ws;
+    ws += (size_t)(heads * ((cols + kWwTile - 1) / kWwTile)) * kWwPrepBytes;
+    a.tiles_before = reinterpret_cast<int32_t*>(ws);
+    a.partial = reinterpret_cast<float2*>(ws + ww_before_bytes(a.B));
+    const unsigned grid = (unsigned)(heads * col_groups) + 1;
     switch (q_dtype) {
-        case OMNI_F32:  return launch_weight_window_t<OMNI_F32, true>(a, status, st);
-        case OMNI_BF16: return a.rotate_q ? launch_weight_window_t<OMNI_BF16, true>(a, status, st) : launch_weight_window_t<OMNI_BF16, false>(a, status, st);
-        default:        return a.rotate_q ? launch_weight_window_t<OMNI_F16, true>(a, status, st) : launch_weight_window_t<OMNI_F16, false>(a, status, st);
+        case OMNI_F32:  weight_prepare_kernel<OMNI_F32><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;
+        case OMNI_BF16: weight_prepare_kernel<OMNI_BF16><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;
+        default:        weight_prepare_kernel<OMNI_F16><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;
     }
+    OMNI_CUDA(cudaGetLastError());
+    // a query of a 16-bit type, not rotated, is exact in its fp16 values
+    return q_dtype == OMNI_F32 || a.rotate_q ? launch_weight_window_t<true>(a, (unsigned)ctas, status, st) : launch_weight_window_t<false>(a, (unsigned)ctas, status, st);
 }
 
 }  // namespace omni

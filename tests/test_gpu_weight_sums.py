@@ -79,6 +79,17 @@ def test_rotation_wide_codebooks_and_scale():
         check(attn_weight_sums(q.to(DEV), *rows, user_id=3, scale=scale, rotate_q=True), turned, (nib, qjl, norms), cb, [3, 3], [200, 200], True, True, scale)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_scales_without_a_sign_of_their_own(scale):
+    """A zero scale weighs every key alike, a negative one prefers the smallest products; for few and many columns."""
+    from omnistack_rs_b200.kernels.eviction import attn_weight_sums
+    nib, qjl, norms, cb = packed(1, 1, 150, seed=11)
+    for T in (1, 12):
+        q = torch.randn(1, 2, T, 128, generator=torch.Generator().manual_seed(T))
+        got = attn_weight_sums(*[x.to(DEV) for x in (q, nib, qjl, norms, cb)], user_id=5, scale=scale, seq_lens=torch.tensor([140]))
+        check(got, q, (nib, qjl, norms), cb, [5], [140], True, True, scale)
+
+
 def test_nan_behind_the_length_is_not_read():
     from omnistack_rs_b200.kernels.eviction import attn_weight_sums
     nib, qjl, norms, cb = packed(1, 1, 100, seed=6)

@@ -6,8 +6,8 @@ No counterpart in the reference.  :func:`attn_weight_sums` measures how much eve
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -17,13 +17,8 @@ from .hadamard import HEAD_DIM
 from .quantize import _NBYTES_NIBBLE, _NBYTES_QJL, _prep_codebooks, _user_args
 
 
-class _Evict(C.Structure):
-    """``omni_evict_t`` of the C header."""
-    _fields_ = ([(n, C.c_void_p) for n in ("sums", "seq_lens", "k_nib", "k_qjl", "k_norms", "v_nib", "v_qjl", "v_norms", "sums_out",
-                                           "k_nib_out", "k_qjl_out", "k_norms_out", "v_nib_out", "v_qjl_out", "v_norms_out",
-                                           "index", "new_lens")]
-                + [(n, C.c_int64) for n in ("B", "S", "budget", "recent", "capacity")]
-                + [("H", C.c_int32), ("v_paired", C.c_int32)])
+# ``omni_evict_t`` of the C header, field by field
+_EVICT = struct.Struct("@8P7P2P5q2i")
 
 
 class EvictedCache(NamedTuple):
@@ -40,7 +35,7 @@ class EvictedCache(NamedTuple):
 
 
 def _check_rows(x: torch.Tensor, name: str, shape, dtype) -> None:
-    if tuple(x.shape) != tuple(shape) or x.dtype is not dtype:
+    if x.shape != shape or x.dtype is not dtype:
         raise ValueError(f"{name} must be {tuple(shape)} {dtype}, got {tuple(x.shape)} {x.dtype}")
 
 
@@ -133,13 +128,11 @@ def evict_keys(sums: torch.Tensor, k_nibbles: torch.Tensor, k_qjl: torch.Tensor,
     dev = _lib.require_cuda(sums, k_nibbles, k_qjl, k_norms, v_nibbles, v_qjl, v_norms)
     lib = _lib.load()
     lens = _lens(seq_lens, B, S, dev)
-    src = [None if x is None else x.contiguous() for x in (sums, k_nibbles, k_qjl, k_norms, v_nibbles, v_qjl, v_norms)]
+    src = [None if x is None else x if x.is_contiguous() else x.contiguous() for x in (sums, k_nibbles, k_qjl, k_norms, v_nibbles, v_qjl, v_norms)]
     out = [None if x is None else torch.empty(B, H, capacity, *x.shape[3:], dtype=x.dtype, device=dev) for x in src]
     index = torch.empty(B, H, budget, dtype=torch.int32, device=dev)
     new_lens = torch.empty(B, dtype=torch.int32, device=dev)
-    p = [_lib.ptr(x) for x in src]
-    call = _Evict(p[0], _lib.ptr(lens), *p[1:], *[_lib.ptr(x) for x in out], _lib.ptr(index), _lib.ptr(new_lens), B, S, budget, recent,
-                  capacity, H, int(bool(v_paired)))
+    at = [0 if x is None else x.data_ptr() for x in (src[0], lens, *src[1:], *out, index, new_lens)]
     with _lib.on_device(dev):
-        _lib.check(lib.omni_evict_keys(C.byref(call), _lib.stream_ptr(dev)))
+        _lib.check(lib.omni_evict_keys(_EVICT.pack(*at, B, S, budget, recent, capacity, H, bool(v_paired)), _lib.stream_ptr(dev)))
     return EvictedCache(index, new_lens, *out)

@@ -5,7 +5,7 @@ No counterpart in the reference, whose queries and keys arrive rotated by their 
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -16,27 +16,26 @@ from .hadamard import HEAD_DIM
 MAX_AXES: int = 4
 
 
-class _NormRope(C.Structure):
-    """``omni_norm_rope_t`` of the C header."""
-    _fields_ = [("x", C.c_void_p * 2), ("y", C.c_void_p * 2), ("weight", C.c_void_p * 2), ("positions", C.c_void_p),
-                ("inv_freq", C.c_void_p), ("xs", (C.c_int64 * 3) * 2), ("ps", C.c_int64 * 3), ("B", C.c_int64), ("T", C.c_int64),
-                ("heads", C.c_int32 * 2), ("weight_dtype", C.c_int32 * 2), ("axis_end", C.c_int32 * MAX_AXES),
-                ("dtype", C.c_int32), ("n_axes", C.c_int32), ("n_pairs", C.c_int32), ("positions64", C.c_int32),
-                ("inv_freq64", C.c_int32), ("interleaved", C.c_int32), ("normalize", C.c_int32), ("eps", C.c_float)]
+# ``omni_norm_rope_t`` of the C header, field by field (packed in one go: filling a ctypes structure costs several microseconds)
+_NORM_ROPE = struct.Struct("@2P2P2PPP6q3q2q2i2i4i7if")
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` itself when a kernel can read its 128-element rows in place (16-byte boundaries), else a contiguous copy."""
-    unit = 4 if x.dtype is torch.float32 else 8
-    s = x.stride()
-    if s[-1] != 1 or any(n > 1 and (st % unit or st < 0) for st, n in zip(s[:-1], x.shape[:-1])) or x.data_ptr() % 16:
-        return x.contiguous() if x.data_ptr() % 16 == 0 or not x.is_contiguous() else x.clone()
-    return x
-
-
-def _strides(x: torch.Tensor):
-    """Strides of users, heads and tokens; those of extents of one do not count and are given as 0."""
-    return [st if n > 1 else 0 for st, n in zip(x.stride()[:3], x.shape[:3])]
+def _place(x: torch.Tensor):
+    """(tensor, address, strides of users, heads and tokens) of rows a kernel can read: ``x`` itself when its 128-element rows are
+    contiguous and start on 16-byte boundaries, else a contiguous copy.  Strides of extents of one do not count and are 0."""
+    n0, n1, n2, _ = x.shape
+    s0, s1, s2, s3 = x.stride()
+    if n0 < 2:
+        s0 = 0
+    if n1 < 2:
+        s1 = 0
+    if n2 < 2:
+        s2 = 0
+    at = x.data_ptr()
+    if s3 != 1 or at & 15 or (s0 | s1 | s2) & (3 if x.dtype is torch.float32 else 7):
+        x = x.clone(memory_format=torch.contiguous_format)
+        return x, x.data_ptr(), n1 * n2 * HEAD_DIM, n2 * HEAD_DIM, HEAD_DIM
+    return x, at, s0, s1, s2
 
 
 def _check_weight(w: Optional[torch.Tensor], name: str) -> None:
@@ -48,13 +47,15 @@ def _check_weight(w: Optional[torch.Tensor], name: str) -> None:
         raise TypeError(f"unsupported {name} dtype {w.dtype}; use float32, bfloat16 or float16")
 
 
-def _weight(w: Optional[torch.Tensor], dev) -> Optional[torch.Tensor]:
+def _weight(w: Optional[torch.Tensor], dev):
+    """(tensor, address, dtype code) of a norm weight as the kernel reads it."""
     if w is None:
-        return None
-    w = w.detach()
-    if not (w.device == dev and w.is_contiguous()):
+        return None, 0, 0
+    if w.device != dev or not w.is_contiguous():
         w = w.to(dev).contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
+    if w.data_ptr() & 15:
+        w = w.clone()
+    return w, w.data_ptr(), _lib.DTYPE_CODE[w.dtype]
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -105,35 +106,27 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     _check_weight(k_weight, "k_weight")
     dev = _lib.require_cuda(q, k)
     lib = _lib.load()
-    q_rows = _rows(q)
-    k_rows = None if k is None else _rows(k)
-    qw, kw = _weight(q_weight, dev), _weight(k_weight, dev)
-    positions = positions.to(dev)
-    inv_freq = inv_freq.detach()
+    q, q_at, *q_strides = _place(q)
+    q_out = torch.empty(B, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
+    Hkv, k_at, k_strides, k_out, k_out_at = 0, 0, (0, 0, 0), None, 0
+    if k is not None:
+        Hkv = k.shape[1]
+        k, k_at, *k_strides = _place(k)
+        k_out = torch.empty(B, Hkv, T, HEAD_DIM, dtype=q.dtype, device=dev)
+        k_out_at = k_out.data_ptr()
+    q_weight, qw_at, qw_code = _weight(q_weight, dev)
+    k_weight, kw_at, kw_code = _weight(k_weight, dev)
+    if positions.device != dev:
+        positions = positions.to(dev)
     if inv_freq.device != dev or not inv_freq.is_contiguous():
         inv_freq = inv_freq.to(dev).contiguous()
-    q_out = torch.empty(B, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
-    k_out = None if k is None else torch.empty(B, k.shape[1], T, HEAD_DIM, dtype=q.dtype, device=dev)
     ps = positions.stride()
-    a = _NormRope()
-    a.x[:] = [q_rows.data_ptr(), _lib.ptr(k_rows)]
-    a.y[:] = [q_out.data_ptr(), _lib.ptr(k_out)]
-    a.weight[:] = [_lib.ptr(qw), _lib.ptr(kw)]
-    a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
-    a.xs[0][:] = _strides(q_rows)
-    if k_rows is not None:
-        a.xs[1][:] = _strides(k_rows)
-    a.ps[:] = [ps[0] if lead else 0, ps[-2] if positions.dim() == len(lead) + 2 else 0, ps[-1]]
-    a.B, a.T = B, T
-    a.heads[:] = [Hq, 0 if k is None else k.shape[1]]
-    a.weight_dtype[:] = [0 if w is None else _lib.DTYPE_CODE[w.dtype] for w in (qw, kw)]
-    end = 0
-    for i, n in enumerate(axis_pairs):
-        end += n
-        a.axis_end[i] = end
-    a.dtype, a.n_axes, a.n_pairs = _lib.DTYPE_CODE[q.dtype], len(axis_pairs), P
-    a.positions64, a.inv_freq64 = int(positions.dtype is torch.int64), int(inv_freq.dtype is torch.float64)
-    a.interleaved, a.normalize, a.eps = int(bool(interleaved)), int(eps is not None), 0.0 if eps is None else float(eps)
+    ends = [sum(axis_pairs[:i + 1]) for i in range(len(axis_pairs))] + [0] * (MAX_AXES - len(axis_pairs))
+    call = _NORM_ROPE.pack(
+        q_at, k_at, q_out.data_ptr(), k_out_at, qw_at, kw_at, positions.data_ptr(), inv_freq.data_ptr(), *q_strides, *k_strides,
+        ps[0] if lead else 0, ps[-2] if positions.dim() == len(lead) + 2 else 0, ps[-1], B, T, Hq, Hkv, qw_code, kw_code, *ends,
+        _lib.DTYPE_CODE[q.dtype], len(axis_pairs), P, positions.dtype is torch.int64, inv_freq.dtype is torch.float64, bool(interleaved),
+        eps is not None, 0.0 if eps is None else eps)
     with _lib.on_device(dev):
-        _lib.check(lib.omni_qk_norm_rope(C.byref(a), _lib.stream_ptr(dev)))
+        _lib.check(lib.omni_qk_norm_rope(call, _lib.stream_ptr(dev)))
     return q_out, k_out

@@ -5,21 +5,25 @@ mask; here a prompt's bounds and the causal order are arguments, and prompts of 
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import torch
 
 from .. import _lib
 from .hadamard import HEAD_DIM
-from .position import _rows, _strides
+from .position import _place
+
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_STRIDES = struct.Struct("@3q")
 
 
-def _tiles(x: torch.Tensor) -> torch.Tensor:
-    """``x`` itself when a kernel can copy boxes of its rows, else a contiguous copy (tensor maps have no stride of 0)."""
-    x = _rows(x)
-    return x.contiguous() if any(st == 0 and n > 1 for st, n in zip(x.stride()[:3], x.shape[:3])) else x
+def _tiles(x: torch.Tensor):
+    """Rows a kernel can copy in boxes: tensor maps have no stride of 0, so rows shared by one are copied."""
+    if 0 in x.stride()[:3]:
+        x = x.contiguous()
+    return _place(x)
 
 
 def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
@@ -77,14 +81,16 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens
     lib = _lib.load()
     if lengths is not None:
         lengths = _lib.as_device(lengths, dev, torch.int32)
-    q, k, v = _tiles(q), _tiles(k), _tiles(v)
+    q, q_at, *q_strides = _tiles(q)
+    k, k_at, *k_strides = _tiles(k)
+    v, v_at, *v_strides = _tiles(v)
     out = torch.empty(B, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
-    i64 = C.c_int64 * 3
     packed = cu_seqlens is not None
+    lens_at = None if lengths is None else lengths.data_ptr()
     with _lib.on_device(dev):
         _lib.check(lib.omni_prompt_attn(
-            _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.DTYPE_CODE[q.dtype], i64(*_strides(q)), i64(*_strides(k)), i64(*_strides(v)),
-            _lib.ptr(lengths) if packed else None, lengths.numel() - 1 if packed else B, None if packed else _lib.ptr(lengths),
-            B, Hq, Hkv, T, float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale), int(bool(causal)),
-            _lib.ptr(out), _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr(dev)))
+            q_at, k_at, v_at, _lib.DTYPE_CODE[q.dtype], _STRIDES.pack(*q_strides), _STRIDES.pack(*k_strides), _STRIDES.pack(*v_strides),
+            lens_at if packed else None, lengths.numel() - 1 if packed else B, None if packed else lens_at,
+            B, Hq, Hkv, T, _SCALE if scale is None else scale, bool(causal), out.data_ptr(), _lib.status_word(dev).data_ptr(),
+            _lib.stream_ptr(dev)))
     return out

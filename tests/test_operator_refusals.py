@@ -92,15 +92,11 @@ def test_c_entries_refuse_bad_arguments(lib):
     """Checks that need no device: they come before the first CUDA call of each entry."""
     one = C.c_void_p(16)
     assert lib.omni_qk_norm_rope(None, None) == _lib.ERR_ARG
-    call = position._NormRope()
-    call.B = call.T = 1
-    call.heads[:] = [1, 0]
-    call.n_axes = 1
-    assert lib.omni_qk_norm_rope(C.byref(call), None) == _lib.ERR_ARG                      # no rows
-    call.n_pairs = 65
-    assert lib.omni_qk_norm_rope(C.byref(call), None) == _lib.ERR_ARG
-    call.n_pairs, call.n_axes = 8, 5
-    assert lib.omni_qk_norm_rope(C.byref(call), None) == _lib.ERR_UNSUPPORTED
+    def norm_rope(q=16, heads=1, axes=1, pairs=0, end=0, stride=128, dtype=1):
+        return lib.omni_qk_norm_rope(position._NORM_ROPE.pack(q, 0, 16, 0, 0, 0, 16, 16, 0, 0, stride, 0, 0, 0, 0, 0, 0, 1, 1, heads, 0, 0, 0, end, 0, 0, 0,
+                                                              dtype, axes, pairs, 0, 0, 0, 1, 1e-6), None)
+    assert norm_rope(q=0) == norm_rope(q=8) == norm_rope(heads=-1) == norm_rope(pairs=65, end=65) == norm_rope(pairs=8) == _lib.ERR_ARG
+    assert norm_rope(stride=132) == norm_rope(dtype=7) == _lib.ERR_ARG and norm_rope(axes=5) == _lib.ERR_UNSUPPORTED and norm_rope(heads=0) == _lib.OK
     st = (C.c_int64 * 3)(0, 0, 128)
     prompt = lambda q=one, dt=1, strides=st, n=1, B=1, Hq=2, Hkv=1, T=4, cu=None: lib.omni_prompt_attn(  # noqa: E731
         q, one, one, dt, strides, st, st, cu, n, None, B, Hq, Hkv, T, 1.0, 1, one, None, None)
@@ -113,9 +109,6 @@ def test_c_entries_refuse_bad_arguments(lib):
     assert sums(q=None) == sums(Hq=3) == sums(ws=0) == _lib.ERR_ARG and sums(S=0) == _lib.OK
     assert sums(Hq=2048, Hkv=2048) == _lib.ERR_UNSUPPORTED
     assert lib.omni_evict_keys(None, None) == _lib.ERR_ARG
-    ev = eviction._Evict()
-    ev.B = ev.H = 1
-    ev.S, ev.budget, ev.capacity = 8, 4, 3
-    assert lib.omni_evict_keys(C.byref(ev), None) == _lib.ERR_ARG
-    ev.capacity = 4
-    assert lib.omni_evict_keys(C.byref(ev), None) == _lib.ERR_ARG                          # no buffers
+    evict = lambda capacity, nib=16, B=1: lib.omni_evict_keys(  # noqa: E731
+        eviction._EVICT.pack(16, 0, nib, 16, 16, 16, 0, 0, 16, 16, 16, 16, 16, 0, 0, 16, 16, B, 8, 4, 0, capacity, 1, 0), None)
+    assert evict(3) == evict(4, nib=0) == evict(4, nib=8) == evict(4, B=-1) == _lib.ERR_ARG and evict(4, B=0) == _lib.OK

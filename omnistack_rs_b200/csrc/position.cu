@@ -14,7 +14,7 @@
 
 namespace omni {
 
-constexpr int kPosThreads = 256;
+constexpr int kPosThreads = 128;
 constexpr int kPosRows = kPosThreads / 16;         // sixteen-lane units per CTA
 
 // Rows a unit works on at a time; as many more are on their way meanwhile.
@@ -97,7 +97,7 @@ struct PosCall {
 };
 
 template <int DT, int MODE>
-__global__ void __launch_bounds__(kPosThreads) norm_rope_kernel(const __grid_constant__ PosCall c) {
+__global__ void __launch_bounds__(kPosThreads, 6) norm_rope_kernel(const __grid_constant__ PosCall c) {
     const omni_norm_rope_t& a = c.a;
     using E = typename Elem<DT>::T;
     constexpr int R = PosBatch<DT>::kRows, NW = PosBatch<DT>::kWords;
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kPosThreads) norm_rope_kernel(const __grid_con
         for (int r = 0; r < R; ++r) {
 #pragma unroll
             for (int k = 0; k < NW; k += 4) {
-                const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + k / 4);           // read once
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + k / 4);           // read once
                 ahead[r][k] = v.x; ahead[r][k + 1] = v.y; ahead[r][k + 2] = v.z; ahead[r][k + 3] = v.w;
             }
             if (h0 + r + 1 < e) p += a.xs[s][1];
@@ -312,7 +312,7 @@ extern "C" int32_t omni_qk_norm_rope(const omni_norm_rope_t* call, void* stream)
     // Few tokens: a unit takes few heads, so that the call still fills the device (the angles are then computed once per unit)
     const int64_t tokens = a.B * a.T;
     int64_t groups = 1;
-    while (groups < H && tokens * groups < (int64_t)148 * 4 * kPosRows) groups *= 2;
+    while (groups < H && tokens * groups < (int64_t)148 * 2 * kPosRows) groups *= 2;
     c.heads_per_unit = (int)((H + groups - 1) / groups);
     c.groups = (int)((H + c.heads_per_unit - 1) / c.heads_per_unit);
     c.units = tokens * c.groups;

@@ -2,8 +2,8 @@
 //
 // Selection.  Keys ordered by (sum descending, position ascending); the budget - recent first of the positions below
 // len - recent stay, and the `recent` last positions.  One CTA per (user, head): the sums become order-preserving 32-bit
-// numbers, four histogram passes of eight bits find the value of the last one that stays, a scan over the positions emits
-// the kept ones in order.
+// numbers in shared memory, three histogram passes find the value of the last one that stays digit by digit, and two scans over
+// the positions (which of its equals stay, and where a kept position goes) emit the kept ones in order.
 //
 // Gather.  A warp moves a group of eight kept rows.  Rows are moved, never recomputed, so the new cache holds the same bits;
 // V's pair layout mixes the nibbles of two keys per row, which the lanes take apart for the old pairs and join for the new.
@@ -11,7 +11,11 @@
 
 namespace omni {
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 512;
+constexpr int kSelKeys = 16;                       // consecutive positions per thread
+constexpr int kSelSpan = kSelThreads * kSelKeys;   // positions a CTA holds at a time: a longer cache is read again for every digit
+constexpr int kSelKeyBytes = kSelThreads * (kSelKeys + 4) * 4;
+constexpr int kSelBins = 2048;
 
 // ascending unsigned order = ascending sum; +0 = -0, NaN above everything
 __device__ __forceinline__ uint32_t sum_key(float x) {
@@ -26,11 +30,37 @@ __device__ __forceinline__ int clamp_len(const int32_t* seq_lens, int64_t b, int
     return (int)(n < 0 ? 0 : (n > S ? S : n));
 }
 
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ omni_evict_t a) {
-    __shared__ uint32_t hist[256];
+// sum over the threads in front of this one, and over all of them (every thread calls this; `part` holds one value per warp)
+__device__ __forceinline__ uint32_t sel_scan(uint32_t v, uint32_t* part, uint32_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t upto = v;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const uint32_t o = __shfl_up_sync(kFullMask, upto, x);
+        if (lane >= x) upto += o;
+    }
+    __syncthreads();                                             // the previous use of `part` is over
+    if (lane == 31) part[warp] = upto;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kSelThreads / 32; ++w) {
+        const uint32_t n = part[w];
+        if (w < warp) before += n;
+        total += n;
+    }
+    return before + upto - v;
+}
+
+__global__ void __launch_bounds__(kSelThreads, 4) evict_select_kernel(const __grid_constant__ omni_evict_t a) {
+    __shared__ uint32_t hist[kSelBins];
+    __shared__ uint32_t part[kSelThreads / 32];
     __shared__ uint32_t s_value, s_need;
-    __shared__ int warp_cnt[32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // this thread's keys, positions base + kSelKeys * tid ..; no candidate: 0.  (Registers for them would halve the CTAs per SM;
+    // 20 words apart, the 16-byte accesses of neighbouring threads meet in no bank.)
+    extern __shared__ __align__(16) uint32_t sel_keys[];
+    const int tid = threadIdx.x;
     const int64_t bh = blockIdx.x, b = bh / a.H;
     const int len = clamp_len(a.seq_lens, b, a.S);
     const int budget = (int)a.budget, recent = (int)a.recent;
@@ -42,87 +72,104 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
     }
     const float* sums = a.sums + bh * a.S;
     const int n = len - recent;                                  // candidates; budget - recent of them stay (fewer than n)
-    if (tid == 0) { s_value = 0; s_need = (uint32_t)(budget - recent); }
-    uint32_t known = 0;                                          // mask of the bits of the threshold found so far
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    const bool one_span = n <= kSelSpan;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(sums) & 15) == 0);
+    uint4* mine4 = reinterpret_cast<uint4*>(sel_keys + (kSelKeys + 4) * tid);
+    auto load = [&](int base) {
+        const int p = base + kSelKeys * tid;
+#pragma unroll
+        for (int k = 0; k < kSelKeys; k += 4) {
+            uint32_t key[4];
+            if (aligned && p + k + 4 <= n) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(sums + p + k));
+                key[0] = sum_key(v.x); key[1] = sum_key(v.y); key[2] = sum_key(v.z); key[3] = sum_key(v.w);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) key[x] = p + k + x < n ? sum_key(__ldg(sums + p + k + x)) : 0u;
+            }
+            mine4[k / 4] = make_uint4(key[0], key[1], key[2], key[3]);
+        }
+    };
+    if (one_span) load(0);
+    uint32_t need = (uint32_t)(budget - recent);                 // this many of the keys that agree with `value` so far stay, the largest
+    uint32_t value = 0;
+    // digits of 11, 11 and 10 bits: the first spans sign, exponent and two bits of the fraction, so that sums of a few binary orders
+    // already spread over dozens of counters
+#pragma unroll 1
+    for (int digit = 0; digit < 3 && need > 0; ++digit) {
+        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+        const uint32_t mask = digit == 2 ? 1023u : 2047u;
+        const uint32_t known = digit == 0 ? 0u : digit == 1 ? 0xffe00000u : 0xfffffc00u;
+        for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
-        const uint32_t value = s_value;
-        for (int i = tid; i < n; i += kSelThreads) {
-            const uint32_t key = sum_key(sums[i]);
-            if ((key & known) == value) atomicAdd(&hist[(key >> shift) & 255], 1u);
+        for (int base = 0; base < n; base += kSelSpan) {
+            if (!one_span) load(base);
+            if (base + kSelKeys * tid >= n) continue;
+#pragma unroll
+            for (int k = 0; k < kSelKeys; k += 4) {
+                const uint4 v = mine4[k / 4];
+                const uint32_t key[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    // no candidate's key is 0 (that of -infinity is 0x007fffff), and from the second digit on `value` is not
+                    if ((key[x] & known) == value && key[x] != 0u) atomicAdd(&hist[(key[x] >> shift) & mask], 1u);
+            }
         }
         __syncthreads();
-        if (warp == 0) {                                         // the digit in which the running count from above reaches the need
-            const uint32_t need = s_need;
-            uint32_t c[8], mine = 0;
+        constexpr int kPer = kSelBins / kSelThreads;             // this thread's counters, from the largest down
+        uint32_t c[kPer], mine = 0, all;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) { c[k] = hist[255 - (8 * lane + k)]; mine += c[k]; }
-            uint32_t upto = mine;
+        for (int k = 0; k < kPer; ++k) { c[k] = hist[kSelBins - 1 - (kPer * tid + k)]; mine += c[k]; }
+        uint32_t before = sel_scan(mine, part, all);
+        if (before < need && before + mine >= need) {
 #pragma unroll
-            for (int x = 1; x < 32; x <<= 1) {
-                const uint32_t o = __shfl_up_sync(kFullMask, upto, x);
-                if (lane >= x) upto += o;
-            }
-            uint32_t before = upto - mine;
-            const bool here = need > 0 ? (before < need && upto >= need) : lane == 0;
-            if (here) {
-                uint32_t digit = 255 - 8 * lane;
-                if (need > 0) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        if (before < need && before + c[k] >= need) { digit = 255 - (8 * lane + k); s_need = need - before; }
-                        before += c[k];
-                    }
+            for (int k = 0; k < kPer; ++k) {
+                if (before < need && before + c[k] >= need) {
+                    s_value = value | ((uint32_t)(kSelBins - 1 - (kPer * tid + k)) << shift);
+                    s_need = need - before;
                 }
-                s_value = value | (digit << shift);
+                before += c[k];
             }
         }
-        known |= 255u << shift;
         __syncthreads();
+        value = s_value;
+        need = s_need;
     }
-    const uint32_t value = s_value;
-    const int ties = (int)s_need;                                // this many of the keys equal to the threshold stay, lowest first
-    int kept = 0, tied = 0;                                      // of the chunks so far
-    for (int i0 = 0; i0 < len; i0 += kSelThreads) {
-        const int i = i0 + tid;
-        const bool last = i >= n && i < len;
-        const uint32_t key = i < n ? sum_key(sums[i]) : 0;
-        const bool above = i < n && budget > recent && key > value;
-        const bool tie = i < n && budget > recent && key == value;
-        const uint32_t tie_ballot = __ballot_sync(kFullMask, tie);
-        // positions of the ties first, then of the kept keys
-        if (lane == 0) warp_cnt[warp] = __popc(tie_ballot);
-        __syncthreads();
-        int v = lane < 32 ? warp_cnt[lane] : 0;
-        int scan = v;
+    const bool some = budget > recent;                           // `need` of the keys equal to `value` stay, lowest positions first
+    uint32_t kept = 0, tied = 0;                                 // of the spans so far
+    for (int base = 0; base < len; base += kSelSpan) {
+        if (!one_span || base > 0) load(base);
+        uint32_t above = 0, equal = 0, total;                    // bit k: the thread's key k
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            const int o = __shfl_up_sync(kFullMask, scan, x);
-            if (lane >= x) scan += o;
-        }
-        const int tie_total = __shfl_sync(kFullMask, scan, 31);
-        const int tie_base = __shfl_sync(kFullMask, scan - v, warp);
-        const int tie_rank = tied + tie_base + __popc(tie_ballot & ((1u << lane) - 1u));
-        const bool keep = last || above || (tie && tie_rank < ties);
-        const uint32_t keep_ballot = __ballot_sync(kFullMask, keep);
-        __syncthreads();
-        if (lane == 0) warp_cnt[warp] = __popc(keep_ballot);
-        __syncthreads();
-        v = warp_cnt[lane];
-        scan = v;
+        for (int k = 0; k < kSelKeys; k += 4) {
+            const uint4 v = mine4[k / 4];
+            const uint32_t key[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            const int o = __shfl_up_sync(kFullMask, scan, x);
-            if (lane >= x) scan += o;
+            for (int x = 0; x < 4; ++x) {
+                above |= key[x] > value ? 1u << (k + x) : 0u;
+                equal |= key[x] == value ? 1u << (k + x) : 0u;
+            }
         }
-        const int keep_total = __shfl_sync(kFullMask, scan, 31);
-        const int keep_base = __shfl_sync(kFullMask, scan - v, warp);
-        const int at = kept + keep_base + __popc(keep_ballot & ((1u << lane) - 1u));
-        if (keep && at < budget) index[at] = i;
-        kept += keep_total;
-        tied += tie_total;
-        __syncthreads();
+        if (!some) above = equal = 0;
+        const uint32_t rank = tied + sel_scan(__popc(equal), part, total);
+        tied += total;
+        uint32_t stay = rank < need ? need - rank : 0;           // the first `stay` of the thread's equals
+        uint32_t keep = above;
+        for (; equal && stay; --stay) {
+            keep |= equal & (0u - equal);
+            equal &= equal - 1;
+        }
+        const int p0 = base + kSelKeys * tid;
+#pragma unroll
+        for (int k = 0; k < kSelKeys; ++k) keep |= p0 + k >= n && p0 + k < len ? 1u << k : 0u;
+        uint32_t at = kept + sel_scan(__popc(keep), part, total);
+        kept += total;
+        while (keep) {
+            const int k = __ffs(keep) - 1;
+            keep &= keep - 1;
+            if (at < (uint32_t)budget) index[at] = base + kSelKeys * tid + k;
+            ++at;
+        }
     }
 }
 
@@ -217,7 +264,8 @@ extern "C" int32_t omni_evict_keys(const omni_evict_t* call, void* stream) {
     const int64_t groups_per_head = (a.capacity + 7) / 8, n_groups = a.B * a.H * groups_per_head;
     OMNI_REQUIRE((n_groups + kGatherWarps - 1) / kGatherWarps <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_evict_keys: too many rows");
     cudaStream_t st = (cudaStream_t)stream;
-    evict_select_kernel<<<(unsigned)(a.B * a.H), kSelThreads, 0, st>>>(a);
+    OMNI_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeyBytes));
+    evict_select_kernel<<<(unsigned)(a.B * a.H), kSelThreads, kSelKeyBytes, st>>>(a);
     OMNI_CUDA(cudaGetLastError());
     evict_gather_kernel<<<(unsigned)((n_groups + kGatherWarps - 1) / kGatherWarps), kGatherWarps * 32, 0, st>>>(a, groups_per_head, n_groups);
     return check_cuda(cudaGetLastError(), "evict_gather_kernel launch");

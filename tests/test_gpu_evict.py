@@ -47,7 +47,8 @@ def check(sums, rows, lens, budget, recent, paired, capacity=None):
 
 @pytest.mark.parametrize("paired,residual", [(False, True), (True, False)])
 @pytest.mark.parametrize("S,lens,budget,recent", [(1, [1, 0], 1, 0), (40, [40, 9], 8, 3), (41, [41, 16], 17, 17), (1500, [1500, 1031], 100, 0),
-                                                  (1025, [1024, 1025], 1023, 5), (300, [299, 8], 256, 64), (64, [64, 10], 64, 0), (30, [30, 12], 50, 10)])
+                                                  (1025, [1024, 1025], 1023, 5), (300, [299, 8], 256, 64), (64, [64, 10], 64, 0), (30, [30, 12], 50, 10),
+                                                  (20000, [20000, 8193], 8000, 100), (8200, [8192, 8200], 4000, 0)])
 def test_against_sorting(paired, residual, S, lens, budget, recent):
     rows = arrays(2, 3, S, seed=S + budget, residual=residual)
     g = torch.Generator().manual_seed(budget)

@@ -53,7 +53,22 @@ int32_t check_cuda(cudaError_t e, const char* what);
         if (!(cond)) return ::omni::set_error((code), __VA_ARGS__); \
     } while (0)
 
+// Launch behind a kernel of the same call that lets its successors start early (follow_me_early): the successor's CTAs are placed while the
+// last ones of its predecessor run, and wait (after_predecessor) before they touch what it wrote.
+template <typename... Params, typename... Args>
+static cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args&&... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = &attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // ---- device helpers ----------------------------------------------------------
+
+__device__ __forceinline__ void follow_me_early() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+__device__ __forceinline__ void after_predecessor() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
 // 128-point normalised Walsh-Hadamard transform of one row spread over a warp:
 // lane l holds elements 4l..4l+3.  Stage order h = 1, 2, 4, ..., 64, every add and

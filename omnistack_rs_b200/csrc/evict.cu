@@ -184,9 +184,10 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
     const int len = clamp_len(a.seq_lens, b, a.S);
     const int64_t new_len = len < a.budget ? len : a.budget;
     const int64_t src0 = bh * a.S, dst0 = bh * a.capacity;
+    after_predecessor();
     // old position of row r of the group in lane r (-1: no key)
     int from = -1;
-    if (lane < 8 && row0 + lane < new_len) from = __ldg(a.index + bh * a.budget + row0 + lane);
+    if (lane < 8 && row0 + lane < new_len) from = a.index[bh * a.budget + row0 + lane];
     {   // K nibbles: four lanes per row
         const int r = lane >> 2, c = lane & 3;
         const int p = __shfl_sync(kFullMask, from, r);
@@ -267,6 +268,6 @@ extern "C" int32_t omni_evict_keys(const omni_evict_t* call, void* stream) {
     OMNI_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeyBytes));
     evict_select_kernel<<<(unsigned)(a.B * a.H), kSelThreads, kSelKeyBytes, st>>>(a);
     OMNI_CUDA(cudaGetLastError());
-    evict_gather_kernel<<<(unsigned)((n_groups + kGatherWarps - 1) / kGatherWarps), kGatherWarps * 32, 0, st>>>(a, groups_per_head, n_groups);
-    return check_cuda(cudaGetLastError(), "evict_gather_kernel launch");
+    return check_cuda(launch_early(evict_gather_kernel, dim3((unsigned)((n_groups + kGatherWarps - 1) / kGatherWarps)), kGatherWarps * 32, 0, st, a, groups_per_head, n_groups),
+                      "evict_gather_kernel launch");
 }

@@ -11,65 +11,65 @@
 // mma.m16n8k16 with keys as rows and columns as columns: value and remainder of a centroid share one table lookup and one
 // accumulator each, signs are exact (+-1), G_i . q is split like the centroids.  A query of a 16-bit type is exact in fp16 after a
 // power-of-two scaling of its row; an fp32 or rotated one is split as well (QLO).
-// Lane (g, c) = (lane / 4, lane % 4) reads bytes 16c .. 16c + 15 of the rows of keys g and g + 8: k-step ks takes its bytes 2ks
+// A warp works alone on a unit of one head's keys.  Lane (g, c) = (lane / 4, lane % 4) reads bytes 16c .. 16c + 15 of the rows of keys g and g + 8: k-step ks takes its bytes 2ks
 // and 2ks + 1, i.e. dims 32c + 4ks .. + 3, and the query fragments are laid out in the same order.
 #include "weight_sums.cuh"
 
 namespace omni {
 
 constexpr int kWmWarps = 8;
+constexpr int kWmLutBytes = 256 * 32 * 8;
 
 __device__ __forceinline__ void wm_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// ... into a fresh accumulator
+__device__ __forceinline__ void wm_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// +-1 as fp16 for bits i and i + 16 of z (1 = +1): what an operand register pairs, at two instructions
+__device__ __forceinline__ uint32_t wm_sign_pair(uint32_t z, int i) { return ((z << (15 - i)) & 0x80008000u) ^ 0xBC00BC00u; }
+
 struct WmKeys { uint4 n0, n1; uint32_t s0, s1; float r0, r1; };          // this lane's part of keys g and g + 8 of a block of 16
 
+// A warp per (user, head): the query and projection fragments of every lane and the score factors of its two result columns, as
+// kWmPieces<QLO> 16-byte pieces [piece][lane].
+template <bool QLO> constexpr int kWmPieces = QLO ? 13 : 9;
+constexpr int kWmPrepWarps = 4;
 template <int DT, bool QLO>
-__global__ void __launch_bounds__(kWmWarps * 32, 2) weight_step_kernel(const __grid_constant__ WeightArgs a, int pad) {
-    extern __shared__ __align__(128) unsigned char wm_smem[];
-    __shared__ float c_s[kWsStepCols][kQjlDim + 4];
-    __shared__ float2 part[kWmWarps][kWsStepCols];
+__global__ void __launch_bounds__(kWmPrepWarps * 32) weight_fragments_kernel(const __grid_constant__ WeightArgs a) {
+    __shared__ __align__(16) float c_s[kWmPrepWarps][kWsStepCols][kQjlDim + 4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-    const int64_t bh = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, b = bh / a.Hkv;
+    follow_me_early();
+    if (blockIdx.x == gridDim.x - 1) {
+        ws_tiles_before<kWmPrepWarps>(a, tid);
+        return;
+    }
+    const int64_t bh = (int64_t)blockIdx.x * kWmPrepWarps + warp;
+    if (bh >= a.B * a.Hkv) return;
+    const int64_t b = bh / a.Hkv;
     const int h = (int)(bh % a.Hkv), G = a.Hq / a.Hkv, cols = G * a.T;
-    const int len = ws_len(a, b);
-    const int k_begin = (int)(chunk * a.chunk_keys);
-    const int k_end = len - k_begin < a.chunk_keys ? len : k_begin + (int)a.chunk_keys;
-    if (k_begin >= k_end) return;
-    const int64_t row0 = bh * a.S;
-    auto load = [&](int k0, WmKeys& x) {                                 // keys past the end repeat the last one
-        const int64_t ra = row0 + (k0 + g < k_end ? k0 + g : k_end - 1), rb = row0 + (k0 + g + 8 < k_end ? k0 + g + 8 : k_end - 1);
-        x.n0 = __ldg(reinterpret_cast<const uint4*>(a.k_nib + ra * kNibBytes) + c);
-        x.n1 = __ldg(reinterpret_cast<const uint4*>(a.k_nib + rb * kNibBytes) + c);
-        if (a.with_qjl) {
-            x.s0 = __ldg(reinterpret_cast<const uint16_t*>(a.k_qjl + ra * kQjlBytes) + c);
-            x.s1 = __ldg(reinterpret_cast<const uint16_t*>(a.k_qjl + rb * kQjlBytes) + c);
-            x.r0 = __ldg(a.k_norms + ra);
-            x.r1 = __ldg(a.k_norms + rb);
-        }
-    };
-    WmKeys next;
-    next.s0 = next.s1 = 0; next.r0 = next.r1 = 0.f;
-    int k0 = k_begin + 16 * warp;
-    if (k0 < k_end) load(k0, next);
+    float cb_top = fabsf(__ldg(a.codebooks + (a.cb_per_head ? h * 16 : 0) + (lane & 15)));
+#pragma unroll
+    for (int x = 8; x >= 1; x >>= 1) cb_top = fmaxf(cb_top, __shfl_xor_sync(kFullMask, cb_top, x));
+    const float cb_mul = ws_pow2(cb_top);
 
-    // ---- table of the head's centroids --------------------------------------------------------------------------------
-    const float cb_mul = ws_build_lut(wm_smem, a.codebooks + (a.cb_per_head ? h * 16 : 0), tid);
-    // ---- query fragments: lane (g, c) has dims 32c .. 32c + 31 of column g ----------------------------------------------
+    // ---- query fragments: lane (g, c) has dims 32c .. 32c + 31 of column g --------------------------------------------
     uint32_t qv[8][2], qr[QLO ? 8 : 1][2];
     float q_mul;
     {
         float q[32];
         const int64_t qrow = g < cols ? (b * a.Hq + (int64_t)h * G + g / a.T) * a.T + g % a.T : 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (g < cols) Elem<DT>::load4(a.q, qrow * kHeadDim + 32 * c + 4 * i, v);
+        for (int i = 0; i < 4; ++i) {
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (g < cols) load8<DT>(a.q, qrow * kHeadDim + 32 * c + 8 * i, v);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) q[4 * i + k] = v[k];
+            for (int k = 0; k < 8; ++k) q[8 * i + k] = v[k];
         }
-        if (a.rotate_q) {                                                // Walsh-Hadamard over 4 lanes x 32 elements, stages in order
+        if (a.rotate_q) {                                            // Walsh-Hadamard over 4 lanes x 32 elements, stages in order
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1) {
 #pragma unroll
@@ -109,38 +109,48 @@ __global__ void __launch_bounds__(kWmWarps * 32, 2) weight_step_kernel(const __g
             }
         }
     }
-    // ---- G . q of the head's 64 projections (G is +-1: exact), four warps of 16 projections each ------------------------------
+    // ---- G . q of the head's 64 projections (G is +-1: exact), sixteen at a time, handed over through shared memory -----------
     uint32_t pv[4][2], pr[4][2];
     float p_mul = 1.f;
     if (a.with_qjl) {
-        if (warp < 4) {
-            const int32_t uid = a.user_ids ? __ldg(a.user_ids + b) : a.user_id;
-            const uint32_t* gr = a.g_rows + ((size_t)seed_of(uid, h) * kQjlDim + 16 * warp) * 4;
-            const uint32_t w0 = __ldg(gr + g * 4 + c), w1 = __ldg(gr + (g + 8) * 4 + c);
+        const int32_t uid = a.user_ids ? __ldg(a.user_ids + b) : a.user_id;
+        const uint32_t* gr = a.g_rows + (size_t)seed_of(uid, h) * kQjlDim * 4 + g * 4 + c;
+        uint32_t gw[4][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) { gw[t][0] = __ldg(gr + 64 * t); gw[t][1] = __ldg(gr + 64 * t + 32); }
+        float (*cw)[kQjlDim + 4] = c_s[warp];
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
             float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-                const uint32_t a0 = ws_signs2(w0 >> (4 * ks)), a1 = ws_signs2(w1 >> (4 * ks)), a2 = ws_signs2(w0 >> (4 * ks + 2)), a3 = ws_signs2(w1 >> (4 * ks + 2));
+                const uint32_t a0 = ws_signs2(gw[t][0] >> (4 * ks)), a1 = ws_signs2(gw[t][1] >> (4 * ks));
+                const uint32_t a2 = ws_signs2(gw[t][0] >> (4 * ks + 2)), a3 = ws_signs2(gw[t][1] >> (4 * ks + 2));
                 wm_mma(d, a0, a1, a2, a3, qv[ks][0], qv[ks][1]);
                 if (QLO) wm_mma(d, a0, a1, a2, a3, qr[ks][0], qr[ks][1]);
             }
-            c_s[2 * c][16 * warp + g] = d[0];
-            c_s[2 * c + 1][16 * warp + g] = d[1];
-            c_s[2 * c][16 * warp + g + 8] = d[2];
-            c_s[2 * c + 1][16 * warp + g + 8] = d[3];
+            cw[2 * c][16 * t + g] = d[0];
+            cw[2 * c + 1][16 * t + g] = d[1];
+            cw[2 * c][16 * t + g + 8] = d[2];
+            cw[2 * c + 1][16 * t + g + 8] = d[3];
         }
-        __syncthreads();
+        __syncwarp();
         float p[16], top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { p[i] = c_s[g][16 * c + i]; top = fmaxf(top, fabsf(p[i])); }
+        for (int i = 0; i < 16; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&cw[g][16 * c + i]);
+            p[i] = v.x; p[i + 1] = v.y; p[i + 2] = v.z; p[i + 3] = v.w;
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
         top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
         top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
         p_mul = ws_pow2(top);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float u = p[4 * s + 2 * x] * p_mul, v = p[4 * s + 2 * x + 1] * p_mul;
+            for (int x = 0; x < 2; ++x) {                            // a register pairs projections i and i + 8 (see wm_sign_pair)
+                const float u = p[2 * s + x] * p_mul, v = p[2 * s + x + 8] * p_mul;
                 pv[s][x] = ws_half2(u, v);
                 pr[s][x] = ws_rest2(u, v, pv[s][x]);
             }
@@ -148,108 +158,234 @@ __global__ void __launch_bounds__(kWmWarps * 32, 2) weight_step_kernel(const __g
     }
     // factors of this lane's two result columns (they are lanes 8c and 8c + 4's columns); powers of two divide exactly
     float f_cb[2], f_sg[2];
-    int last[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const float qm = __shfl_sync(kFullMask, q_mul, 8 * c + 4 * x), pm = __shfl_sync(kFullMask, p_mul, 8 * c + 4 * x);
         f_cb[x] = a.scale * kWsLog2e / qm / cb_mul;
         f_sg[x] = a.scale * kWsLog2e * kQjlCoef / qm / pm;
-        const int col = 2 * c + x;
-        last[x] = col < cols ? (a.causal ? len - a.T + col % a.T : len - 1) : -1;
     }
-    __syncthreads();                                                     // the table is complete
+    uint4* out = reinterpret_cast<uint4*>(a.prepared) + bh * (kWmPieces<QLO> * 32) + lane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        out[32 * k] = make_uint4(qv[2 * k][0], qv[2 * k][1], qv[2 * k + 1][0], qv[2 * k + 1][1]);
+        if (a.with_qjl) out[32 * (4 + k)] = make_uint4(pv[k][0], pv[k][1], pr[k][0], pr[k][1]);
+        if constexpr (QLO) out[32 * (9 + k)] = make_uint4(qr[2 * k][0], qr[2 * k][1], qr[2 * k + 1][0], qr[2 * k + 1][1]);
+    }
+    out[32 * 8] = make_uint4(__float_as_uint(f_cb[0]), __float_as_uint(f_cb[1]), __float_as_uint(f_sg[0]), __float_as_uint(f_sg[1]));
+}
 
-    // ---- keys -----------------------------------------------------------------------------------------------------------
-    const unsigned char* lut = wm_smem + 8 * (lane & 15);
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (; k0 < k_end; k0 += 16 * kWmWarps) {
-        const WmKeys x = next;
-        if (k0 + 16 * kWmWarps < k_end) load(k0 + 16 * kWmWarps, next);
-        float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t u0 = w == 0 ? x.n0.x : w == 1 ? x.n0.y : w == 2 ? x.n0.z : x.n0.w;
-            const uint32_t u1 = w == 0 ? x.n1.x : w == 1 ? x.n1.y : w == 2 ? x.n1.z : x.n1.w;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int ks = 2 * w + k;
-                const uint2 t0 = *reinterpret_cast<const uint2*>(lut + ((k ? u0 >> 9 : u0 << 7) & 0x7f80u));
-                const uint2 t1 = *reinterpret_cast<const uint2*>(lut + ((k ? u1 >> 9 : u1 << 7) & 0x7f80u));
-                const uint2 t2 = *reinterpret_cast<const uint2*>(lut + ((k ? u0 >> 17 : u0 >> 1) & 0x7f80u));
-                const uint2 t3 = *reinterpret_cast<const uint2*>(lut + ((k ? u1 >> 17 : u1 >> 1) & 0x7f80u));
-                wm_mma(d, t0.x, t1.x, t2.x, t3.x, qv[ks][0], qv[ks][1]);
-                wm_mma(e, t0.y, t1.y, t2.y, t3.y, qv[ks][0], qv[ks][1]);
-                if (QLO) wm_mma(e, t0.x, t1.x, t2.x, t3.x, qr[ks][0], qr[ks][1]);
+// A CTA's share of the row of tiles, heads first (kv head, user, tile), so that its centroid table rarely changes.  Warp w takes keys
+// 16 w .. 16 w + 15 of every tile; its maximum and sum of a span are entry w of span (head number, CTA) = head number + CTA.
+template <bool QLO>
+__global__ void __launch_bounds__(kWmWarps * 32, 2) weight_step_kernel(const __grid_constant__ WeightArgs a, int pad) {
+    extern __shared__ __align__(128) unsigned char wm_smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+    const int cols = a.Hq / a.Hkv * a.T;
+    int table = -1;                                                      // head whose table is in shared memory
+    if (!a.cb_per_head) {
+        ws_build_lut<32>(wm_smem, a.codebooks, tid);
+        table = 0;
+    }
+    after_predecessor();
+    __syncthreads();
+    const int64_t per_head = *(volatile const int32_t*)(a.tiles_before + a.B), all = per_head * a.Hkv;
+    const int64_t sharers = ws_sharers(gridDim.x, all);
+    if (blockIdx.x >= sharers) return;
+    const int64_t x0 = blockIdx.x * all / sharers, x1 = (blockIdx.x + 1) * all / sharers;
+    int left = (int)(x1 - x0);                                           // tiles still to come, this span's among them
+    int h = (int)(x0 / per_head), b = ws_user_of(a, x0 % per_head, 1, lane);
+    int tile = (int)(x0 % per_head) - a.tiles_before[b];
+    const uint32_t lane8 = 8 * lane;
+    // entry of byte k of word u, this lane's copy: the address is (byte << 8) | lane8
+    auto look = [&](uint32_t u, int k) { return *reinterpret_cast<const uint2*>(wm_smem + __byte_perm(u, lane8, 0x5504 | (k << 4))); };
+    while (left > 0) {
+        const int64_t bh = (int64_t)b * a.Hkv + h, row0 = bh * a.S;
+        const int len = ws_len(a, b), tiles = (len + kWsTile - 1) / kWsTile;
+        const int n_span = tiles - tile < left ? tiles - tile : left;
+        const int k_end = len < (tile + n_span) * kWsTile ? len : (tile + n_span) * kWsTile;
+        int k0 = tile * kWsTile + 16 * warp;
+        const uint4* nib = reinterpret_cast<const uint4*>(a.k_nib + row0 * kNibBytes) + c;
+        const uint16_t* sgn = reinterpret_cast<const uint16_t*>(a.k_qjl + row0 * kQjlBytes) + c;
+        const float* nrm = a.k_norms + row0;
+        auto load = [&](WmKeys& x) {
+            int ka = k0 + g, kb = k0 + g + 8;
+            if (k0 + 16 > k_end) {                                       // keys past the end repeat the last one
+                ka = ka < k_end ? ka : k_end - 1;
+                kb = kb < k_end ? kb : k_end - 1;
             }
+            x.n0 = __ldg(nib + 4 * (int64_t)ka);
+            x.n1 = __ldg(nib + 4 * (int64_t)kb);
+            if (a.with_qjl) {
+                x.s0 = __ldg(sgn + 4 * (int64_t)ka);
+                x.s1 = __ldg(sgn + 4 * (int64_t)kb);
+                x.r0 = __ldg(nrm + ka);
+                x.r1 = __ldg(nrm + kb);
+            }
+        };
+        WmKeys next;
+        next.s0 = next.s1 = 0; next.r0 = next.r1 = 0.f;
+        if (k0 < k_end) load(next);
+        uint32_t qv[8][2], qr[QLO ? 8 : 1][2], pv[4][2], pr[4][2];
+        float f_cb[2], f_sg[2];
+        {
+            const uint4* in = reinterpret_cast<const uint4*>(a.prepared) + bh * (kWmPieces<QLO> * 32) + lane;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint4 v = in[32 * k];
+                qv[2 * k][0] = v.x; qv[2 * k][1] = v.y; qv[2 * k + 1][0] = v.z; qv[2 * k + 1][1] = v.w;
+                uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                if (a.with_qjl) u = in[32 * (4 + k)];
+                pv[k][0] = u.x; pv[k][1] = u.y; pr[k][0] = u.z; pr[k][1] = u.w;
+                if constexpr (QLO) {
+                    const uint4 r = in[32 * (9 + k)];
+                    qr[2 * k][0] = r.x; qr[2 * k][1] = r.y; qr[2 * k + 1][0] = r.z; qr[2 * k + 1][1] = r.w;
+                }
+            }
+            const uint4 f = in[32 * 8];
+            f_cb[0] = __uint_as_float(f.x); f_cb[1] = __uint_as_float(f.y); f_sg[0] = __uint_as_float(f.z); f_sg[1] = __uint_as_float(f.w);
         }
+        if (table != (a.cb_per_head ? h : 0)) {                          // (the same for the whole CTA)
+            __syncthreads();
+            table = a.cb_per_head ? h : 0;
+            ws_build_lut<32>(wm_smem, a.codebooks + 16 * table, tid);
+            __syncthreads();
+        }
+        int last[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = (d[i] + e[i]) * f_cb[i & 1];
-        if (a.with_qjl) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < 2; ++x) {
+            const int col = 2 * c + x;
+            last[x] = col < cols ? (a.causal ? len - a.T + col % a.T : len - 1) : -1;
+            last[x] = last[x] < k_end - 1 ? last[x] : k_end - 1;
+        }
+        // keys below this are open to every column; with columns to spare, none are
+        const int open_to = cols < kWsStepCols ? 0 : (a.causal && len - a.T + 1 < k_end ? len - a.T + 1 : k_end);
+
+        // ---- keys -------------------------------------------------------------------------------------------------------
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        auto block = [&](const WmKeys& x, int at) {                      // keys at .. at + 15
+            float* dst = a.scores + (row0 + at + g) * pad + 2 * c;
+            // rows g and g + 8 of a product: value and remainder of key g (d), of key g + 8 (e); a lookup's two words are then neighbouring
+            // operand registers (with keys as all sixteen rows, 64 register moves per block)
+            float d[4], e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a0 = ws_signs2(x.s0 >> (4 * i)), a1 = ws_signs2(x.s1 >> (4 * i)), a2 = ws_signs2(x.s0 >> (4 * i + 2)), a3 = ws_signs2(x.s1 >> (4 * i + 2));
-                wm_mma(s, a0, a1, a2, a3, pv[i][0], pv[i][1]);
-                wm_mma(t, a0, a1, a2, a3, pr[i][0], pr[i][1]);
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t u0 = w == 0 ? x.n0.x : w == 1 ? x.n0.y : w == 2 ? x.n0.z : x.n0.w;
+                const uint32_t u1 = w == 0 ? x.n1.x : w == 1 ? x.n1.y : w == 2 ? x.n1.z : x.n1.w;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int ks = 2 * w + k;
+                    const uint2 t0 = look(u0, 2 * k), t1 = look(u0, 2 * k + 1), t2 = look(u1, 2 * k), t3 = look(u1, 2 * k + 1);
+                    if (ks == 0) {
+                        wm_mma0(d, t0.x, t0.y, t1.x, t1.y, qv[ks][0], qv[ks][1]);
+                        wm_mma0(e, t2.x, t2.y, t3.x, t3.y, qv[ks][0], qv[ks][1]);
+                    } else {
+                        wm_mma(d, t0.x, t0.y, t1.x, t1.y, qv[ks][0], qv[ks][1]);
+                        wm_mma(e, t2.x, t2.y, t3.x, t3.y, qv[ks][0], qv[ks][1]);
+                    }
+                    if (QLO) {
+                        wm_mma(d, t0.x, t0.y, t1.x, t1.y, qr[ks][0], qr[ks][1]);
+                        wm_mma(e, t2.x, t2.y, t3.x, t3.y, qr[ks][0], qr[ks][1]);
+                    }
+                }
+            }
+            d[0] = (d[0] + d[2]) * f_cb[0];
+            d[1] = (d[1] + d[3]) * f_cb[1];
+            d[2] = (e[0] + e[2]) * f_cb[0];
+            d[3] = (e[1] + e[3]) * f_cb[1];
+            if (a.with_qjl) {
+                float s[4], t[4];
+                const uint32_t z0 = __byte_perm(x.s0, 0, 0x4140), z1 = __byte_perm(x.s1, 0, 0x4140);    // bits 0-7 and 8-15 to the halves
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t a0 = wm_sign_pair(z0, 2 * i), a1 = wm_sign_pair(z1, 2 * i), a2 = wm_sign_pair(z0, 2 * i + 1), a3 = wm_sign_pair(z1, 2 * i + 1);
+                    if (i == 0) {
+                        wm_mma0(s, a0, a1, a2, a3, pv[i][0], pv[i][1]);
+                        wm_mma0(t, a0, a1, a2, a3, pr[i][0], pr[i][1]);
+                    } else {
+                        wm_mma(s, a0, a1, a2, a3, pv[i][0], pv[i][1]);
+                        wm_mma(t, a0, a1, a2, a3, pr[i][0], pr[i][1]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = fmaf((s[i] + t[i]) * f_sg[i & 1], i < 2 ? x.r0 : x.r1, d[i]);
+            }
+            if (at + 16 > open_to) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at + g + (i < 2 ? 0 : 8) > last[i & 1]) d[i] = -INFINITY;
+            }
+            if (2 * c < cols) {
+                if (at + g < k_end) *reinterpret_cast<float2*>(dst) = make_float2(d[0], d[1]);
+                if (at + g + 8 < k_end) *reinterpret_cast<float2*>(dst + 8 * pad) = make_float2(d[2], d[3]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = fmaf((s[i] + t[i]) * f_sg[i & 1], i < 2 ? x.r0 : x.r1, d[i]);
+            for (int i = 0; i < 2; ++i) {
+                // NaN scores: fmaxf drops them, the sum keeps them
+                const float m_new = fmaxf(m[i], fmaxf(d[i], d[i + 2]));
+                const float ref = m_new == -INFINITY ? 0.f : m_new;
+                l[i] = l[i] * ws_ex2(m[i] - ref) + (ws_ex2(d[i] - ref) + ws_ex2(d[i + 2] - ref));
+                m[i] = m_new;
+            }
+        };
+        WmKeys other;
+        other.s0 = other.s1 = 0; other.r0 = other.r1 = 0.f;
+        while (k0 < k_end) {                                             // two sets of registers in turn: copying one costs a dozen moves
+            k0 += kWsTile;
+            if (k0 < k_end) load(other);
+            block(next, k0 - kWsTile);
+            if (k0 >= k_end) break;
+            k0 += kWsTile;
+            if (k0 < k_end) load(next);
+            block(other, k0 - kWsTile);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = k0 + g + (i < 2 ? 0 : 8);
-            if (key > last[i & 1] || key >= k_end) d[i] = -INFINITY;
-        }
-        if (2 * c < cols) {
-            float* dst = a.scores + (row0 + k0 + g) * pad + 2 * c;
-            if (k0 + g < k_end) *reinterpret_cast<float2*>(dst) = make_float2(d[0], d[1]);
-            if (k0 + g + 8 < k_end) *reinterpret_cast<float2*>(dst + 8 * pad) = make_float2(d[2], d[3]);
-        }
+        // ---- this warp's maximum and sum per column of the span -----------------------------------------------------------------
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            // NaN scores: fmaxf drops them, the sum keeps them
-            const float m_new = fmaxf(m[i], fmaxf(d[i], d[i + 2]));
-            const float ref = m_new == -INFINITY ? 0.f : m_new;
-            l[i] = l[i] * ws_ex2(m[i] - ref) + (ws_ex2(d[i] - ref) + ws_ex2(d[i + 2] - ref));
-            m[i] = m_new;
+            float top = m[i];
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, s));
+            const float ref = top == -INFINITY ? 0.f : top;
+            float sum = l[i] * ws_ex2(m[i] - ref);
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) sum += __shfl_xor_sync(kFullMask, sum, s);
+            if (g == 0 && 2 * c + i < cols)
+                a.partial[(((int64_t)h * a.B + b + blockIdx.x) * kWmWarps + warp) * cols + 2 * c + i] = make_float2(top, sum);
         }
-    }
-    // ---- the chunk's maximum and sum per column ---------------------------------------------------------------------------
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        float top = m[i];
-#pragma unroll
-        for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, s));
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = l[i] * ws_ex2(m[i] - ref);
-#pragma unroll
-        for (int s = 4; s < 32; s <<= 1) sum += __shfl_xor_sync(kFullMask, sum, s);
-        if (g == 0) part[warp][2 * c + i] = make_float2(top, sum);
-    }
-    __syncthreads();
-    if (tid < cols) {
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWmWarps; ++w) top = fmaxf(top, part[w][tid].x);
-        const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int w = 0; w < kWmWarps; ++w) sum += part[w][tid].y * ws_ex2(part[w][tid].x - ref);
-        a.partial[(bh * a.chunks + chunk) * cols + tid] = make_float2(top, sum);
+        left -= n_span;
+        tile = 0;
+        if (left > 0) {                                                  // the next user with keys, or the next head's first one
+            do {
+                if (++b == a.B) { b = 0; ++h; }
+            } while (ws_len(a, b) == 0);
+        }
     }
 }
 
 // weights of the kept scores: sums[s] (+)= sum_c 2^(score_c - lse_c)
-constexpr int kWfThreads = 256;
-__global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_constant__ WeightArgs a, int pad, int64_t segments) {
+constexpr int kWfThreads = 256, kWfKeys = 2;       // keys per thread
+__global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_constant__ WeightArgs a, int pad, int64_t segments, int64_t ctas) {
     __shared__ float lse[kWsStepCols];
     const int tid = threadIdx.x;
-    const int64_t bh = blockIdx.x / segments, s0 = blockIdx.x % segments * (4 * kWfThreads);
-    const int len = ws_len(a, bh / a.Hkv), cols = a.Hq / a.Hkv * a.T;
+    const int64_t bh = blockIdx.x / segments, s0 = blockIdx.x % segments * (kWfKeys * kWfThreads);
+    const int64_t b = bh / a.Hkv, h = bh % a.Hkv;
+    const int len = ws_len(a, b), cols = a.Hq / a.Hkv * a.T;
+    after_predecessor();
+    float2 v[kWfKeys][kWsStepCols / 2];                                  // the scores, requested before the normalisers are known
+#pragma unroll
+    for (int k = 0; k < kWfKeys; ++k) {
+        const int64_t s = s0 + k * kWfThreads + tid;
+#pragma unroll
+        for (int i = 0; i < kWsStepCols / 2; ++i)
+            v[k][i] = s < len && 2 * i < cols ? *(reinterpret_cast<const float2*>(a.scores + (bh * a.S + s) * pad) + i) : make_float2(-INFINITY, -INFINITY);
+    }
     if (s0 < len) {
-        const int n = (int)((len + a.chunk_keys - 1) / a.chunk_keys);
+        // the entries of the head's spans: of the CTAs whose shares hold its first and its last tile, and those between
+        const int64_t per_head = a.tiles_before[a.B], all = per_head * a.Hkv;
+        const int64_t first = h * per_head + a.tiles_before[b], c0 = ws_cta_of(first, ctas, all);
+        const int n = (int)(ws_cta_of(first + (len + kWsTile - 1) / kWsTile - 1, ctas, all) - c0 + 1) * kWmWarps;
         const int warp = tid >> 5, lane = tid & 31;                      // a warp per column
         if (warp < cols) {
-            const float2* p = a.partial + bh * a.chunks * cols + warp;
+            const float2* p = a.partial + (h * a.B + b + c0) * kWmWarps * cols + warp;
             float m = -INFINITY, l = 0.f;
             for (int i = lane; i < n; i += 32) m = fmaxf(m, p[(int64_t)i * cols].x);
 #pragma unroll
@@ -265,16 +401,15 @@ __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_
         return;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kWfKeys; ++k) {
         const int64_t s = s0 + k * kWfThreads + tid;
         if (s >= a.S) break;
         float total = 0.f;
         if (s < len) {
-            const float2* p = reinterpret_cast<const float2*>(a.scores + (bh * a.S + s) * pad);
-            for (int i = 0; i < cols; i += 2) {
-                const float2 v = __ldg(p + (i >> 1));
-                total += ws_ex2(v.x - lse[i]);
-                if (i + 1 < cols) total += ws_ex2(v.y - lse[i + 1]);
+#pragma unroll
+            for (int i = 0; i < kWsStepCols / 2; ++i) {
+                if (2 * i < cols) total += ws_ex2(v[k][i].x - lse[2 * i]);
+                if (2 * i + 1 < cols) total += ws_ex2(v[k][i].y - lse[2 * i + 1]);
             }
         }
         float* d = a.sums + bh * a.S + s;
@@ -283,25 +418,31 @@ __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_
     }
 }
 
-// keys of a chunk: about two rounds of two CTAs per SM, at least 256 (the prologue of a CTA costs about as much as 128 keys)
-static int64_t wm_chunk_keys(int64_t heads, int64_t S) {
-    const int64_t per = (heads * S + 148 * 4 - 1) / (148 * 4);
-    const int64_t keys = per < 256 ? 256 : (per > 4096 ? 4096 : per);
-    return (keys + 127) / 128 * 128;
+// The CTAs of a call: two per SM, or one per tile where there are fewer
+static int64_t wm_ctas(int64_t heads, int64_t S) {
+    const int64_t tiles = heads * ((S + kWsTile - 1) / kWsTile);
+    return tiles < 148 * 2 ? tiles : 148 * 2;
 }
+static size_t wm_prep_bytes(int64_t heads, bool split) { return (size_t)heads * (split ? kWmPieces<true> : kWmPieces<false>) * 32 * 16; }
+static size_t wm_partial_bytes(int64_t heads, int64_t S, int64_t cols) { return (size_t)(heads + wm_ctas(heads, S)) * kWmWarps * cols * sizeof(float2); }
 
 template <int DT, bool QLO>
 static int32_t launch_weight_step(WeightArgs a, cudaStream_t st) {
-    const int64_t heads = a.B * a.Hkv, segments = (a.S + 4 * kWfThreads - 1) / (4 * kWfThreads);
-    const int pad = (a.Hq / a.Hkv * a.T + 1) & ~1;
-    a.chunk_keys = wm_chunk_keys(heads, a.S);
-    a.chunks = (a.S + a.chunk_keys - 1) / a.chunk_keys;
-    a.scores = reinterpret_cast<float*>(a.partial + heads * a.chunks * (a.Hq / a.Hkv * a.T));
-    OMNI_REQUIRE(heads * a.chunks <= 0x7fffffffLL && heads * segments <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_attn_weight_sums: too many keys");
-    weight_step_kernel<DT, QLO><<<(unsigned)(heads * a.chunks), kWmWarps * 32, kWsLutBytes, st>>>(a, pad);
+    const int64_t heads = a.B * a.Hkv, segments = (a.S + kWfKeys * kWfThreads - 1) / (kWfKeys * kWfThreads), ctas = wm_ctas(heads, a.S), cols = (int64_t)(a.Hq / a.Hkv) * a.T;
+    const int pad = (int)((cols + 1) & ~1);
+    OMNI_REQUIRE(heads * segments <= 0x7fffffffLL && a.B * ((a.S + kWsTile - 1) / kWsTile) <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_attn_weight_sums: too many keys");
+    unsigned char* ws = reinterpret_cast<unsigned char*>(a.partial);     // prepared columns, tiles in front of every user, partial states, scores
+    a.prepared = ws;
+    ws += wm_prep_bytes(heads, QLO);
+    a.tiles_before = reinterpret_cast<int32_t*>(ws);
+    ws += ws_before_bytes(a.B);
+    a.partial = reinterpret_cast<float2*>(ws);
+    a.scores = reinterpret_cast<float*>(ws + wm_partial_bytes(heads, a.S, cols));
+    weight_fragments_kernel<DT, QLO><<<(unsigned)((heads + kWmPrepWarps - 1) / kWmPrepWarps + 1), kWmPrepWarps * 32, 0, st>>>(a);
     OMNI_CUDA(cudaGetLastError());
-    weight_finish_kernel<<<(unsigned)(heads * segments), kWfThreads, 0, st>>>(a, pad, segments);
-    return check_cuda(cudaGetLastError(), "weight_finish_kernel launch");
+    OMNI_CUDA(cudaFuncSetAttribute(weight_step_kernel<QLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWmLutBytes));
+    OMNI_CUDA(launch_early(weight_step_kernel<QLO>, dim3((unsigned)ctas), kWmWarps * 32, kWmLutBytes, st, a, pad));
+    return check_cuda(launch_early(weight_finish_kernel, dim3((unsigned)(heads * segments)), kWfThreads, 0, st, a, pad, segments, ctas), "weight_finish_kernel launch");
 }
 
 }  // namespace omni
@@ -312,8 +453,8 @@ extern "C" size_t omni_attn_weight_sums_workspace_bytes(int64_t B, int32_t Hq, i
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || S <= 0) return 0;
     const size_t heads = (size_t)B * Hkv, cols = (size_t)(Hq / Hkv) * T;
     if (cols > kWsStepCols) return weight_window_workspace(B, Hq, Hkv, T, S);
-    const size_t keys = (size_t)wm_chunk_keys((int64_t)heads, S), chunks = ((size_t)S + keys - 1) / keys;
-    return heads * cols * chunks * sizeof(float2) + heads * S * ((cols + 1) & ~(size_t)1) * sizeof(float);
+    return wm_prep_bytes((int64_t)heads, true) + ws_before_bytes(B) + wm_partial_bytes((int64_t)heads, S, (int64_t)cols) +
+           heads * S * ((cols + 1) & ~(size_t)1) * sizeof(float);
 }
 
 extern "C" int32_t omni_attn_weight_sums(const void* q, int32_t q_dtype, const uint8_t* k_nib, const uint8_t* k_qjl,

@@ -16,11 +16,10 @@ struct WeightArgs {
     int64_t B; int Hq, Hkv, T; int64_t S; float scale;
     int with_qjl, rotate_q, causal, accumulate;
     const uint32_t* g_rows;
-    float2* partial;                               // [B * Hkv][chunks][columns] maximum (base 2) and sum
+    float2* partial;                               // per span and column (and warp): maximum (base 2) and sum
     float* scores;                                 // warp-level kernel: [B * Hkv][S][columns, rounded up to even]
-    int64_t chunk_keys, chunks;
-    int32_t* tiles_before;                         // tcgen05 kernel: [B + 1] tiles of one kv head in front of every user
-    void* prepared;                                // tcgen05 kernel: the columns, ready for tensor memory
+    int32_t* tiles_before;                         // [B + 1] tiles of one kv head in front of every user
+    void* prepared;                                // the columns, ready for registers or tensor memory
     float* sums;
 };
 
@@ -57,9 +56,10 @@ __device__ __forceinline__ uint32_t ws_signs2(uint32_t bits) {
 }
 
 // Centroid table of a head in shared memory: the entry of a code byte holds the fp16 values of both centroids and what they
-// leave, 8 bytes in sixteen copies side by side, one per lane of a half-warp (an 8-byte load is served in two halves), so
-// that lookups never meet in a bank.  256 threads build it; the centroids are scaled by ws_pow2 of the largest, returned.
-constexpr int kWsLutBytes = 256 * 16 * 8;
+// leave, 8 bytes in COPIES copies side by side.  An 8-byte load is served in two half-warps, so sixteen copies (128 bytes per entry,
+// 32 KiB) keep the lanes in banks of their own; thirty-two (256 bytes, 64 KiB) let one byte permutation make a lane's address.
+// 256 threads build it; the centroids are scaled by ws_pow2 of the largest, returned.
+template <int COPIES>
 __device__ __forceinline__ float ws_build_lut(unsigned char* lut, const float* cb, int tid) {
     float top = 0.f;
 #pragma unroll
@@ -69,11 +69,60 @@ __device__ __forceinline__ float ws_build_lut(unsigned char* lut, const float* c
         const float x0 = __ldg(cb + (tid & 15)) * mul, x1 = __ldg(cb + (tid >> 4)) * mul;
         const uint32_t v = ws_half2(x0, x1), r = ws_rest2(x0, x1, v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)                // every thread starts at another copy: the stores of a warp spread over the banks
-            *reinterpret_cast<uint4*>(lut + tid * 128 + 16 * ((k + tid) & 7)) = make_uint4(v, r, v, r);
+        for (int k = 0; k < COPIES / 2; ++k)       // every thread starts at another copy: the stores of a warp spread over the banks
+            *reinterpret_cast<uint4*>(lut + tid * (8 * COPIES) + 16 * ((k + tid) & (COPIES / 2 - 1))) = make_uint4(v, r, v, r);
     }
     return mul;
 }
+
+// The keys of all (user, head) in tiles of 128 lie in one row, which is cut into equal shares, one per CTA: lengths differ, and only the
+// device knows them.  A run of tiles of one head inside a share is a span.  tiles_before[b]: tiles of one kv head of the users in front of
+// b, written by one CTA of WARPS warps of the launch that prepares the columns.
+constexpr int kWsTile = 128;
+template <int WARPS>
+__device__ __forceinline__ void ws_tiles_before(const WeightArgs& a, int tid) {
+    __shared__ int part[WARPS];
+    const int lane = tid & 31, warp = tid >> 5;
+    int before = 0;
+    for (int64_t b0 = 0; b0 <= a.B; b0 += WARPS * 32) {
+        const int64_t b = b0 + tid;
+        const int n = b < a.B ? (ws_len(a, b) + kWsTile - 1) / kWsTile : 0;
+        int upto = n;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int o = __shfl_up_sync(kFullMask, upto, x);
+            if (lane >= x) upto += o;
+        }
+        if (lane == 31) part[warp] = upto;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) upto += part[w];
+            total += part[w];
+        }
+        if (b <= a.B) a.tiles_before[b] = before + upto - n;
+        before += total;
+        __syncthreads();
+    }
+}
+// The last user with at most x / `heads` tiles in front of it, by a warp.
+__device__ __forceinline__ int ws_user_of(const WeightArgs& a, int64_t x, int64_t heads, int lane) {
+    int64_t lo = 0, n = a.B;                       // it lies in [lo, lo + n)
+    while (n > 1) {
+        const int64_t step = (n + 31) / 32, i = lo + lane * step;
+        const bool below = lane == 0 || (i < lo + n && (int64_t)a.tiles_before[i] * heads <= x);
+        const int64_t next = lo + (31 - __clz((int)__ballot_sync(kFullMask, below))) * step;
+        n = lo + n - next < step ? lo + n - next : step;
+        lo = next;
+    }
+    return (int)lo;
+}
+// The CTAs that have a share: no more than there are tiles, so that every CTA between two spans of a head has one of it as well.
+__device__ __forceinline__ int64_t ws_sharers(int64_t ctas, int64_t all) { return ctas < all ? ctas : all; }
+// The CTA of `ctas` launched ones whose share of `all` tiles holds tile x.
+__device__ __forceinline__ int64_t ws_cta_of(int64_t x, int64_t ctas, int64_t all) { return ((x + 1) * ws_sharers(ctas, all) + all - 1) / all - 1; }
+__host__ __device__ __forceinline__ size_t ws_before_bytes(int64_t B) { return ((size_t)(B + 1) * 4 + 15) & ~(size_t)15; }
 
 // tcgen05 kernel for more columns (weight_window.cu)
 int32_t launch_weight_window(WeightArgs a, int q_dtype, int32_t* status, cudaStream_t st);

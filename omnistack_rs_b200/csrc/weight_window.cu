@@ -20,7 +20,7 @@
 
 namespace omni {
 
-constexpr int kWwTile = 128;                       // keys per tile, columns per CTA
+constexpr int kWwTile = kWsTile;                   // keys per tile, columns per CTA
 constexpr int kWwThreads = 640;                    // warps 17-19 only complete the last warpgroup
 // Registers: launched with 96 per thread (61,440); scores go up to 144, dequantisation down to 72, the rest to 48
 // (256 * 144 + 256 * 72 + 128 * 48 = 61,440).
@@ -35,8 +35,9 @@ constexpr float kWwProjMul = 1.f / 128.f;
 constexpr uint32_t kWwLbo = 128;                   // K-major operands: bytes between the two 8-element chunks of a k-step
 constexpr uint32_t kWwSbo = 16 * 128, kWwSboSign = 8 * 128;         // ... and between groups of eight keys
 constexpr uint32_t kWwBytesV = 128 * 128 * 2, kWwBytesSign = 128 * 64 * 2;
+constexpr uint32_t kWwLutBytes = 256 * 16 * 8;
 constexpr uint32_t kWwBuf = 2 * kWwBytesV + kWwBytesSign;           // values, remainders, signs
-constexpr uint32_t kWwOffLut = 2 * kWwBuf, kWwOffNorm = kWwOffLut + kWsLutBytes, kWwOffRed = kWwOffNorm + 4 * kWwTile * 4,
+constexpr uint32_t kWwOffLut = 2 * kWwBuf, kWwOffNorm = kWwOffLut + kWwLutBytes, kWwOffRed = kWwOffNorm + 4 * kWwTile * 4,
                    kWwOffBar = kWwOffRed + 4 * kWwTile * 4, kWwSmem = kWwOffBar + 128;
 constexpr uint32_t kWwColA = 0, kWwColB = 128, kWwColQhi = 256, kWwColQlo = 320, kWwColChi = 384, kWwColClo = 416, kWwTmemCols = 512;
 constexpr uint32_t kWwWaitLimit = 1u << 20;
@@ -139,30 +140,9 @@ __global__ void __launch_bounds__(kWpWarps * 32) weight_prepare_kernel(const __g
     __shared__ __align__(16) float q_s[kWpWarps][kHeadDim];
     __shared__ uint4 g_s[kQjlDim];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (blockIdx.x == gridDim.x - 1) {                                   // tiles of one kv head in front of every user
-        __shared__ int part[kWpWarps];
-        int before = 0;
-        for (int64_t b0 = 0; b0 <= a.B; b0 += kWpWarps * 32) {
-            const int64_t b = b0 + tid;
-            const int n = b < a.B ? (ws_len(a, b) + kWwTile - 1) / kWwTile : 0;
-            int upto = n;
-#pragma unroll
-            for (int x = 1; x < 32; x <<= 1) {
-                const int o = __shfl_up_sync(kFullMask, upto, x);
-                if (lane >= x) upto += o;
-            }
-            if (lane == 31) part[warp] = upto;
-            __syncthreads();
-            int total = 0;
-#pragma unroll
-            for (int w = 0; w < kWpWarps; ++w) {
-                if (w < warp) upto += part[w];
-                total += part[w];
-            }
-            if (b <= a.B) a.tiles_before[b] = before + upto - n;
-            before += total;
-            __syncthreads();
-        }
+    follow_me_early();
+    if (blockIdx.x == gridDim.x - 1) {
+        ws_tiles_before<kWpWarps>(a, tid);
         return;
     }
     const int64_t bh = blockIdx.x / col_groups, b = bh / a.Hkv;
@@ -231,17 +211,9 @@ struct WwPlace {
     __device__ __forceinline__ void user(const WeightArgs& a) { len = ws_len(a, b); n_tiles = (len + kWwTile - 1) / kWwTile; }
     // the place of tile x, by a warp
     __device__ __forceinline__ void find(const WeightArgs& a, int64_t x, int lane) {
-        int64_t lo = 0, n = a.B;                   // the last user with at most x tiles in front of it lies in [lo, lo + n)
-        while (n > 1) {
-            const int64_t step = (n + 31) / 32, i = lo + lane * step;
-            const bool below = lane == 0 || (i < lo + n && (int64_t)__ldg(a.tiles_before + i) * a.Hkv <= x);
-            const int64_t next = lo + (31 - __clz((int)__ballot_sync(kFullMask, below))) * step;
-            n = lo + n - next < step ? lo + n - next : step;
-            lo = next;
-        }
-        b = (int)lo;
+        b = ws_user_of(a, x, a.Hkv, lane);
         user(a);
-        const int64_t in = x - (int64_t)__ldg(a.tiles_before + b) * a.Hkv;
+        const int64_t in = x - (int64_t)a.tiles_before[b] * a.Hkv;
         h = (int)(in / n_tiles);
         tile = (int)(in % n_tiles);
     }
@@ -259,14 +231,17 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
     extern __shared__ __align__(1024) unsigned char ww_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int cols = a.Hq / a.Hkv * a.T;
+    follow_me_early();
+    after_predecessor();
     if (PASS == 2 && !a.accumulate && col0 == 0) {                       // zeros behind the lengths
         for (int64_t bh = blockIdx.x; bh < a.B * a.Hkv; bh += gridDim.x)
             for (int64_t s = ws_len(a, bh / a.Hkv) + tid; s < a.S; s += kWwThreads) a.sums[bh * a.S + s] = 0.f;
     }
-    const int64_t all = (int64_t)__ldg(a.tiles_before + a.B) * a.Hkv;    // this CTA's share: tiles x0 .. x1 - 1
-    const int64_t x0 = blockIdx.x * all / gridDim.x, x1 = (blockIdx.x + 1) * all / gridDim.x;
+    const int64_t all = (int64_t)a.tiles_before[a.B] * a.Hkv;    // this CTA's share: tiles x0 .. x1 - 1
+    const int64_t sharers = ws_sharers(gridDim.x, all);
+    if (blockIdx.x >= sharers) return;
+    const int64_t x0 = blockIdx.x * all / sharers, x1 = (blockIdx.x + 1) * all / sharers;
     const int n_share = (int)(x1 - x0);
-    if (n_share <= 0) return;
     WwPlace at;
     at.find(a, x0, lane);
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(ww_smem);
@@ -363,7 +338,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
         for (int t = 0; t < n_share; ++t) {
             if (new_table) {                                             // no lookup of the previous table is still to come
                 asm volatile("bar.sync 2, 256;\n" ::: "memory");
-                norm_mul = kQjlCoef / kWwProjMul * ws_build_lut(ww_smem + kWwOffLut, a.codebooks + (a.cb_per_head ? at.h * 16 : 0), tid - 256);
+                norm_mul = kQjlCoef / kWwProjMul * ws_build_lut<16>(ww_smem + kWwOffLut, a.codebooks + (a.cb_per_head ? at.h * 16 : 0), tid - 256);
                 asm volatile("bar.sync 2, 256;\n" ::: "memory");
             }
             if (ok && t > 1) ok = ww_bar_wait(bar_empty + 8 * (t & 1), ((t >> 1) - 1) & 1);
@@ -414,14 +389,14 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             const int n_span = at.n_tiles - at.tile < n_share - done ? at.n_tiles - at.tile : n_share - done;
             float* sums = a.sums + bh * a.S;
             const unsigned char* prep = reinterpret_cast<const unsigned char*>(a.prepared) + (bh * ((cols + kWwTile - 1) / kWwTile) + col0 / kWwTile) * kWwPrepBytes;
-            const float f = col_on ? __ldg(reinterpret_cast<const float*>(prep + (size_t)kWwPrepRows * kWwTile * 16) + row) : 1.f;
+            const float f = col_on ? reinterpret_cast<const float*>(prep + (size_t)kWwPrepRows * kWwTile * 16)[row] : 1.f;
             // Q' of the columns into tensor memory, half of each part per thread, once no product of the previous span reads it
             if (ok && done > 0) ok = ww_bar_wait(bar_empty + 8 * ((done - 1) & 1), ((done - 1) >> 1) & 1);
             ww_fence_after();
             {
                 const uint4* src = reinterpret_cast<const uint4*>(prep) + row;
                 auto piece = [&](int r, uint32_t* dst) {
-                    const uint4 x = col_on ? __ldg(src + (size_t)r * kWwTile) : make_uint4(0u, 0u, 0u, 0u);
+                    const uint4 x = col_on ? src[(size_t)r * kWwTile] : make_uint4(0u, 0u, 0u, 0u);
                     dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w;
                 };
                 uint32_t v[32], r[32], p[16], o[16];
@@ -451,8 +426,8 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             float m = -INFINITY, l = 0.f, lse = 0.f;
             if (PASS == 2 && col_on) {
                 // the head's spans: the CTAs whose shares hold its first and its last tile, and those between
-                const int64_t first = ((int64_t)__ldg(a.tiles_before + at.b)) * a.Hkv + (int64_t)at.h * at.n_tiles;
-                const int64_t c0 = ((first + 1) * gridDim.x + all - 1) / all - 1, c1 = ((first + at.n_tiles) * gridDim.x + all - 1) / all - 1;
+                const int64_t first = ((int64_t)a.tiles_before[at.b]) * a.Hkv + (int64_t)at.h * at.n_tiles;
+                const int64_t c0 = ws_cta_of(first, gridDim.x, all), c1 = ws_cta_of(first + at.n_tiles - 1, gridDim.x, all);
                 const float2* p = a.partial + (bh + c0) * cols + col;
                 for (int64_t i = 0; i <= c1 - c0; ++i) m = fmaxf(m, p[i * cols].x);
                 const float ref = m == -INFINITY ? 0.f : m;
@@ -585,11 +560,10 @@ static int64_t ww_ctas(int64_t heads, int64_t S) {
     const int64_t tiles = heads * ((S + kWwTile - 1) / kWwTile);
     return tiles < 148 ? tiles : 148;
 }
-static size_t ww_before_bytes(int64_t B) { return ((size_t)(B + 1) * 4 + 15) & ~(size_t)15; }
 
 size_t weight_window_workspace(int64_t B, int Hq, int Hkv, int T, int64_t S) {
     const int64_t heads = B * Hkv, cols = (int64_t)(Hq / Hkv) * T, col_tiles = (cols + kWwTile - 1) / kWwTile;
-    return (size_t)(heads * col_tiles) * kWwPrepBytes + ww_before_bytes(B) + (size_t)(heads + ww_ctas(heads, S)) * cols * sizeof(float2);
+    return (size_t)(heads * col_tiles) * kWwPrepBytes + ws_before_bytes(B) + (size_t)(heads + ww_ctas(heads, S)) * cols * sizeof(float2);
 }
 
 template <bool QLO>
@@ -599,9 +573,8 @@ static int32_t launch_weight_window_t(const WeightArgs& a, unsigned grid, int32_
     OMNI_CUDA(cudaFuncSetAttribute(weight_window_kernel<QLO, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWwSmem));
     for (int pass = 1; pass <= 2; ++pass) {
         for (int col0 = 0; col0 < cols; col0 += kWwTile) {
-            if (pass == 1) weight_window_kernel<QLO, 1><<<grid, kWwThreads, kWwSmem, st>>>(a, col0, status);
-            else weight_window_kernel<QLO, 2><<<grid, kWwThreads, kWwSmem, st>>>(a, col0, status);
-            OMNI_CUDA(cudaGetLastError());
+            if (pass == 1) OMNI_CUDA(launch_early(weight_window_kernel<QLO, 1>, dim3(grid), kWwThreads, kWwSmem, st, a, col0, status));
+            else OMNI_CUDA(launch_early(weight_window_kernel<QLO, 2>, dim3(grid), kWwThreads, kWwSmem, st, a, col0, status));
         }
     }
     return OMNI_OK;
@@ -615,7 +588,7 @@ int32_t launch_weight_window(WeightArgs a, int q_dtype, int32_t* status, cudaStr
     a.prepared = ws;
     ws += (size_t)(heads * ((cols + kWwTile - 1) / kWwTile)) * kWwPrepBytes;
     a.tiles_before = reinterpret_cast<int32_t*>(ws);
-    a.partial = reinterpret_cast<float2*>(ws + ww_before_bytes(a.B));
+    a.partial = reinterpret_cast<float2*>(ws + ws_before_bytes(a.B));
     const unsigned grid = (unsigned)(heads * col_groups) + 1;
     switch (q_dtype) {
         case OMNI_F32:  weight_prepare_kernel<OMNI_F32><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;

@@ -90,6 +90,22 @@ def test_scales_without_a_sign_of_their_own(scale):
         check(got, q, (nib, qjl, norms), cb, [5], [140], True, True, scale)
 
 
+def test_few_tiles_for_many_ctas():
+    """Most users empty, the others short: more CTAs than tiles.  Scratch memory holds whatever it held before."""
+    from omnistack_rs_b200.kernels.eviction import attn_weight_sums
+    nib, qjl, norms, cb = packed(12, 2, 600, seed=21)
+    lens = [0, 0, 130, 0, 1, 0, 0, 0, 600, 0, 3, 0]
+    dev = [x.to(DEV) for x in (nib, qjl, norms, cb)]
+    for T in (1, 12):
+        q = torch.randn(12, 4, T, 128, generator=torch.Generator().manual_seed(T))
+        for fill in (1e30, float("nan")):
+            torch.cuda.synchronize()
+            trash = [torch.full((1 << 20,), fill, device=DEV) for _ in range(16)]
+            del trash
+            got = attn_weight_sums(q.to(DEV), *dev, user_id=9, seq_lens=torch.tensor(lens, device=DEV))
+            check(got, q, (nib, qjl, norms), cb, [9] * 12, lens, True, True)
+
+
 def test_nan_behind_the_length_is_not_read():
     from omnistack_rs_b200.kernels.eviction import attn_weight_sums
     nib, qjl, norms, cb = packed(1, 1, 100, seed=6)

@@ -15,6 +15,7 @@
 #include "prompt.cuh"
 #include <cuda.h>
 #include <mutex>
+#include <type_traits>
 
 namespace omni {
 
@@ -30,6 +31,7 @@ constexpr uint32_t kPuOffBar = kPuOffK + kPuStages * kPuTile;
 constexpr uint32_t kPuSmem = kPuOffBar + 256 + 1024;       // barriers, and room to start on a 1,024-byte boundary
 constexpr uint32_t kPuColS = 0, kPuColO = 256, kPuTmemCols = 512;
 constexpr uint32_t kPuWaitLimit = 1u << 20;
+constexpr int kPuPoly = 4;
 constexpr float kPuLog2e = 1.4426950408889634f;
 
 // ---- PTX wrappers --------------------------------------------------------------------------------
@@ -112,6 +114,57 @@ __device__ __forceinline__ float pu_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+// two fp32 operations in one instruction, on register pairs
+__device__ __forceinline__ uint64_t pu_pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 pu_parts(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t pu_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pu_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float pu_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x for a pair, on the FP32 units: x = n + f with n the nearest integer, 2^f by a polynomial with the smallest largest relative error on
+// [-1/2, 1/2] (found by exchange of its extrema: 2^-13.7 at degree 3, an eighth of a bf16 rounding; 2^-18.6 at degree 4 for fp16), n added
+// to the exponent.  x is at most 16 here; below -126 it counts as -126, and a NaN does not come through (see `odd` below).
+template <int DT> __device__ __forceinline__ float2 pu_exp2_pair(uint64_t x) {
+    const float magic = 12582912.f;                // 1.5 * 2^23: adding it rounds to an integer, in the sum's low bits
+    const float2 u = pu_parts(x);
+    const uint64_t v = pu_pair(fmaxf(u.x, -126.f), fmaxf(u.y, -126.f));
+    const uint64_t t = pu_add2(v, pu_pair(magic, magic));
+    const uint64_t n = pu_add2(t, pu_pair(-magic, -magic));
+    const uint64_t f = pu_fma2(n, pu_pair(-1.f, -1.f), v);
+    uint64_t p;
+    if constexpr (DT == OMNI_BF16) {
+        p = pu_fma2(f, pu_pair(0.05517167f, 0.05517167f), pu_pair(0.24261113f, 0.24261113f));
+        p = pu_fma2(p, f, pu_pair(0.69326097f, 0.69326097f));
+        p = pu_fma2(p, f, pu_pair(0.99992806f, 0.99992806f));
+    } else {
+        p = pu_fma2(f, pu_pair(0.0095701021f, 0.0095701021f), pu_pair(0.055917859f, 0.055917859f));
+        p = pu_fma2(p, f, pu_pair(0.24024744f, 0.24024744f));
+        p = pu_fma2(p, f, pu_pair(0.69312179f, 0.69312179f));
+        p = pu_fma2(p, f, pu_pair(0.99999928f, 0.99999928f));
+    }
+    const float2 tv = pu_parts(t), pv = pu_parts(p);
+    return make_float2(__uint_as_float(__float_as_uint(tv.x) * 8388608u + __float_as_uint(pv.x)),
+                       __uint_as_float(__float_as_uint(tv.y) * 8388608u + __float_as_uint(pv.y)));
+}
 template <int DT> __device__ __forceinline__ uint32_t pu_pack(float lo, float hi) {
     uint32_t r;
     if constexpr (DT == OMNI_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
@@ -177,12 +230,13 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
     const uint32_t base = ((uint32_t)__cvta_generic_to_shared(pu_smem) + 1023u) & ~1023u;
     const uint32_t sQ = base, sKV = base + kPuOffK, bars = base + kPuOffBar;
     const uint32_t bar_q = bars, bar_full = bars + 16, bar_empty = bar_full + 8 * kPuStages, bar_s = bar_empty + 8 * kPuStages, bar_p = bar_s + 16,
-                   bar_o = bar_p + 16, tmem_at = bar_o + 16;
+                   bar_h = bar_p + 16, bar_o = bar_h + 16, tmem_at = bar_o + 16;
     if (tid == 0) {
         for (int x = 0; x < 2; ++x) {
             pu_bar_init(bar_q + 8 * x, 1);
             pu_bar_init(bar_s + 8 * x, 1);
             pu_bar_init(bar_p + 8 * x, 4);
+            pu_bar_init(bar_h + 8 * x, 4);
             pu_bar_init(bar_o + 8 * x, 1);
         }
         for (int i = 0; i < kPuStages; ++i) {
@@ -232,7 +286,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             auto issue_s = [&](int x, uint32_t sK) {
                 if (pu_elect()) {
                     const uint32_t da = pu_desc(sQ + x * kPuTile, 16), db = pu_desc(sK, 16);
-    #pragma unroll
+#pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
                         const uint32_t off = ((ks >> 2) * kPuHalf + (ks & 3) * 32) >> 4;
                         pu_mma_ss(tmem + kPuColS + 128 * x, da + off, db + off, pu_idesc<DT>(false), ks > 0);
@@ -257,19 +311,25 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                 if (++st == kPuStages) { st = 0; ph ^= 1u; }                 // K_{j+1}
                 if (ok && j + 1 < n_all) ok = pu_bar_wait_warp(bar_full + 8 * st, ph);
                 const uint32_t sV = sKV + stv * kPuTile, sK = sKV + st * kPuTile;
-    #pragma unroll 1
+#pragma unroll 1
                 for (int x = 0; ok && x < 2; ++x) {
                     if (j >= n_blocks[x]) continue;
-                    ok = pu_bar_wait_warp(bar_p + 8 * x, j & 1);
-                    if (!ok) break;
-                    pu_fence_after();
-                    if (pu_elect()) {
-                        const uint32_t db = pu_desc(sV, kPuHalf), dd = tmem + kPuColO + 128 * x, da = tmem + kPuColS + 128 * x;
-    #pragma unroll
-                        for (int ks = 0; ks < 8; ++ks) pu_mma_ts(dd, da + 8 * ks, db + ks * (2048 >> 4), pu_idesc<DT>(true), (j > 0 || ks > 0) ? 1u : 0u);
-                        if (j + 1 >= n_blocks[x]) pu_commit(bar_o + 8 * x);
+                    // the weights come in halves: the product over keys 0-63 runs while the softmax works on the rest
+#pragma unroll
+                    for (int half = 0; half < 2 && ok; ++half) {
+                        ok = pu_bar_wait_warp((half ? bar_p : bar_h) + 8 * x, j & 1);
+                        if (!ok) break;
+                        pu_fence_after();
+                        if (pu_elect()) {
+                            const uint32_t db = pu_desc(sV, kPuHalf), dd = tmem + kPuColO + 128 * x, da = tmem + kPuColS + 128 * x;
+#pragma unroll
+                            for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
+                                pu_mma_ts(dd, da + 8 * ks, db + ks * (2048 >> 4), pu_idesc<DT>(true), (j > 0 || ks > 0) ? 1u : 0u);
+                            if (half == 1 && j + 1 >= n_blocks[x]) pu_commit(bar_o + 8 * x);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
                     if (j + 1 < n_blocks[x]) issue_s(x, sK);
                 }
                 if (ok && pu_elect()) {
@@ -292,6 +352,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
         const int n_free = a.causal ? w.t0 + x * tt + 1 : w.len;         // keys below this are open to every row of the tile
         const float c = a.scale * kPuLog2e;
         float m = -INFINITY, l = 0.f;                                    // m: in units of c * score
+        uint64_t odd = pu_pair(0.f, 0.f);                                // zero times the scores that the polynomial took
         for (int j = 0; j < n_blocks[x]; ++j) {
             ok = pu_bar_wait_warp(bar_s + 8 * x, j & 1);
             if (!ok) break;
@@ -307,9 +368,9 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 128; i += 4) {
+            for (int i = 0; i < 128; i += 8) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(s[i + k]));
+                for (int k = 0; k < 4; ++k) mx[k] = pu_max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
             }
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
             const bool raise = top > m + kSlack;
@@ -330,33 +391,47 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                     }
                 }
             }
-            const float neg = kBias - m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t c2 = pu_pair(c, c), neg2 = pu_pair(kBias - m, kBias - m);
+            uint64_t sum[2] = {pu_pair(0.f, 0.f), pu_pair(0.f, 0.f)};
+            auto weights = [&](auto masked) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t p[32];
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t p[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float p0 = pu_ex2(fmaf(__uint_as_float(s[64 * h + 2 * i]), c, neg));
-                    const float p1 = pu_ex2(fmaf(__uint_as_float(s[64 * h + 2 * i + 1]), c, neg));
-                    sum[(2 * i) & 3] += p0;
-                    sum[(2 * i + 1) & 3] += p1;
-                    p[i] = pu_pack<DT>(p0, p1);
+                    for (int i = 0; i < 32; ++i) {
+                        const uint64_t raw = pu_pair(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1]));
+                        const uint64_t x2 = pu_fma2(raw, c2, neg2);
+                        float2 e;
+                        // every kPuPoly-th pair on the FP32 units, the rest on the special function unit; masked blocks have exact zeros
+                        if (!decltype(masked)::value && i % kPuPoly == kPuPoly - 1) {
+                            e = pu_exp2_pair<DT>(x2);
+                            odd = pu_fma2(raw, pu_pair(0.f, 0.f), odd);          // NaN or infinite scores make the row's sum NaN
+                        } else {
+                            const float2 v = pu_parts(x2);
+                            e = make_float2(pu_ex2(v.x), pu_ex2(v.y));
+                        }
+                        sum[i & 1] = pu_add2(sum[i & 1], pu_pair(e.x, e.y));
+                        p[i] = pu_pack<DT>(e.x, e.y);
+                    }
+                    pu_st32(t_s + 32 * h, p);
+                    pu_wait_st();
+                    pu_fence_before();
+                    __syncwarp();
+                    if (lane == 0) pu_bar_arrive((h ? bar_p : bar_h) + 8 * x);
                 }
-                pu_st32(t_s + 32 * h, p);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            pu_wait_st();
-            pu_fence_before();
-            __syncwarp();
-            if (lane == 0) pu_bar_arrive(bar_p + 8 * x);
+            };
+            if (128 * j + 128 > n_free) weights(std::true_type{});
+            else weights(std::false_type{});
+            const float2 both = pu_parts(pu_add2(sum[0], sum[1]));
+            l += both.x + both.y;
         }
         // ---- result rows ---------------------------------------------------------------------------------------------
         if (n_blocks[x] > 0) {
             if (ok) ok = pu_bar_wait_warp(bar_o + 8 * x, 0);
             if (ok) {
                 pu_fence_after();
-                const float inv = 1.f / l;
+                const float2 odd2 = pu_parts(odd);
+                const float inv = 1.f / (l + (odd2.x + odd2.y));
                 uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) +
                                                       ((w.b * a.Hq + head0 + (live ? g : 0)) * a.T + w.row0 + (live ? t : w.t0)) * kHeadDim);
                 bool bad = false;

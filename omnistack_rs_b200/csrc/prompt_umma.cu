@@ -10,12 +10,16 @@
 // A block's maximum only replaces the running one when it exceeds it by 2^slack, so O is rescaled rarely; the softmax threads
 // do it themselves: S_t of a block is issued behind P_t V of the block before, so its arrival says that O_t is complete.
 //
+// What bounds it: the chain of one tile, scores (512 cycles) - softmax (about 1,900) - product (512), two tiles deep, and on long prompts
+// the board's power: 16,384 tokens of 32 heads in fp16 take 1.80 ms, 1,220 TFLOP/s at about 1.62 GHz under the 1,000 W cap, 75 % of the
+// measured burst rate of a plain matrix product and 87 % of its sustained one.  A quarter of the exponentials as a polynomial on the
+// FP32 units (1.84 ms) or a third (1.90 ms) gained nothing.
+//
 // A zero weight times an infinite or NaN value of a masked key would be NaN.  Rows that come out NaN are therefore formed
 // again from global memory over their own keys alone (prompt_row_again), which settles NaN that belong there too.
 #include "prompt.cuh"
 #include <cuda.h>
 #include <mutex>
-#include <type_traits>
 
 namespace omni {
 
@@ -31,7 +35,6 @@ constexpr uint32_t kPuOffBar = kPuOffK + kPuStages * kPuTile;
 constexpr uint32_t kPuSmem = kPuOffBar + 256 + 1024;       // barriers, and room to start on a 1,024-byte boundary
 constexpr uint32_t kPuColS = 0, kPuColO = 256, kPuTmemCols = 512;
 constexpr uint32_t kPuWaitLimit = 1u << 20;
-constexpr int kPuPoly = 4;
 constexpr float kPuLog2e = 1.4426950408889634f;
 
 // ---- PTX wrappers --------------------------------------------------------------------------------
@@ -139,31 +142,6 @@ __device__ __forceinline__ float pu_max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-// 2^x for a pair, on the FP32 units: x = n + f with n the nearest integer, 2^f by a polynomial with the smallest largest relative error on
-// [-1/2, 1/2] (found by exchange of its extrema: 2^-13.7 at degree 3, an eighth of a bf16 rounding; 2^-18.6 at degree 4 for fp16), n added
-// to the exponent.  x is at most 16 here; below -126 it counts as -126, and a NaN does not come through (see `odd` below).
-template <int DT> __device__ __forceinline__ float2 pu_exp2_pair(uint64_t x) {
-    const float magic = 12582912.f;                // 1.5 * 2^23: adding it rounds to an integer, in the sum's low bits
-    const float2 u = pu_parts(x);
-    const uint64_t v = pu_pair(fmaxf(u.x, -126.f), fmaxf(u.y, -126.f));
-    const uint64_t t = pu_add2(v, pu_pair(magic, magic));
-    const uint64_t n = pu_add2(t, pu_pair(-magic, -magic));
-    const uint64_t f = pu_fma2(n, pu_pair(-1.f, -1.f), v);
-    uint64_t p;
-    if constexpr (DT == OMNI_BF16) {
-        p = pu_fma2(f, pu_pair(0.05517167f, 0.05517167f), pu_pair(0.24261113f, 0.24261113f));
-        p = pu_fma2(p, f, pu_pair(0.69326097f, 0.69326097f));
-        p = pu_fma2(p, f, pu_pair(0.99992806f, 0.99992806f));
-    } else {
-        p = pu_fma2(f, pu_pair(0.0095701021f, 0.0095701021f), pu_pair(0.055917859f, 0.055917859f));
-        p = pu_fma2(p, f, pu_pair(0.24024744f, 0.24024744f));
-        p = pu_fma2(p, f, pu_pair(0.69312179f, 0.69312179f));
-        p = pu_fma2(p, f, pu_pair(0.99999928f, 0.99999928f));
-    }
-    const float2 tv = pu_parts(t), pv = pu_parts(p);
-    return make_float2(__uint_as_float(__float_as_uint(tv.x) * 8388608u + __float_as_uint(pv.x)),
-                       __uint_as_float(__float_as_uint(tv.y) * 8388608u + __float_as_uint(pv.y)));
 }
 template <int DT> __device__ __forceinline__ uint32_t pu_pack(float lo, float hi) {
     uint32_t r;
@@ -352,7 +330,6 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
         const int n_free = a.causal ? w.t0 + x * tt + 1 : w.len;         // keys below this are open to every row of the tile
         const float c = a.scale * kPuLog2e;
         float m = -INFINITY, l = 0.f;                                    // m: in units of c * score
-        uint64_t odd = pu_pair(0.f, 0.f);                                // zero times the scores that the polynomial took
         for (int j = 0; j < n_blocks[x]; ++j) {
             ok = pu_bar_wait_warp(bar_s + 8 * x, j & 1);
             if (!ok) break;
@@ -393,35 +370,22 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             }
             const uint64_t c2 = pu_pair(c, c), neg2 = pu_pair(kBias - m, kBias - m);
             uint64_t sum[2] = {pu_pair(0.f, 0.f), pu_pair(0.f, 0.f)};
-            auto weights = [&](auto masked) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32];
+            for (int h = 0; h < 2; ++h) {
+                uint32_t p[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const uint64_t raw = pu_pair(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1]));
-                        const uint64_t x2 = pu_fma2(raw, c2, neg2);
-                        float2 e;
-                        // every kPuPoly-th pair on the FP32 units, the rest on the special function unit; masked blocks have exact zeros
-                        if (!decltype(masked)::value && i % kPuPoly == kPuPoly - 1) {
-                            e = pu_exp2_pair<DT>(x2);
-                            odd = pu_fma2(raw, pu_pair(0.f, 0.f), odd);          // NaN or infinite scores make the row's sum NaN
-                        } else {
-                            const float2 v = pu_parts(x2);
-                            e = make_float2(pu_ex2(v.x), pu_ex2(v.y));
-                        }
-                        sum[i & 1] = pu_add2(sum[i & 1], pu_pair(e.x, e.y));
-                        p[i] = pu_pack<DT>(e.x, e.y);
-                    }
-                    pu_st32(t_s + 32 * h, p);
-                    pu_wait_st();
-                    pu_fence_before();
-                    __syncwarp();
-                    if (lane == 0) pu_bar_arrive((h ? bar_p : bar_h) + 8 * x);
+                for (int i = 0; i < 32; ++i) {
+                    const float2 v = pu_parts(pu_fma2(pu_pair(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1])), c2, neg2));
+                    const float2 e = make_float2(pu_ex2(v.x), pu_ex2(v.y));
+                    sum[i & 1] = pu_add2(sum[i & 1], pu_pair(e.x, e.y));
+                    p[i] = pu_pack<DT>(e.x, e.y);
                 }
-            };
-            if (128 * j + 128 > n_free) weights(std::true_type{});
-            else weights(std::false_type{});
+                pu_st32(t_s + 32 * h, p);
+                pu_wait_st();
+                pu_fence_before();
+                __syncwarp();
+                if (lane == 0) pu_bar_arrive((h ? bar_p : bar_h) + 8 * x);
+            }
             const float2 both = pu_parts(pu_add2(sum[0], sum[1]));
             l += both.x + both.y;
         }
@@ -430,8 +394,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             if (ok) ok = pu_bar_wait_warp(bar_o + 8 * x, 0);
             if (ok) {
                 pu_fence_after();
-                const float2 odd2 = pu_parts(odd);
-                const float inv = 1.f / (l + (odd2.x + odd2.y));
+                const float inv = 1.f / l;
                 uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) +
                                                       ((w.b * a.Hq + head0 + (live ? g : 0)) * a.T + w.row0 + (live ? t : w.t0)) * kHeadDim);
                 bool bad = false;

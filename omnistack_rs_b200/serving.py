@@ -17,7 +17,9 @@ import torch
 
 from . import _lib
 from .kernels.quantize import _NBYTES_NIBBLE, _NBYTES_QJL, _codec_rows, _prep_codebooks, _user_args, rotate_quantize_append
+from .kernels.eviction import EvictedCache, attn_weight_sums, evict_keys
 from .kernels.fused_attention import _qattn, _auto_splits, pair_v_rows
+from .kernels.prompt_attention import prompt_attn
 
 HEAD_DIM = 128
 
@@ -142,6 +144,7 @@ class QuantizedKVCache:
         self.lens32 = torch.zeros(n_users, dtype=torch.int32, device=self.device)
         self.user_ids = (torch.arange(n_users, dtype=torch.int32, device=self.device) if user_ids is None
                          else user_ids.to(device=self.device, dtype=torch.int32).contiguous())
+        self.weight_sums: Optional[torch.Tensor] = None     # accumulated attention weight per key (see observe)
 
     def bytes_per_key(self) -> int:
         return 2 * (_NBYTES_NIBBLE + _NBYTES_QJL + 4) if self.v_qjl is not None else 2 * _NBYTES_NIBBLE + _NBYTES_QJL + 4
@@ -199,6 +202,62 @@ class QuantizedKVCache:
                 _lib.ptr(self.k_nib), _lib.ptr(self.k_qjl), _lib.ptr(self.k_norms), _lib.ptr(self.v_nib), _lib.ptr(self.v_qjl),
                 _lib.ptr(self.v_norms), S, _lib.ptr(self.lens), _lib.ptr(self.lens32), int(self.pair_v), _lib.stream_ptr(dev)))
         return True
+
+    def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompt_lens: Optional[torch.Tensor] = None, *,
+                causal: bool = True, scale: Optional[float] = None, rotate: bool = True) -> torch.Tensor:
+        """Take in every user's prompt: ``prompt_attn`` of ``q`` (n_users, n_heads, T, 128) over ``k`` and ``v`` (n_users,
+        n_kv_heads, T, 128) in full precision, and the keys and values packed into the (empty) cache.  ``prompt_lens`` (n_users,):
+        user b's prompt is its first ``prompt_lens[b]`` rows; the others are neither attended to nor kept.  Returns the
+        attention's result, zeros in the rows behind a prompt."""
+        T = k.shape[2]
+        lens = None
+        if prompt_lens is not None:
+            if prompt_lens.shape != (self.n_users,):
+                raise ValueError(f"prompt_lens must have shape ({self.n_users},), got {tuple(prompt_lens.shape)}")
+            lens = prompt_lens.to(device=self.device, dtype=torch.int64)
+            lo, hi = _lib.index_range(lens) if self.n_users else (0, 0)
+            if lo < 0 or hi > T:
+                raise ValueError(f"prompt_lens must lie in [0, {T}]")
+        if self.n_users and _lib.index_range(self.lens) != (0, 0):
+            raise ValueError("prefill takes whole prompts: the cache already holds keys")
+        out = prompt_attn(q, k, v, seq_lens=lens, causal=causal, scale=scale)
+        self.append(k, v, rotate=rotate)
+        if lens is not None:
+            if self.pair_v:                        # groups that are not complete below the prompt's length go back to single rows
+                pair_v_rows(self.v_nib, lens, self.lens)
+            self.lens.copy_(lens)
+            self.lens32.copy_(lens)
+        return out
+
+    def observe(self, q: torch.Tensor, scale: Optional[float] = None, with_qjl: bool = True, rotate_q: bool = False,
+                causal: bool = True) -> torch.Tensor:
+        """Add the attention weight that every cached key receives from ``q`` (n_users, n_heads, T, 128), the queries of the last T
+        tokens, to ``weight_sums`` (float32 (n_users, n_kv_heads, max_len), kept from the first call on), which decides what
+        :meth:`evict` keeps.  Arguments as in :meth:`attend`; returns ``weight_sums``."""
+        if self.weight_sums is None:
+            self.weight_sums = torch.zeros(self.n_users, self.n_kv_heads, self.max_len, dtype=torch.float32, device=self.device)
+        return attn_weight_sums(q, self.k_nib, self.k_qjl, self.k_norms, self.codebooks, self.user_ids, scale, with_qjl,
+                                seq_lens=self.lens32, rotate_q=rotate_q, causal=causal, into=self.weight_sums)
+
+    def evict(self, budget: int, recent: int = 0, max_len: Optional[int] = None) -> torch.Tensor:
+        """Keep at most ``budget`` keys per user and head: the ``recent`` last ones and the heaviest others by ``weight_sums``
+        (without a call of :meth:`observe`, the first ones).  The kept rows move into new arrays of ``max_len`` rows (the cache's
+        present capacity when ``None``; a smaller one gives memory back), their sums with them.  Returns the kept keys' old
+        positions, int32 (n_users, n_kv_heads, budget), -1 behind a user's keys.  Calls captured on the old arrays
+        (``GraphedAttention``, ``HostDecodeStep``) have to be made anew."""
+        capacity = self.max_len if max_len is None else int(max_len)
+        sums = self.weight_sums
+        if sums is None:
+            sums = torch.zeros(self.n_users, self.n_kv_heads, self.max_len, dtype=torch.float32, device=self.device)
+        kept: EvictedCache = evict_keys(sums, self.k_nib, self.k_qjl, self.k_norms, self.v_nib, budget, recent=recent, seq_lens=self.lens32,
+                                        v_qjl=self.v_qjl, v_norms=self.v_norms, v_paired=self.pair_v, capacity=capacity)
+        self.k_nib, self.k_qjl, self.k_norms, self.v_nib = kept.k_nibbles, kept.k_qjl, kept.k_norms, kept.v_nibbles
+        self.v_qjl, self.v_norms, self.max_len = kept.v_qjl, kept.v_norms, capacity
+        if self.weight_sums is not None:
+            self.weight_sums = kept.sums
+        self.lens32.copy_(kept.seq_lens)
+        self.lens.copy_(kept.seq_lens)
+        return kept.index
 
     def attend(self, q: torch.Tensor, scale: Optional[float] = None, with_qjl: bool = True,
                rotate_q: bool = False, unrotate_out: bool = False, n_splits: Optional[int] = None) -> torch.Tensor:

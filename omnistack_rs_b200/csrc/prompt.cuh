@@ -47,7 +47,7 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& a, int64_t s
         const int64_t i = lo + lane * step;
         bool below = lane == 0;
         if (lane > 0 && i < lo + n) {
-            int64_t c = __ldg(a.cu + i);
+            int64_t c = a.cu[i];
             c = c < 0 ? 0 : (c > a.T ? a.T : c);
             below = c / a.tpt + i <= slot;
         }
@@ -56,7 +56,7 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& a, int64_t s
         n = lo + n - next < step ? lo + n - next : step;
         lo = next;
     }
-    int64_t c0 = __ldg(a.cu + lo), c1 = __ldg(a.cu + lo + 1);
+    int64_t c0 = a.cu[lo], c1 = a.cu[lo + 1];
     c0 = c0 < 0 ? 0 : (c0 > a.T ? a.T : c0);
     c1 = c1 < c0 ? c0 : (c1 > a.T ? a.T : c1);
     r.b = 0;

@@ -4,8 +4,12 @@
 // prompt in blocks of 128:   S_t = Q_t K^T  ->  P_t = exp2(c S_t - m)  ->  O_t += P_t V     (t = 0, 1;  c = scale * log2 e)
 // Q, K and V tiles come by TMA (128-byte swizzle); S, P and O live in tensor memory (512 columns: S0 S1 O0 O1, each P in the
 // columns of its S, which the softmax threads have read by then).  Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1,
-// thread = row; warp 8 issues every product; warp 9 every copy.  While the softmax of one tile runs, the products of the
-// other do.
+// thread = row; warp 8 issues every product; warp 9 every copy; warp 10 finds the work; warp 11 clears rows of no prompt.  While the
+// softmax of one tile runs, the products of the other do.
+//
+// A pair of tiles of one head group is a work item, one per launched CTA.  A CTA that runs takes over items of CTAs that are not yet
+// placed (cluster launch control), so the items are handed out as SMs become free, and the copies and first products of the next item
+// run under the last softmax and the output of this one.
 //
 // A block's maximum only replaces the running one when it exceeds it by 2^slack, so O is rescaled rarely; the softmax threads
 // do it themselves: S_t of a block is issued behind P_t V of the block before, so its arrival says that O_t is complete.
@@ -23,18 +27,22 @@
 
 namespace omni {
 
-constexpr int kPuThreads = 384;                    // warps 10 and 11 only complete the third warpgroup
-// Registers: 384 threads are launched with 168 each (64,512); the softmax warpgroups go up to 232, the third down to 40
-// (256 * 232 + 128 * 40 = 64,512).
-constexpr int kPuSoftmaxRegs = 232, kPuOtherRegs = 40;
+constexpr int kPuThreads = 384;
+// Registers: 384 threads are launched with 168 each (64,512); the softmax warpgroups go up to 224, the third down to 56
+// (256 * 224 + 128 * 56 = 64,512).
+constexpr int kPuSoftmaxRegs = 224, kPuOtherRegs = 56;
 constexpr int kPuStages = 5;                       // ring of K and V tiles, 32 KiB each, in the order K0 V0 K1 V1 ...
 constexpr uint32_t kPuTile = 128 * 128 * 2;        // bytes of a 128-row tile: two halves of 64 dims, 128 bytes a row
 constexpr uint32_t kPuHalf = kPuTile / 2;
 constexpr uint32_t kPuOffK = 2 * kPuTile;
 constexpr uint32_t kPuOffBar = kPuOffK + kPuStages * kPuTile;
-constexpr uint32_t kPuSmem = kPuOffBar + 256 + 1024;       // barriers, and room to start on a 1,024-byte boundary
+constexpr int kPuItems = 2;                        // ring of work items
+constexpr int kPuCu = 256;                         // prompt bounds kept in shared memory (more are read from global memory)
+constexpr uint32_t kPuOffCu = kPuOffBar + 256;
+constexpr uint32_t kPuOffItem = kPuOffCu + kPuCu * 4;           // item: batch, first row, length, first token, kv head, first query head, valid
+constexpr uint32_t kPuSmem = kPuOffItem + kPuItems * 32 + 16 + 1024;   // items, a stolen CTA's handle, and room to start on a 1,024-byte boundary
 constexpr uint32_t kPuColS = 0, kPuColO = 256, kPuTmemCols = 512;
-constexpr uint32_t kPuWaitLimit = 1u << 20;
+constexpr uint32_t kPuWaitLimit = 1u << 18;        // waits may last as long as a CTA's item does (rows formed again take milliseconds)
 constexpr float kPuLog2e = 1.4426950408889634f;
 
 // ---- PTX wrappers --------------------------------------------------------------------------------
@@ -181,6 +189,20 @@ __device__ __forceinline__ void prompt_row_again(const PromptArgs& a, int64_t b,
     Elem<DT>::store4(a.out, ((b * a.Hq + head) * a.T + row0 + t) * kHeadDim + 4 * lane, o);
 }
 
+// A work item: two tiles (32-bit: a prompt's rows and a call's slots are).
+struct PuItem {
+    int b, row0, len, t0, hkv, head0, slot;
+    int n[2];                                      // key blocks of each tile (0: no rows)
+    __device__ __forceinline__ void blocks(const PromptArgs& a, int tt) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int first = t0 + x * tt, last = first + tt - 1 < len ? first + tt - 1 : len - 1;
+            n[x] = first >= len ? 0 : ((a.causal ? last + 1 : len) + 127) / 128;
+        }
+    }
+    __device__ __forceinline__ int all() const { return n[0] > n[1] ? n[0] : n[1]; }
+};
+
 template <int DT>
 __global__ void __launch_bounds__(kPuThreads, 1)
 prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -189,26 +211,14 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
     // fp16 weights carry 2^bias: the type ends at 2^-24, and weights far below the row's largest would lose their bits there
     constexpr float kBias = DT == OMNI_F16 ? 8.f : 0.f, kSlack = DT == OMNI_F16 ? 7.f : 8.f;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t slot = (int64_t)gridDim.x - 1 - blockIdx.x;            // a prompt's last tiles have the most keys: first
-    const PromptTile w = prompt_tile(a, slot, lane);
-    const int hg = blockIdx.y % a.n_hg, hkv = blockIdx.y / a.n_hg;
-    const int head0 = hkv * (a.Hq / a.Hkv) + hg * a.gp;
-    prompt_zero_rows<DT>(a, w, slot, head0, tid, kPuThreads);
-    if (w.t0 >= w.len) return;
-
     const int tt = a.tpt / 2;                                            // tokens of one tile
-    int n_blocks[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int first = w.t0 + x * tt, last = first + tt - 1 < w.len ? first + tt - 1 : w.len - 1;
-        n_blocks[x] = first >= w.len ? 0 : ((a.causal ? last + 1 : w.len) + 127) / 128;
-    }
-    const int n_all = n_blocks[0] > n_blocks[1] ? n_blocks[0] : n_blocks[1];
 
     const uint32_t base = ((uint32_t)__cvta_generic_to_shared(pu_smem) + 1023u) & ~1023u;
     const uint32_t sQ = base, sKV = base + kPuOffK, bars = base + kPuOffBar;
     const uint32_t bar_q = bars, bar_full = bars + 16, bar_empty = bar_full + 8 * kPuStages, bar_s = bar_empty + 8 * kPuStages, bar_p = bar_s + 16,
-                   bar_h = bar_p + 16, bar_o = bar_h + 16, tmem_at = bar_o + 16;
+                   bar_h = bar_p + 16, bar_o = bar_h + 16, bar_qe = bar_o + 16, bar_item = bar_qe + 16, bar_taken = bar_item + 8 * kPuItems,
+                   bar_steal = bar_taken + 8 * kPuItems, bar_want = bar_steal + 8, tmem_at = bar_want + 8;
+    const uint32_t items = base + kPuOffItem, handle = items + kPuItems * 32;
     if (tid == 0) {
         for (int x = 0; x < 2; ++x) {
             pu_bar_init(bar_q + 8 * x, 1);
@@ -216,7 +226,14 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             pu_bar_init(bar_p + 8 * x, 4);
             pu_bar_init(bar_h + 8 * x, 4);
             pu_bar_init(bar_o + 8 * x, 1);
+            pu_bar_init(bar_qe + 8 * x, 1);
         }
+        for (int i = 0; i < kPuItems; ++i) {
+            pu_bar_init(bar_item + 8 * i, 1);
+            pu_bar_init(bar_taken + 8 * i, 11);                          // every warp but the one that finds the work
+        }
+        pu_bar_init(bar_steal, 1);
+        pu_bar_init(bar_want, 1);
         for (int i = 0; i < kPuStages; ++i) {
             pu_bar_init(bar_full + 8 * i, 1);
             pu_bar_init(bar_empty + 8 * i, 1);
@@ -234,34 +251,116 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
     asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(tmem) : "r"(tmem_at));
     bool ok = true;                                                      // false once a bounded wait has run out
 
+    // the k-th item of this CTA, by a warp; false when there is none (or a wait ran out)
+    PuItem it;
+    auto next_item = [&](int k) {
+        const int at = k % kPuItems;
+        ok = pu_bar_wait_warp(bar_item + 8 * at, (k / kPuItems) & 1);
+        if (!ok) return false;
+        uint32_t v[7];
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(items + 32 * at) : "memory");
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%3+16];\n ld.shared.u32 %2, [%3+24];\n" : "=r"(v[4]), "=r"(v[5]), "=r"(v[6]) : "r"(items + 32 * at) : "memory");
+        __syncwarp();
+        if (lane == 0) pu_bar_arrive(bar_taken + 8 * at);
+        it.b = (int)v[0]; it.row0 = (int)v[1]; it.len = (int)v[2]; it.t0 = (int)v[3]; it.hkv = (int)v[4]; it.head0 = (int)v[5]; it.slot = (int)v[6];
+        it.blocks(a, tt);
+        return it.slot >= 0;
+    };
+
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" :: "n"(kPuOtherRegs));
-        if (warp == 9) {
-            // ---- copies -----------------------------------------------------------------------------------------------
-            if (lane == 0) {
-                const uint32_t q_bytes = (uint32_t)(tt * a.gp) * 256u;
-                for (int x = 0; x < 2; ++x) {
-                    if (n_blocks[x] == 0) continue;
-                    pu_bar_expect(bar_q + 8 * x, q_bytes);
-                    for (int h = 0; h < 2; ++h)
-                        pu_tma_load(sQ + x * kPuTile + h * kPuHalf, &map_q, 64 * h, (int)w.row0 + w.t0 + x * tt, head0, (int)w.b, bar_q + 8 * x);
-                }
-                int i = 0;
-                for (; i < 2 * n_all; ++i) {                                 // tile i: K of block i / 2, or V when odd
-                    const int st = i % kPuStages, round = i / kPuStages;
-                    if (round > 0 && !pu_bar_wait(bar_empty + 8 * st, (round - 1) & 1)) { ok = false; break; }
-                    const uint32_t dst = sKV + st * kPuTile, bar = bar_full + 8 * st;
-                    pu_bar_expect(bar, kPuTile);
-                    const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
-                    for (int h = 0; h < 2; ++h) pu_tma_load(dst + h * kPuHalf, map, 64 * h, (int)w.row0 + 128 * (i >> 1), hkv, (int)w.b, bar);
-                }
-                // no copy may still be under way when the CTA ends (they all are complete unless a wait ran out)
-                if (!ok)
-                    for (int k = i < kPuStages ? 0 : i - kPuStages; k < i; ++k) pu_bar_wait(bar_full + 8 * (k % kPuStages), (k / kPuStages) & 1);
+        if (warp == 10) {
+            // ---- work: this CTA's own item, then those of CTAs that have not been placed ---------------------------------
+            uint32_t bx = blockIdx.x, by = blockIdx.y, valid = 1;
+            PromptArgs near = a;                                         // the same, with the bounds at hand
+            if (a.cu && a.n_seqs < kPuCu) {
+                int32_t* cu = reinterpret_cast<int32_t*>(pu_smem + (base - (uint32_t)__cvta_generic_to_shared(pu_smem)) + kPuOffCu);
+                for (int i = lane; i <= a.n_seqs; i += 32) cu[i] = __ldg(a.cu + i);
+                __syncwarp();
+                near.cu = cu;
             }
-        } else if (warp == 8) {
+            for (int k = 0;; ++k) {
+                const int at = k % kPuItems;
+                if (k >= kPuItems) ok = pu_bar_wait_warp(bar_taken + 8 * at, (k / kPuItems - 1) & 1);
+                if (!ok) break;
+                const int64_t slot = (int64_t)gridDim.x - 1 - bx;        // a prompt's last tiles have the most keys: first
+                PromptTile w{};
+                if (valid) w = prompt_tile(near, slot, lane);
+                if (lane == 0) {
+                    const uint32_t hkv = by / a.n_hg, head0 = hkv * (uint32_t)(a.Hq / a.Hkv) + by % a.n_hg * a.gp;
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" :: "r"(items + 32 * at), "r"((uint32_t)w.b), "r"((uint32_t)w.row0), "r"(w.len), "r"(w.t0) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0+16], {%1,%2};\n st.shared.u32 [%0+24], %3;\n" :: "r"(items + 32 * at), "r"(hkv), "r"(head0),
+                                 "r"(valid ? (uint32_t)slot : 0xffffffffu) : "memory");
+                    pu_bar_arrive(bar_item + 8 * at);
+                }
+                __syncwarp();
+                if (!valid) break;
+                // the next item is taken when the copies of this one have been issued, no sooner: what a busy CTA holds, an idle one cannot get
+                ok = pu_bar_wait_warp(bar_want, k & 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    pu_bar_expect(bar_steal, 16);
+                    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" :: "r"(handle), "r"(bar_steal) : "memory");
+                }
+                ok = pu_bar_wait_warp(bar_steal, k & 1);
+                if (!ok) break;
+                asm volatile("{\n .reg .pred p;\n .reg .b128 h;\n ld.shared.b128 h, [%3];\n clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+                             " selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n"
+                             " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n @p clusterlaunchcontrol.query_cancel.get_first_ctaid::y.b32.b128 %2, h;\n}\n"
+                             : "=r"(valid), "=r"(bx), "=r"(by) : "r"(handle) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");       // the handle has been read before the next one is written
+                __syncwarp();
+            }
+        } else if (warp == 11) {
+            for (int k = 0; next_item(k); ++k) {
+                PromptTile w;
+                w.b = it.b; w.row0 = it.row0; w.len = it.len; w.t0 = it.t0;
+                prompt_zero_rows<DT>(a, w, it.slot, it.head0, lane, 32);
+            }
+        } else if (warp == 9) {
+            // ---- copies -----------------------------------------------------------------------------------------------
+            const uint32_t q_bytes = (uint32_t)(tt * a.gp) * 256u;
+            int i = 0;                                                   // tiles of the ring so far
+            int used[2] = {0, 0};                                        // items so far whose first, second tile had rows
+            for (int k = 0; next_item(k); ++k) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (!ok || it.n[x] == 0) continue;
+                    // the products of the previous item have read the tile's queries
+                    if (used[x] > 0) ok = pu_bar_wait_warp(bar_qe + 8 * x, (used[x] - 1) & 1);
+                    if (!ok) continue;
+                    ++used[x];
+                    if (lane == 0) {
+                        pu_bar_expect(bar_q + 8 * x, q_bytes);
+                        for (int h = 0; h < 2; ++h)
+                            pu_tma_load(sQ + x * kPuTile + h * kPuHalf, &map_q, 64 * h, it.row0 + it.t0 + x * tt, it.head0, it.b, bar_q + 8 * x);
+                    }
+                }
+                const int n_tiles = 2 * it.all();                        // K and V in turn
+                for (int n = 0; ok && n < n_tiles; ++n, ++i) {
+                    const int st = i % kPuStages, round = i / kPuStages;
+                    if (round > 0) ok = pu_bar_wait_warp(bar_empty + 8 * st, (round - 1) & 1);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        const uint32_t dst = sKV + st * kPuTile, bar = bar_full + 8 * st;
+                        pu_bar_expect(bar, kPuTile);
+                        const CUtensorMap* map = (n & 1) ? &map_v : &map_k;
+                        for (int h = 0; h < 2; ++h) pu_tma_load(dst + h * kPuHalf, map, 64 * h, it.row0 + 128 * (n >> 1), it.hkv, it.b, bar);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (lane == 0) pu_bar_arrive(bar_want);
+            }
+            // no copy may still be under way when the CTA ends (they all are complete unless a wait ran out)
+            if (!ok) {
+                for (int k = i < kPuStages ? 0 : i - kPuStages; k < i; ++k) pu_bar_wait(bar_full + 8 * (k % kPuStages), (k / kPuStages) & 1);
+                for (int x = 0; x < 2; ++x)
+                    if (used[x] > 0) pu_bar_wait(bar_q + 8 * x, (used[x] - 1) & 1);
+            }
+        } else {
             // ---- products: the whole warp waits, one thread issues ----------------------------------------------------------
-            auto issue_s = [&](int x, uint32_t sK) {
+            auto issue_s = [&](int x, uint32_t sK, bool last) {
                 if (pu_elect()) {
                     const uint32_t da = pu_desc(sQ + x * kPuTile, 16), db = pu_desc(sK, 16);
 #pragma unroll
@@ -270,51 +369,70 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                         pu_mma_ss(tmem + kPuColS + 128 * x, da + off, db + off, pu_idesc<DT>(false), ks > 0);
                     }
                     pu_commit(bar_s + 8 * x);
+                    if (last) pu_commit(bar_qe + 8 * x);
                 }
                 __syncwarp();
             };
-            ok = pu_bar_wait_warp(bar_full, 0);
-            for (int x = 0; ok && x < 2; ++x) {
-                if (n_blocks[x] == 0) continue;
-                ok = pu_bar_wait_warp(bar_q + 8 * x, 0);
-                if (ok) { pu_fence_after(); issue_s(x, sKV); }
-            }
-            if (ok && pu_elect()) pu_commit(bar_empty);
-            int st = 0;                                                      // ring stage of K_j, and the parity of its round
+            int st = 0;                                                  // ring stage of the next tile, and the parity of its round
             uint32_t ph = 0;
-            for (int j = 0; ok && j < n_all; ++j) {
-                if (++st == kPuStages) { st = 0; ph ^= 1u; }                 // V_j
-                const int stv = st;
+            uint32_t done[2] = {0u, 0u}, used[2] = {0u, 0u};             // per tile: blocks and items so far (their parities are the barriers')
+            for (int k = 0; next_item(k); ++k) {
+                const int n_all = it.all();
+                if (n_all == 0) continue;
+                int stk = st;                                            // stage of K_j
                 ok = pu_bar_wait_warp(bar_full + 8 * st, ph);
-                if (++st == kPuStages) { st = 0; ph ^= 1u; }                 // K_{j+1}
-                if (ok && j + 1 < n_all) ok = pu_bar_wait_warp(bar_full + 8 * st, ph);
-                const uint32_t sV = sKV + stv * kPuTile, sK = sKV + st * kPuTile;
-#pragma unroll 1
-                for (int x = 0; ok && x < 2; ++x) {
-                    if (j >= n_blocks[x]) continue;
-                    // the weights come in halves: the product over keys 0-63 runs while the softmax works on the rest
+                if (++st == kPuStages) { st = 0; ph ^= 1u; }
 #pragma unroll
-                    for (int half = 0; half < 2 && ok; ++half) {
-                        ok = pu_bar_wait_warp((half ? bar_p : bar_h) + 8 * x, j & 1);
-                        if (!ok) break;
-                        pu_fence_after();
-                        if (pu_elect()) {
-                            const uint32_t db = pu_desc(sV, kPuHalf), dd = tmem + kPuColO + 128 * x, da = tmem + kPuColS + 128 * x;
-#pragma unroll
-                            for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
-                                pu_mma_ts(dd, da + 8 * ks, db + ks * (2048 >> 4), pu_idesc<DT>(true), (j > 0 || ks > 0) ? 1u : 0u);
-                            if (half == 1 && j + 1 >= n_blocks[x]) pu_commit(bar_o + 8 * x);
-                        }
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                    if (j + 1 < n_blocks[x]) issue_s(x, sK);
+                for (int x = 0; x < 2; ++x) {
+                    if (!ok || it.n[x] == 0) continue;
+                    ok = pu_bar_wait_warp(bar_q + 8 * x, used[x] & 1);
+                    if (!ok) continue;
+                    ++used[x];
+                    pu_fence_after();
+                    issue_s(x, sKV + stk * kPuTile, it.n[x] == 1);
                 }
-                if (ok && pu_elect()) {
-                    pu_commit(bar_empty + 8 * stv);
-                    if (j + 1 < n_all) pu_commit(bar_empty + 8 * st);
-                }
+                if (ok && pu_elect()) pu_commit(bar_empty + 8 * stk);
                 __syncwarp();
+                for (int j = 0; ok && j < n_all; ++j) {
+                    const int stv = st;                                  // V_j
+                    ok = pu_bar_wait_warp(bar_full + 8 * st, ph);
+                    if (++st == kPuStages) { st = 0; ph ^= 1u; }
+                    const bool more = j + 1 < n_all;
+                    if (more) {                                          // K_{j+1}
+                        stk = st;
+                        if (ok) ok = pu_bar_wait_warp(bar_full + 8 * st, ph);
+                        if (++st == kPuStages) { st = 0; ph ^= 1u; }
+                    }
+                    const uint32_t sV = sKV + stv * kPuTile, sK = sKV + stk * kPuTile;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (!ok || j >= it.n[x]) continue;
+                        // the weights come in halves: the product over keys 0-63 runs while the softmax works on the rest
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (ok) ok = pu_bar_wait_warp((half ? bar_p : bar_h) + 8 * x, done[x] & 1);
+                            if (!ok) break;
+                            pu_fence_after();
+                            if (pu_elect()) {
+                                const uint32_t db = pu_desc(sV, kPuHalf), dd = tmem + kPuColO + 128 * x, da = tmem + kPuColS + 128 * x;
+#pragma unroll
+                                for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
+                                    pu_mma_ts(dd, da + 8 * ks, db + ks * (2048 >> 4), pu_idesc<DT>(true), (j > 0 || ks > 0) ? 1u : 0u);
+                                if (half == 1 && j + 1 >= it.n[x]) pu_commit(bar_o + 8 * x);
+                            }
+                            __syncwarp();
+                        }
+                        if (!ok) continue;
+                        ++done[x];
+                        if (j + 1 < it.n[x]) issue_s(x, sK, j + 2 >= it.n[x]);
+                    }
+                    if (ok && pu_elect()) {
+                        pu_commit(bar_empty + 8 * stv);
+                        if (more) pu_commit(bar_empty + 8 * stk);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
             }
         }
     } else {
@@ -323,105 +441,110 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
         const int x = warp >> 2, row = tid & 127;
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t t_s = t_lane + kPuColS + 128 * x, t_o = t_lane + kPuColO + 128 * x;
-        const int g = row / tt, t = w.t0 + x * tt + row % tt;
-        const bool live = g < a.gp && t < w.len;
-        // newest key of the row; rows without a query go through the motions on whatever their operands hold
-        const int lim = live ? (a.causal ? t : w.len - 1) : w.len - 1;
-        const int n_free = a.causal ? w.t0 + x * tt + 1 : w.len;         // keys below this are open to every row of the tile
+        const int g = row / tt, t_in = row % tt;
         const float c = a.scale * kPuLog2e;
-        float m = -INFINITY, l = 0.f;                                    // m: in units of c * score
-        for (int j = 0; j < n_blocks[x]; ++j) {
-            ok = pu_bar_wait_warp(bar_s + 8 * x, j & 1);
+        uint32_t done = 0, used = 0;                                     // blocks and items of this tile so far
+        for (int k = 0; next_item(k); ++k) {
+            const int n_mine = x ? it.n[1] : it.n[0];
+            if (n_mine == 0) continue;
+            const int t = it.t0 + x * tt + t_in;
+            const bool live = g < a.gp && t < it.len;
+            // newest key of the row; rows without a query go through the motions on whatever their operands hold
+            const int lim = live ? (a.causal ? t : it.len - 1) : it.len - 1;
+            const int n_free = a.causal ? it.t0 + x * tt + 1 : it.len;       // keys below this are open to every row of the tile
+            float m = -INFINITY, l = 0.f;                                    // m: in units of c * score
+            for (int j = 0; j < n_mine; ++j) {
+                ok = pu_bar_wait_warp(bar_s + 8 * x, done & 1);
+                if (!ok) break;
+                pu_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pu_ld32(t_s + 32 * i, s + 32 * i);
+                pu_wait_ld();
+                if (128 * j + 128 > n_free) {
+                    const int open = lim - 128 * j;                          // columns 0 .. open of the block are seen
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) s[i] = i <= open ? s[i] : 0xff800000u;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 128; i += 8) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = pu_max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                const bool raise = top > m + kSlack;
+                if (__any_sync(kFullMask, raise)) {
+                    const float m_new = raise ? top : m;
+                    const float alpha = raise ? pu_ex2(m - m_new) : 1.f;
+                    m = m_new;
+                    l *= alpha;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t o[32];
+                            pu_ld32(t_o + 32 * i, o);
+                            pu_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                            pu_st32(t_o + 32 * i, o);
+                        }
+                    }
+                }
+                const uint64_t c2 = pu_pair(c, c), neg2 = pu_pair(kBias - m, kBias - m);
+                uint64_t sum[2] = {pu_pair(0.f, 0.f), pu_pair(0.f, 0.f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 v = pu_parts(pu_fma2(pu_pair(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1])), c2, neg2));
+                        const float2 e = make_float2(pu_ex2(v.x), pu_ex2(v.y));
+                        sum[i & 1] = pu_add2(sum[i & 1], pu_pair(e.x, e.y));
+                        p[i] = pu_pack<DT>(e.x, e.y);
+                    }
+                    pu_st32(t_s + 32 * h, p);
+                    pu_wait_st();
+                    pu_fence_before();
+                    __syncwarp();
+                    if (lane == 0) pu_bar_arrive((h ? bar_p : bar_h) + 8 * x);
+                }
+                const float2 both = pu_parts(pu_add2(sum[0], sum[1]));
+                l += both.x + both.y;
+                ++done;
+            }
+            // ---- result rows ---------------------------------------------------------------------------------------------
+            if (ok) ok = pu_bar_wait_warp(bar_o + 8 * x, used & 1);
+            ++used;
             if (!ok) break;
             pu_fence_after();
-            uint32_t s[128];
+            const float inv = 1.f / l;
+            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) +
+                                                  (((int64_t)it.b * a.Hq + it.head0 + (live ? g : 0)) * a.T + it.row0 + (live ? t : it.t0)) * kHeadDim);
+            bool bad = false;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pu_ld32(t_s + 32 * i, s + 32 * i);
-            pu_wait_ld();
-            if (128 * j + 128 > n_free) {
-                const int open = lim - 128 * j;                          // columns 0 .. open of the block are seen
+            for (int i = 0; i < 4; ++i) {
+                uint32_t o[32];
+                pu_ld32(t_o + 32 * i, o);
+                pu_wait_ld();
+                uint32_t r[16];
 #pragma unroll
-                for (int i = 0; i < 128; ++i) s[i] = i <= open ? s[i] : 0xff800000u;
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int k = 0; k < 16; ++k) {
+                    const float u = __uint_as_float(o[2 * k]) * inv, v = __uint_as_float(o[2 * k + 1]) * inv;
+                    bad = bad || u != u || v != v;
+                    r[k] = pu_pack<DT>(u, v);
+                }
+                if (live) {
 #pragma unroll
-            for (int i = 0; i < 128; i += 8) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mx[k] = pu_max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
-            }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-            const bool raise = top > m + kSlack;
-            if (__any_sync(kFullMask, raise)) {
-                const float m_new = raise ? top : m;
-                const float alpha = raise ? pu_ex2(m - m_new) : 1.f;
-                m = m_new;
-                l *= alpha;
-                if (j > 0) {
-#pragma unroll 1
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t o[32];
-                        pu_ld32(t_o + 32 * i, o);
-                        pu_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                        pu_st32(t_o + 32 * i, o);
-                    }
+                    for (int k = 0; k < 4; ++k) dst[4 * i + k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
                 }
             }
-            const uint64_t c2 = pu_pair(c, c), neg2 = pu_pair(kBias - m, kBias - m);
-            uint64_t sum[2] = {pu_pair(0.f, 0.f), pu_pair(0.f, 0.f)};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t p[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float2 v = pu_parts(pu_fma2(pu_pair(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1])), c2, neg2));
-                    const float2 e = make_float2(pu_ex2(v.x), pu_ex2(v.y));
-                    sum[i & 1] = pu_add2(sum[i & 1], pu_pair(e.x, e.y));
-                    p[i] = pu_pack<DT>(e.x, e.y);
-                }
-                pu_st32(t_s + 32 * h, p);
-                pu_wait_st();
-                pu_fence_before();
-                __syncwarp();
-                if (lane == 0) pu_bar_arrive((h ? bar_p : bar_h) + 8 * x);
-            }
-            const float2 both = pu_parts(pu_add2(sum[0], sum[1]));
-            l += both.x + both.y;
-        }
-        // ---- result rows ---------------------------------------------------------------------------------------------
-        if (n_blocks[x] > 0) {
-            if (ok) ok = pu_bar_wait_warp(bar_o + 8 * x, 0);
-            if (ok) {
-                pu_fence_after();
-                const float inv = 1.f / l;
-                uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) +
-                                                      ((w.b * a.Hq + head0 + (live ? g : 0)) * a.T + w.row0 + (live ? t : w.t0)) * kHeadDim);
-                bool bad = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t o[32];
-                    pu_ld32(t_o + 32 * i, o);
-                    pu_wait_ld();
-                    uint32_t r[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float u = __uint_as_float(o[2 * k]) * inv, v = __uint_as_float(o[2 * k + 1]) * inv;
-                        bad = bad || u != u || v != v;
-                        r[k] = pu_pack<DT>(u, v);
-                    }
-                    if (live) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) dst[4 * i + k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
-                    }
-                }
-                uint32_t again = __ballot_sync(kFullMask, live && bad);
-                while (again) {
-                    const int src = __ffs(again) - 1;
-                    again &= again - 1;
-                    prompt_row_again<DT>(a, w.b, w.row0, __shfl_sync(kFullMask, t, src), __shfl_sync(kFullMask, lim, src),
-                                         head0 + __shfl_sync(kFullMask, g, src), lane);
-                }
+            uint32_t again = __ballot_sync(kFullMask, live && bad);
+            while (again) {
+                const int src = __ffs(again) - 1;
+                again &= again - 1;
+                prompt_row_again<DT>(a, it.b, it.row0, __shfl_sync(kFullMask, t, src), __shfl_sync(kFullMask, lim, src),
+                                     it.head0 + __shfl_sync(kFullMask, g, src), lane);
             }
         }
     }

@@ -382,7 +382,7 @@ int32_t omni_qk_norm_rope(const omni_norm_rope_t* call, void* stream);
  *   cu_seqlens   device int32 [n_seqs + 1], ascending: prompt i is rows cu[i] .. cu[i+1]-1 of the one user (B == 1) whose T
  *                rows hold all prompts; rows of no prompt get zeros.  NULL: every user is one prompt (n_seqs == B)
  *   seq_lens     device int32 [B] or NULL (T): without cu_seqlens, rows of a user at and behind its length get zeros
- *   out          contiguous [B][Hq][T][128] of `dtype`
+ *   out          contiguous [B][Hq][T][128] of `dtype`, on a 32-byte boundary
  * Values of masked keys never reach a row, whatever they hold (infinities and NaN included).  Scores, softmax statistics and
  * sums are fp32; for bf16 and fp16 the weights are rounded to that type for the second product.
  *   status_word  device int32 or NULL, as in omni_qattn_decode */

@@ -199,12 +199,13 @@ extern "C" int32_t omni_prompt_attn(const void* q, const void* k, const void* v,
     OMNI_REQUIRE(B >= 0 && T >= 0 && Hq > 0 && Hkv > 0 && n_seqs >= 0, OMNI_ERR_ARG, "omni_prompt_attn: bad extent");
     OMNI_REQUIRE(Hq % Hkv == 0, OMNI_ERR_ARG, "omni_prompt_attn: Hq=%d is not a multiple of Hkv=%d", Hq, Hkv);
     OMNI_REQUIRE(dtype >= 0 && dtype <= 2, OMNI_ERR_ARG, "omni_prompt_attn: unknown dtype code %d", dtype);
-    OMNI_REQUIRE(T <= 0x3fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: more than 2^30 rows per user");
+    OMNI_REQUIRE(T <= 0x3fffffffLL && n_seqs <= 0x3fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: more than 2^30 rows or prompts");
     OMNI_REQUIRE(cu_seqlens ? B == 1 && !seq_lens : n_seqs == B, OMNI_ERR_ARG, "omni_prompt_attn: packed prompts are the rows of one user; otherwise every user is one prompt");
     if (B == 0 || T == 0) return OMNI_OK;
     OMNI_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides, OMNI_ERR_ARG, "omni_prompt_attn: NULL buffer");
     const int64_t unit = dtype == OMNI_F32 ? 4 : 8;
     OMNI_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");
+    OMNI_REQUIRE(((uintptr_t)out & 31) == 0, OMNI_ERR_ARG, "omni_prompt_attn: out must start on a 32-byte boundary");
     PromptArgs a{};
     for (int i = 0; i < 3; ++i) {
         OMNI_REQUIRE(q_strides[i] % unit == 0 && k_strides[i] % unit == 0 && v_strides[i] % unit == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");

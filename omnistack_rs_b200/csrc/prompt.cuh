@@ -29,41 +29,42 @@ struct PromptTile {
 // The prompt and tile behind a slot.  Padded: slots are (b, tile).  Packed: prompt i owns the slots from cu[i] / tpt + i up to
 // those of prompt i + 1, which are at least ceil(len / tpt) of them; a warp finds the prompt with 32 probes a step.
 // All 32 lanes of a warp call this together.
-__device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& a, int64_t slot, int lane) {
+__device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& a, int64_t slot64, int lane) {
     PromptTile r;
+    const uint32_t slot = (uint32_t)slot64, tpt = (uint32_t)a.tpt;       // rows, slots and prompts of a call are below 2^31
     if (!a.cu) {
-        const int64_t per = a.slots / a.n_seqs;
+        const uint32_t per = (uint32_t)a.slots / (uint32_t)a.n_seqs;
         r.b = slot / per;
         r.row0 = 0;
-        int64_t len = a.seq_lens ? (int64_t)__ldg(a.seq_lens + r.b) : a.T;
+        const int64_t len = a.seq_lens ? (int64_t)__ldg(a.seq_lens + r.b) : a.T;
         r.len = (int)(len < 0 ? 0 : (len > a.T ? a.T : len));
-        r.t0 = (int)(slot % per) * a.tpt;
+        r.t0 = (int)(slot % per * tpt);
         return r;
     }
     // the last prompt whose first slot is at or below `slot` (first slots ascend strictly; that of prompt 0 counts as 0)
-    int64_t lo = 0, n = a.n_seqs;                  // the answer lies in [lo, lo + n)
+    const int T = (int)a.T;
+    uint32_t lo = 0, n = (uint32_t)a.n_seqs;       // the answer lies in [lo, lo + n)
     while (n > 1) {
-        const int64_t step = (n + 31) / 32;
-        const int64_t i = lo + lane * step;
+        const uint32_t step = (n + 31) / 32;
+        const uint32_t i = lo + lane * step;
         bool below = lane == 0;
         if (lane > 0 && i < lo + n) {
-            int64_t c = a.cu[i];
-            c = c < 0 ? 0 : (c > a.T ? a.T : c);
-            below = c / a.tpt + i <= slot;
+            int c = a.cu[i];
+            c = c < 0 ? 0 : (c > T ? T : c);
+            below = (uint32_t)c / tpt + i <= slot;
         }
-        const int hit = 31 - __clz((int)__ballot_sync(kFullMask, below));
-        const int64_t next = lo + hit * step;
+        const uint32_t next = lo + (31 - __clz((int)__ballot_sync(kFullMask, below))) * step;
         n = lo + n - next < step ? lo + n - next : step;
         lo = next;
     }
-    int64_t c0 = a.cu[lo], c1 = a.cu[lo + 1];
-    c0 = c0 < 0 ? 0 : (c0 > a.T ? a.T : c0);
-    c1 = c1 < c0 ? c0 : (c1 > a.T ? a.T : c1);
+    int c0 = a.cu[lo], c1 = a.cu[lo + 1];
+    c0 = c0 < 0 ? 0 : (c0 > T ? T : c0);
+    c1 = c1 < c0 ? c0 : (c1 > T ? T : c1);
     r.b = 0;
     r.row0 = c0;
-    r.len = (int)(c1 - c0);
-    const int64_t first = c0 / a.tpt + lo;
-    const int64_t t0 = (slot - first) * a.tpt;
+    r.len = c1 - c0;
+    const uint32_t first = (uint32_t)c0 / tpt + lo;
+    const int64_t t0 = ((int64_t)slot - first) * tpt;
     r.t0 = slot < first || t0 > r.len ? r.len : (int)t0;
     return r;
 }

@@ -125,6 +125,10 @@ __device__ __forceinline__ float pu_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ void pu_store32(void* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" :: "l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7]) : "memory");
+}
 // two fp32 operations in one instruction, on register pairs
 __device__ __forceinline__ uint64_t pu_pair(float x, float y) {
     uint64_t r;
@@ -534,9 +538,9 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                     bad = bad || u != u || v != v;
                     r[k] = pu_pack<DT>(u, v);
                 }
-                if (live) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) dst[4 * i + k] = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+                if (live) {                                              // a thread's row, whole 32-byte sectors at a time
+                    pu_store32(dst + 4 * i, r);
+                    pu_store32(dst + 4 * i + 2, r + 8);
                 }
             }
             uint32_t again = __ballot_sync(kFullMask, live && bad);

@@ -90,7 +90,7 @@ def test_evict_refusals(change, error, match):
 
 def test_c_entries_refuse_bad_arguments(lib):
     """Checks that need no device: they come before the first CUDA call of each entry."""
-    one = C.c_void_p(16)
+    one = C.c_void_p(32)
     assert lib.omni_qk_norm_rope(None, None) == _lib.ERR_ARG
     def norm_rope(q=16, heads=1, axes=1, pairs=0, end=0, stride=128, dtype=1):
         return lib.omni_qk_norm_rope(position._NORM_ROPE.pack(q, 0, 16, 0, 0, 0, 16, 16, 0, 0, stride, 0, 0, 0, 0, 0, 0, 1, 1, heads, 0, 0, 0, end, 0, 0, 0,

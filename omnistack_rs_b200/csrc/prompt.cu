@@ -2,18 +2,34 @@
 //
 //   s_ij = scale q_i . k_j (j of the same prompt, j <= i when causal),  o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
 //
-// One pass over the keys with the running maximum m and sum of each row.  64 x 64 tiles of scores on the FP32 units: 256
-// threads, 4 x 4 scores and 4 x 8 outputs each; K and V share one buffer so that two CTAs fit an SM.
+// One pass over the keys with the running maximum m and sum of each row.  64 x 64 tiles of scores on the FP32 units (two products per
+// instruction): 256 threads, 4 x 4 scores and 4 x 8 outputs each; K and V share one buffer so that two CTAs fit an SM.  4 prompts of up
+// to 611 tokens and 8 heads take 152 us (189 with one product per instruction), 1,500 tokens run at 33 TFLOP/s: bound by the loads
+// between the phases of a tile, which only the other CTA covers.  Tiles of 32 rows (three CTAs per SM) win below 100 tokens (18 us
+// against 23) and lose above (180 us).
 #include "prompt.cuh"
 
 namespace omni {
 
 constexpr int kPfM = 64, kPfN = 64;                // rows (token, head) and keys of a tile
+constexpr int kPfR = kPfM / 16;                    // rows per thread
 constexpr int kPfThreads = 256;
 constexpr int kPfStride = kHeadDim + 4;            // floats: a warp's sixteen key rows start in different banks
 constexpr int kPfPStride = kPfN + 4;
-constexpr int kPfSmem = (2 * kPfM * kPfStride + kPfM * kPfPStride) * 4;
+constexpr int kPfSmem = ((kPfM + kPfN) * kPfStride + kPfM * kPfPStride) * 4;
 constexpr float kPfLog2e = 1.4426950408889634f;
+
+// two fp32 operations in one instruction: (a.x b.x + c.x, a.y b.y + c.y)
+__device__ __forceinline__ float2 pf_fma2(float2 a, float2 b, float2 c) {
+    uint64_t x, y, z, r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(x) : "f"(a.x), "f"(a.y));
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(y) : "f"(b.x), "f"(b.y));
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(z) : "f"(c.x), "f"(c.y));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
 
 // rows [r0, r0 + 64) of a strided head into shared memory as fp32, zeros from row `end` on
 template <int DT>
@@ -29,9 +45,10 @@ __device__ __forceinline__ void pf_load_tile(float* dst, const void* src, int64_
 
 template <int DT>
 __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid_constant__ PromptArgs a) {
-    extern __shared__ __align__(16) float pf_smem[];
-    float* Qs = pf_smem;
-    float* Ks = Qs + kPfM * kPfStride;                                   // keys, then the values of the same tile
+    constexpr int M = kPfM, R = kPfR;
+    extern __shared__ __align__(16) float pf_shared[];
+    float* Qs = pf_shared;
+    float* Ks = Qs + M * kPfStride;                                   // keys, then the values of the same tile
     float* Ps = Ks + kPfN * kPfStride;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int64_t slot = (int64_t)gridDim.x - 1 - blockIdx.x;            // a prompt's last tiles have the most keys: first
@@ -45,17 +62,17 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
 
     // ---- queries, scaled for exponents of two --------------------------------------------------------------------------
     const float qs = a.scale * kPfLog2e;
-    for (int at = tid; at < kPfM * 32; at += kPfThreads) {
+    for (int at = tid; at < M * 32; at += kPfThreads) {
         const int row = at >> 5, c = (at & 31) * 4;
         const int t = w.t0 + row % a.tpt, g = row / a.tpt;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (g < a.gp && t < w.len) Elem<DT>::load4(a.q, w.b * a.qs[0] + (int64_t)(head0 + g) * a.qs[1] + (w.row0 + t) * a.qs[2] + c, v);
         *reinterpret_cast<float4*>(Qs + row * kPfStride + c) = make_float4(v[0] * qs, v[1] * qs, v[2] * qs, v[3] * qs);
     }
-    int lim[4];                                                          // newest key of this thread's rows (-1: no row)
+    int lim[R];                                                          // newest key of this thread's rows (-1: no row)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = 4 * ty + i, t = w.t0 + row % a.tpt;
+    for (int i = 0; i < R; ++i) {
+        const int row = R * ty + i, t = w.t0 + row % a.tpt;
         lim[i] = row / a.tpt < a.gp && t < w.len ? (a.causal ? t : w.len - 1) : -1;
     }
     const int t_last = w.t0 + a.tpt - 1 < w.len ? w.t0 + a.tpt - 1 : w.len - 1;
@@ -63,9 +80,9 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
     const int n_free = a.causal ? w.t0 + 1 : w.len;                      // keys below this are open to every row of the tile
     const int64_t kbase = w.b * a.ks[0] + (int64_t)hkv * a.ks[1] + w.row0 * a.ks[2];
     const int64_t vbase = w.b * a.vs[0] + (int64_t)hkv * a.vs[1] + w.row0 * a.vs[2];
-    float m[4], l[4], o[4][8];
+    float m[R], l[R], o[R][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
         m[i] = -INFINITY; l[i] = 0.f;
 #pragma unroll
         for (int c = 0; c < 8; ++c) o[i][c] = 0.f;
@@ -76,32 +93,35 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
         __syncthreads();                                                 // the previous tile's values are no longer read
         pf_load_tile<DT>(Ks, a.k, kbase, a.ks[2], j0, n_keys);
         __syncthreads();
-        float s[4][4];
+        float2 s2[R][4];                                                 // even and odd dims apart
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+            for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 4
         for (int d = 0; d < kHeadDim; d += 4) {
-            float4 qv[4], kv[4];
+            float4 qv[R], kv[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(Qs + (4 * ty + i) * kPfStride + d);
+            for (int i = 0; i < R; ++i) qv[i] = *reinterpret_cast<const float4*>(Qs + (R * ty + i) * kPfStride + d);
 #pragma unroll
             for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * kPfStride + d);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    s[i][j] = fmaf(qv[i].x, kv[j].x, s[i][j]);
-                    s[i][j] = fmaf(qv[i].y, kv[j].y, s[i][j]);
-                    s[i][j] = fmaf(qv[i].z, kv[j].z, s[i][j]);
-                    s[i][j] = fmaf(qv[i].w, kv[j].w, s[i][j]);
+                    s2[i][j] = pf_fma2(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
+                    s2[i][j] = pf_fma2(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
                 }
         }
+        float s[R][4];
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
         __syncthreads();                                                 // the keys have been read
         pf_load_tile<DT>(Ks, a.v, vbase, a.vs[2], j0, n_keys);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < R; ++i) {
             if (masked) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -119,7 +139,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
             for (int j = 0; j < 4; ++j) {
                 const float p = exp2f(s[i][j] - ref);
                 sum += p;
-                Ps[(4 * ty + i) * kPfPStride + tx + 16 * j] = p;
+                Ps[(R * ty + i) * kPfPStride + tx + 16 * j] = p;
             }
 #pragma unroll
             for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(kFullMask, sum, x);
@@ -128,23 +148,26 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
             for (int c = 0; c < 8; ++c) o[i][c] *= alpha;
         }
         __syncthreads();
-        if (!masked) {
+        if (!masked || !a.causal) {                                      // without the causal mask, masked keys lie behind the end: zeros
 #pragma unroll 2
             for (int j = 0; j < kPfN; j += 4) {
-                float4 pv[4];
+                float4 pv[R];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(Ps + (4 * ty + i) * kPfPStride + j);
+                for (int i = 0; i < R; ++i) pv[i] = *reinterpret_cast<const float4*>(Ps + (R * ty + i) * kPfPStride + j);
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj) {
                     const float4 va = *reinterpret_cast<const float4*>(Ks + (j + jj) * kPfStride + 4 * tx);
                     const float4 vb = *reinterpret_cast<const float4*>(Ks + (j + jj) * kPfStride + 64 + 4 * tx);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < R; ++i) {
                         const float p = jj == 0 ? pv[i].x : jj == 1 ? pv[i].y : jj == 2 ? pv[i].z : pv[i].w;
-                        o[i][0] = fmaf(p, va.x, o[i][0]); o[i][1] = fmaf(p, va.y, o[i][1]);
-                        o[i][2] = fmaf(p, va.z, o[i][2]); o[i][3] = fmaf(p, va.w, o[i][3]);
-                        o[i][4] = fmaf(p, vb.x, o[i][4]); o[i][5] = fmaf(p, vb.y, o[i][5]);
-                        o[i][6] = fmaf(p, vb.z, o[i][6]); o[i][7] = fmaf(p, vb.w, o[i][7]);
+                        const float2 p2 = make_float2(p, p), v2[4] = {{va.x, va.y}, {va.z, va.w}, {vb.x, vb.y}, {vb.z, vb.w}};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float2 r = pf_fma2(p2, v2[c], make_float2(o[i][2 * c], o[i][2 * c + 1]));
+                            o[i][2 * c] = r.x;
+                            o[i][2 * c + 1] = r.y;
+                        }
                     }
                 }
             }
@@ -153,9 +176,9 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
                 const float4 va = *reinterpret_cast<const float4*>(Ks + j * kPfStride + 4 * tx);
                 const float4 vb = *reinterpret_cast<const float4*>(Ks + j * kPfStride + 64 + 4 * tx);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < R; ++i) {
                     if (j0 + j > lim[i]) continue;
-                    const float p = Ps[(4 * ty + i) * kPfPStride + j];
+                    const float p = Ps[(R * ty + i) * kPfPStride + j];
                     o[i][0] = fmaf(p, va.x, o[i][0]); o[i][1] = fmaf(p, va.y, o[i][1]);
                     o[i][2] = fmaf(p, va.z, o[i][2]); o[i][3] = fmaf(p, va.w, o[i][3]);
                     o[i][4] = fmaf(p, vb.x, o[i][4]); o[i][5] = fmaf(p, vb.y, o[i][5]);
@@ -165,8 +188,8 @@ __global__ void __launch_bounds__(kPfThreads, 2) prompt_fp32_kernel(const __grid
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = 4 * ty + i, t = w.t0 + row % a.tpt;
+    for (int i = 0; i < R; ++i) {
+        const int row = R * ty + i, t = w.t0 + row % a.tpt;
         if (lim[i] < 0) continue;
         const float inv = 1.f / l[i];
         const int64_t at = ((w.b * a.Hq + head0 + row / a.tpt) * a.T + w.row0 + t) * kHeadDim;

@@ -361,10 +361,10 @@ __global__ void __launch_bounds__(kWmWarps * 32, 2) weight_step_kernel(const __g
     }
 }
 
-// weights of the kept scores: sums[s] (+)= sum_c 2^(score_c - lse_c)
+// weights of the kept scores: sums[s] (+)= sum_c 2^(score_c - max_c) / sum_c
 constexpr int kWfThreads = 256, kWfKeys = 2;       // keys per thread
 __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_constant__ WeightArgs a, int pad, int64_t segments, int64_t ctas) {
-    __shared__ float lse[kWsStepCols];
+    __shared__ float2 norm[kWsStepCols];                                 // the columns' maxima and reciprocal sums
     const int tid = threadIdx.x;
     const int64_t bh = blockIdx.x / segments, s0 = blockIdx.x % segments * (kWfKeys * kWfThreads);
     const int64_t b = bh / a.Hkv, h = bh % a.Hkv;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_
             for (int i = lane; i < n; i += 32) l += p[(int64_t)i * cols].y * exp2f(p[(int64_t)i * cols].x - ref);
 #pragma unroll
             for (int x = 16; x >= 1; x >>= 1) l += __shfl_xor_sync(kFullMask, l, x);
-            if (lane == 0) lse[warp] = m == -INFINITY && l == 0.f ? 0.f : ref + log2f(l);   // no open key: its scores are -inf
+            if (lane == 0) norm[warp] = make_float2(ref, m == -INFINITY && l == 0.f ? 0.f : 1.f / l);   // no open key: its scores are -inf
         }
         __syncthreads();
     } else if (a.accumulate) {
@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_
         if (s < len) {
 #pragma unroll
             for (int i = 0; i < kWsStepCols / 2; ++i) {
-                if (2 * i < cols) total += ws_ex2(v[k][i].x - lse[2 * i]);
-                if (2 * i + 1 < cols) total += ws_ex2(v[k][i].y - lse[2 * i + 1]);
+                if (2 * i < cols) total = fmaf(ws_ex2(v[k][i].x - norm[2 * i].x), norm[2 * i].y, total);
+                if (2 * i + 1 < cols) total = fmaf(ws_ex2(v[k][i].y - norm[2 * i + 1].x), norm[2 * i + 1].y, total);
             }
         }
         float* d = a.sums + bh * a.S + s;

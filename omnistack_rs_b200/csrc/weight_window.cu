@@ -8,7 +8,7 @@
 // The tiles of all (user, head) lie in one row, cut into equal shares, one per CTA: lengths differ, and only the device knows
 // them.  A run of tiles of one head inside a share is a span; span (head, CTA) is number head + CTA, which no other span has.
 // Pass 1: thread = column, running maximum and sum over a span's keys, one pair per (span, column) into the workspace.
-// Pass 2: the same scores again (cheaper than 4 bytes per key and column written and read), weights 2^(s - lse), and their sum over
+// Pass 2: the same scores again (cheaper than 4 bytes per key and column written and read), weights 2^(s - max) / sum, and their sum over
 // the columns: a halving exchange between the lanes of a warp, then the four warps' parts in order.
 //
 // Warps 0-7: scores, two threads per column with 64 of a tile's keys each.  Warps 8-15: dequantisation, two threads per key, up to
@@ -292,19 +292,20 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                 ww_fence_after();
                 if (ww_elect()) {
                     const uint32_t kx = kv + x * 8 * kWwSbo, sx = kv + 2 * kWwBytesV + x * 8 * kWwSboSign, da = tmem + kWwColA + 64 * x, db = tmem + kWwColB + 64 * x;
+                    // the remainders' products first: added to an accumulator that already holds the values', each would cost it a rounding
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, ks > 0);
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + kWwBytesV + ks * 2 * kWwLbo, kWwSbo, 64, 1);
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + kWwBytesV + ks * 2 * kWwLbo, kWwSbo, 64, ks > 0);
                     if (QLO) {
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQlo + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, 1);
                     }
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, 1);
                     if (a.with_qjl) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColChi + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, ks > 0);
+                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColClo + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, ks > 0);
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColClo + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, 1);
+                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColChi + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, 1);
                     }
                     if (x == 1) ww_commit(bar_empty + 8 * (t & 1));
                     ww_commit(bar_s + 8 * x);
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             }
             const int last = col_on ? (a.causal ? len - a.T + col % a.T : len - 1) : -1;    // newest key of the column
             const int open_to = a.causal ? len - a.T : len - 1;          // newest key that every column sees
-            float m = -INFINITY, l = 0.f, lse = 0.f;
+            float m = -INFINITY, l = 0.f, top_all = 0.f, inv = 0.f;          // pass 2: the column's maximum and reciprocal sum
             if (PASS == 2 && col_on) {
                 // the head's spans: the CTAs whose shares hold its first and its last tile, and those between
                 const int64_t first = ((int64_t)a.tiles_before[at.b]) * a.Hkv + (int64_t)at.h * at.n_tiles;
@@ -432,7 +433,8 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                 for (int64_t i = 0; i <= c1 - c0; ++i) m = fmaxf(m, p[i * cols].x);
                 const float ref = m == -INFINITY ? 0.f : m;
                 for (int64_t i = 0; i <= c1 - c0; ++i) l += p[i * cols].y * exp2f(p[i * cols].x - ref);
-                lse = m == -INFINITY && l == 0.f ? 0.f : ref + log2f(l); // no open key: its scores are -inf
+                top_all = ref;
+                inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;         // no open key: its scores are -inf
             }
             for (int t = done; t < done + n_span; ++t) {
                 // after a wait that ran out the warp still goes through the barriers it shares with the others, storing nothing
@@ -498,12 +500,12 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                     m = m_new;
                 } else {
                     float p[64];
-                    const uint64_t f2 = ww_pack2(f, f), r2 = ww_pack2(-lse, -lse);
+                    const uint64_t f2 = ww_pack2(f, f), r2 = ww_pack2(-top_all, -top_all);
 #pragma unroll
                     for (int i = 0; i < 64; i += 2) {
                         const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, r2));
-                        p[i] = ws_ex2(e.x);
-                        p[i + 1] = ws_ex2(e.y);
+                        p[i] = ws_ex2(e.x) * inv;
+                        p[i + 1] = ws_ex2(e.y) * inv;
                     }
                     // sum over the warp's 32 columns: lanes trade halves of their keys until each has the totals of two
 #pragma unroll

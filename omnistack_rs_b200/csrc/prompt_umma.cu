@@ -42,7 +42,7 @@ constexpr uint32_t kPuOffCu = kPuOffBar + 256;
 constexpr uint32_t kPuOffItem = kPuOffCu + kPuCu * 4;           // item: batch, first row, length, first token, kv head, first query head, valid
 constexpr uint32_t kPuSmem = kPuOffItem + kPuItems * 32 + 16 + 1024;   // items, a stolen CTA's handle, and room to start on a 1,024-byte boundary
 constexpr uint32_t kPuColS = 0, kPuColO = 256, kPuTmemCols = 512;
-constexpr uint32_t kPuWaitLimit = 1u << 18;        // waits may last as long as a CTA's item does (rows formed again take milliseconds)
+constexpr uint32_t kPuWaitLimit = 1u << 26;        // waits may last as long as a CTA's item does (rows formed again take milliseconds)
 constexpr float kPuLog2e = 1.4426950408889634f;
 
 // ---- PTX wrappers --------------------------------------------------------------------------------

@@ -40,7 +40,7 @@ constexpr uint32_t kWwBuf = 2 * kWwBytesV + kWwBytesSign;           // values, r
 constexpr uint32_t kWwOffLut = 2 * kWwBuf, kWwOffNorm = kWwOffLut + kWwLutBytes, kWwOffRed = kWwOffNorm + 4 * kWwTile * 4,
                    kWwOffBar = kWwOffRed + 4 * kWwTile * 4, kWwSmem = kWwOffBar + 128;
 constexpr uint32_t kWwColA = 0, kWwColB = 128, kWwColQhi = 256, kWwColQlo = 320, kWwColChi = 384, kWwColClo = 416, kWwTmemCols = 512;
-constexpr uint32_t kWwWaitLimit = 1u << 20;
+constexpr uint32_t kWwWaitLimit = 1u << 22;
 
 __device__ __forceinline__ void ww_bar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" :: "r"(bar), "r"(count) : "memory");

@@ -386,11 +386,15 @@ int32_t omni_qk_norm_rope(const omni_norm_rope_t* call, void* stream);
  * Values of masked keys never reach a row, whatever they hold (infinities and NaN included).  Scores, softmax statistics and
  * sums are fp32; for bf16 and fp16 the weights are rounded to that type for the second product.
  *   status_word  device int32 or NULL, as in omni_qattn_decode */
-int32_t omni_prompt_attn(const void* q, const void* k, const void* v, int32_t dtype,
-                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                         const int32_t* cu_seqlens, int64_t n_seqs, const int32_t* seq_lens,
-                         int64_t B, int32_t Hq, int32_t Hkv, int64_t T, float scale, int32_t causal,
-                         void* out, int32_t* status_word, void* stream);
+typedef struct omni_prompt_t {
+    const void* q; const void* k; const void* v; void* out;
+    const int32_t* cu_seqlens; const int32_t* seq_lens; int32_t* status_word;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    int64_t n_seqs, B, T;
+    int32_t dtype, Hq, Hkv, causal;
+    float   scale;
+} omni_prompt_t;
+int32_t omni_prompt_attn(const omni_prompt_t* call, void* stream);
 
 /* ---- eviction: keeping the cache small -----------------------------------------------------------------------
  * The softmax weight that every cached key receives from T queries of its kv head's group (what omni_qattn_decode weighs
@@ -403,12 +407,14 @@ int32_t omni_prompt_attn(const void* q, const void* k, const void* v, int32_t dt
  * gives the same bits.  `workspace`: omni_attn_weight_sums_workspace_bytes(...) bytes of device scratch.
  *   status_word  device int32 or NULL, as in omni_qattn_decode */
 size_t  omni_attn_weight_sums_workspace_bytes(int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S);
-int32_t omni_attn_weight_sums(const void* q, int32_t q_dtype, const uint8_t* k_nib, const uint8_t* k_qjl,
-                              const float* k_norms, const float* codebooks, int32_t cb_per_head,
-                              const int32_t* user_ids, int32_t user_id, const int32_t* seq_lens,
-                              int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S, float scale, int32_t with_qjl,
-                              int32_t rotate_q, int32_t causal, int32_t accumulate, void* workspace,
-                              size_t workspace_bytes, float* sums, int32_t* status_word, void* stream);
+typedef struct omni_weight_sums_t {
+    const void* q; const uint8_t* k_nib; const uint8_t* k_qjl; const float* k_norms; const float* codebooks;
+    const int32_t* user_ids; const int32_t* seq_lens; void* workspace; float* sums; int32_t* status_word;
+    int64_t B, S; uint64_t workspace_bytes;
+    int32_t q_dtype, cb_per_head, user_id, Hq, Hkv, T, with_qjl, rotate_q, causal, accumulate;
+    float   scale;
+} omni_weight_sums_t;
+int32_t omni_attn_weight_sums(const omni_weight_sums_t* call, void* stream);
 
 /* Eviction by accumulated weight: of every (user, head) with more than `budget` keys the `recent` last ones and the
  * budget - recent others with the largest sums stay (equal sums: the lower position; NaN counts as the largest), in their

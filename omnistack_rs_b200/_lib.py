@@ -61,10 +61,9 @@ SIGNATURES = {
     "omni_qattn_noalloc_status": (_i32, [_vp, _i32]),
     "omni_diag_bounded_wait": (_i32, [_i32, _vp, _vp]),
     "omni_qk_norm_rope": (_i32, [_vp, _vp]),
-    "omni_prompt_attn": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i64, _f32, _i32, _vp, _vp, _vp]),
+    "omni_prompt_attn": (_i32, [_vp, _vp]),
     "omni_attn_weight_sums_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64]),
-    "omni_attn_weight_sums": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i64, _f32, _i32, _i32,
-                                     _i32, _i32, _vp, _sz, _vp, _vp, _vp]),
+    "omni_attn_weight_sums": (_i32, [_vp, _vp]),
     "omni_evict_keys": (_i32, [_vp, _vp]),
 }
 

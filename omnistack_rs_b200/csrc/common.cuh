@@ -6,6 +6,7 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <stdarg.h>
+#include <atomic>
 #include <vector>
 #include "../../include/omni_b200.h"
 
@@ -51,6 +52,23 @@ int32_t check_cuda(cudaError_t e, const char* what);
 #define OMNI_REQUIRE(cond, code, ...)                           \
     do {                                                        \
         if (!(cond)) return ::omni::set_error((code), __VA_ARGS__); \
+    } while (0)
+
+// The dynamic shared memory a kernel may be launched with, set once per device (`done`: one bit each).
+static inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint32_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint32_t bit = 1u << (dev & 31);
+    if (dev < 32 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 32) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+#define OMNI_ALLOW_SMEM(kernel, bytes)                                                          \
+    do {                                                                                        \
+        static std::atomic<uint32_t> _done{0};                                                  \
+        OMNI_CUDA(::omni::allow_smem(reinterpret_cast<const void*>(kernel), (int)(bytes), _done)); \
     } while (0)
 
 // Launch behind a kernel of the same call that lets its successors start early (follow_me_early): the successor's CTAs are placed while the

@@ -265,7 +265,7 @@ extern "C" int32_t omni_evict_keys(const omni_evict_t* call, void* stream) {
     const int64_t groups_per_head = (a.capacity + 7) / 8, n_groups = a.B * a.H * groups_per_head;
     OMNI_REQUIRE((n_groups + kGatherWarps - 1) / kGatherWarps <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_evict_keys: too many rows");
     cudaStream_t st = (cudaStream_t)stream;
-    OMNI_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeyBytes));
+    OMNI_ALLOW_SMEM((evict_select_kernel), kSelKeyBytes);
     evict_select_kernel<<<(unsigned)(a.B * a.H), kSelThreads, kSelKeyBytes, st>>>(a);
     OMNI_CUDA(cudaGetLastError());
     return check_cuda(launch_early(evict_gather_kernel, dim3((unsigned)((n_groups + kGatherWarps - 1) / kGatherWarps)), kGatherWarps * 32, 0, st, a, groups_per_head, n_groups),

@@ -205,7 +205,7 @@ static int32_t launch_prompt_fp32(PromptArgs a, cudaStream_t st) {
     a.tpt = kPfM / a.gp;
     a.slots = a.cu ? a.T / a.tpt + a.n_seqs : a.B * ((a.T + a.tpt - 1) / a.tpt);
     OMNI_REQUIRE(a.slots <= 0x7fffffffLL && (int64_t)a.Hkv * a.n_hg <= 65535, OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: too many tiles");
-    OMNI_CUDA(cudaFuncSetAttribute(prompt_fp32_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmem));
+    OMNI_ALLOW_SMEM((prompt_fp32_kernel<DT>), kPfSmem);
     prompt_fp32_kernel<DT><<<dim3((unsigned)a.slots, (unsigned)(a.Hkv * a.n_hg)), kPfThreads, kPfSmem, st>>>(a);
     return check_cuda(cudaGetLastError(), "prompt_fp32_kernel launch");
 }
@@ -214,40 +214,40 @@ static int32_t launch_prompt_fp32(PromptArgs a, cudaStream_t st) {
 
 using namespace omni;
 
-extern "C" int32_t omni_prompt_attn(const void* q, const void* k, const void* v, int32_t dtype,
-                                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                                    const int32_t* cu_seqlens, int64_t n_seqs, const int32_t* seq_lens,
-                                    int64_t B, int32_t Hq, int32_t Hkv, int64_t T, float scale, int32_t causal,
-                                    void* out, int32_t* status_word, void* stream) {
+extern "C" int32_t omni_prompt_attn(const omni_prompt_t* call, void* stream) {
+    OMNI_REQUIRE(call != nullptr, OMNI_ERR_ARG, "omni_prompt_attn: NULL call");
+    const omni_prompt_t& p = *call;
+    const int64_t B = p.B, T = p.T, n_seqs = p.n_seqs;
+    const int32_t Hq = p.Hq, Hkv = p.Hkv, dtype = p.dtype;
     OMNI_REQUIRE(B >= 0 && T >= 0 && Hq > 0 && Hkv > 0 && n_seqs >= 0, OMNI_ERR_ARG, "omni_prompt_attn: bad extent");
     OMNI_REQUIRE(Hq % Hkv == 0, OMNI_ERR_ARG, "omni_prompt_attn: Hq=%d is not a multiple of Hkv=%d", Hq, Hkv);
     OMNI_REQUIRE(dtype >= 0 && dtype <= 2, OMNI_ERR_ARG, "omni_prompt_attn: unknown dtype code %d", dtype);
     OMNI_REQUIRE(T <= 0x3fffffffLL && n_seqs <= 0x3fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_prompt_attn: more than 2^30 rows or prompts");
-    OMNI_REQUIRE(cu_seqlens ? B == 1 && !seq_lens : n_seqs == B, OMNI_ERR_ARG, "omni_prompt_attn: packed prompts are the rows of one user; otherwise every user is one prompt");
+    OMNI_REQUIRE(p.cu_seqlens ? B == 1 && !p.seq_lens : n_seqs == B, OMNI_ERR_ARG, "omni_prompt_attn: packed prompts are the rows of one user; otherwise every user is one prompt");
     if (B == 0 || T == 0) return OMNI_OK;
-    OMNI_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides, OMNI_ERR_ARG, "omni_prompt_attn: NULL buffer");
+    OMNI_REQUIRE(p.q && p.k && p.v && p.out, OMNI_ERR_ARG, "omni_prompt_attn: NULL buffer");
     const int64_t unit = dtype == OMNI_F32 ? 4 : 8;
-    OMNI_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");
-    OMNI_REQUIRE(((uintptr_t)out & 31) == 0, OMNI_ERR_ARG, "omni_prompt_attn: out must start on a 32-byte boundary");
+    OMNI_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15) == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");
+    OMNI_REQUIRE(((uintptr_t)p.out & 31) == 0, OMNI_ERR_ARG, "omni_prompt_attn: out must start on a 32-byte boundary");
     PromptArgs a{};
     for (int i = 0; i < 3; ++i) {
-        OMNI_REQUIRE(q_strides[i] % unit == 0 && k_strides[i] % unit == 0 && v_strides[i] % unit == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");
-        a.qs[i] = q_strides[i]; a.ks[i] = k_strides[i]; a.vs[i] = v_strides[i];
+        OMNI_REQUIRE(p.q_strides[i] % unit == 0 && p.k_strides[i] % unit == 0 && p.v_strides[i] % unit == 0, OMNI_ERR_ARG, "omni_prompt_attn: rows must start on 16-byte boundaries");
+        a.qs[i] = p.q_strides[i]; a.ks[i] = p.k_strides[i]; a.vs[i] = p.v_strides[i];
     }
     cudaStream_t st = (cudaStream_t)stream;
     if (n_seqs == 0) {
-        OMNI_CUDA(cudaMemsetAsync(out, 0, (size_t)(B * Hq * T) * kHeadDim * (dtype == OMNI_F32 ? 4 : 2), st));
+        OMNI_CUDA(cudaMemsetAsync(p.out, 0, (size_t)(B * Hq * T) * kHeadDim * (dtype == OMNI_F32 ? 4 : 2), st));
         return OMNI_OK;
     }
-    a.q = q; a.k = k; a.v = v; a.out = out; a.cu = cu_seqlens; a.seq_lens = seq_lens;
-    a.B = B; a.T = T; a.n_seqs = n_seqs; a.Hq = Hq; a.Hkv = Hkv; a.scale = scale; a.causal = causal; a.status = status_word;
+    a.q = p.q; a.k = p.k; a.v = p.v; a.out = p.out; a.cu = p.cu_seqlens; a.seq_lens = p.seq_lens;
+    a.B = B; a.T = T; a.n_seqs = n_seqs; a.Hq = Hq; a.Hkv = Hkv; a.scale = p.scale; a.causal = p.causal; a.status = p.status_word;
     // heads per tile: the largest divisor of the group up to sixteen
     const int G = Hq / Hkv;
     a.gp = 1;
     for (int g = 2; g <= 16; ++g) if (G % g == 0) a.gp = g;
     a.n_hg = G / a.gp;
     // The tensor-core kernel takes its running maximum over unscaled scores, which needs a positive scale.
-    if (dtype != OMNI_F32 && scale > 0.f) return launch_prompt_umma(a, dtype, st);
+    if (dtype != OMNI_F32 && p.scale > 0.f) return launch_prompt_umma(a, dtype, st);
     switch (dtype) {
         case OMNI_F32:  return launch_prompt_fp32<OMNI_F32>(a, st);
         case OMNI_BF16: return launch_prompt_fp32<OMNI_BF16>(a, st);

@@ -605,7 +605,7 @@ static int32_t launch_prompt_umma_t(const PromptArgs& a, cudaStream_t st) {
     if (rc == OMNI_OK) rc = pu_map(&mk, a.k, DT, a.ks, a.T, a.Hkv, a.B, 128, 1);
     if (rc == OMNI_OK) rc = pu_map(&mv, a.v, DT, a.vs, a.T, a.Hkv, a.B, 128, 1);
     if (rc != OMNI_OK) return rc;
-    OMNI_CUDA(cudaFuncSetAttribute(prompt_umma_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPuSmem));
+    OMNI_ALLOW_SMEM((prompt_umma_kernel<DT>), kPuSmem);
     prompt_umma_kernel<DT><<<dim3((unsigned)a.slots, (unsigned)(a.Hkv * a.n_hg)), kPuThreads, kPuSmem, st>>>(a, mq, mk, mv);
     return check_cuda(cudaGetLastError(), "prompt_umma_kernel launch");
 }

@@ -440,7 +440,7 @@ static int32_t launch_weight_step(WeightArgs a, cudaStream_t st) {
     a.scores = reinterpret_cast<float*>(ws + wm_partial_bytes(heads, a.S, cols));
     weight_fragments_kernel<DT, QLO><<<(unsigned)((heads + kWmPrepWarps - 1) / kWmPrepWarps + 1), kWmPrepWarps * 32, 0, st>>>(a);
     OMNI_CUDA(cudaGetLastError());
-    OMNI_CUDA(cudaFuncSetAttribute(weight_step_kernel<QLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWmLutBytes));
+    OMNI_ALLOW_SMEM((weight_step_kernel<QLO>), kWmLutBytes);
     OMNI_CUDA(launch_early(weight_step_kernel<QLO>, dim3((unsigned)ctas), kWmWarps * 32, kWmLutBytes, st, a, pad));
     return check_cuda(launch_early(weight_finish_kernel, dim3((unsigned)(heads * segments)), kWfThreads, 0, st, a, pad, segments, ctas), "weight_finish_kernel launch");
 }
@@ -457,36 +457,35 @@ extern "C" size_t omni_attn_weight_sums_workspace_bytes(int64_t B, int32_t Hq, i
            heads * S * ((cols + 1) & ~(size_t)1) * sizeof(float);
 }
 
-extern "C" int32_t omni_attn_weight_sums(const void* q, int32_t q_dtype, const uint8_t* k_nib, const uint8_t* k_qjl,
-                                         const float* k_norms, const float* codebooks, int32_t cb_per_head,
-                                         const int32_t* user_ids, int32_t user_id, const int32_t* seq_lens,
-                                         int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S, float scale, int32_t with_qjl,
-                                         int32_t rotate_q, int32_t causal, int32_t accumulate, void* workspace,
-                                         size_t workspace_bytes, float* sums, int32_t* status_word, void* stream) {
+extern "C" int32_t omni_attn_weight_sums(const omni_weight_sums_t* call, void* stream) {
+    OMNI_REQUIRE(call != nullptr, OMNI_ERR_ARG, "omni_attn_weight_sums: NULL call");
+    const omni_weight_sums_t& p = *call;
+    const int64_t B = p.B, S = p.S;
+    const int32_t Hq = p.Hq, Hkv = p.Hkv, T = p.T, q_dtype = p.q_dtype, with_qjl = p.with_qjl, rotate_q = p.rotate_q;
     OMNI_REQUIRE(B >= 0 && S >= 0 && T >= 0 && Hq > 0 && Hkv > 0, OMNI_ERR_ARG, "omni_attn_weight_sums: bad extent");
     OMNI_REQUIRE(Hq % Hkv == 0, OMNI_ERR_ARG, "omni_attn_weight_sums: Hq=%d is not a multiple of Hkv=%d", Hq, Hkv);
     OMNI_REQUIRE(Hkv <= kSeeds, OMNI_ERR_UNSUPPORTED, "omni_attn_weight_sums: Hkv=%d exceeds %d heads", Hkv, kSeeds);
     OMNI_REQUIRE(q_dtype >= 0 && q_dtype <= 2, OMNI_ERR_ARG, "omni_attn_weight_sums: unknown dtype code %d", q_dtype);
     if (B == 0 || S == 0) return OMNI_OK;
-    OMNI_REQUIRE(sums != nullptr, OMNI_ERR_ARG, "omni_attn_weight_sums: NULL buffer");
+    OMNI_REQUIRE(p.sums != nullptr, OMNI_ERR_ARG, "omni_attn_weight_sums: NULL buffer");
     cudaStream_t st = (cudaStream_t)stream;
     if (T == 0) {
-        if (!accumulate) OMNI_CUDA(cudaMemsetAsync(sums, 0, (size_t)(B * Hkv * S) * sizeof(float), st));
+        if (!p.accumulate) OMNI_CUDA(cudaMemsetAsync(p.sums, 0, (size_t)(B * Hkv * S) * sizeof(float), st));
         return OMNI_OK;
     }
-    OMNI_REQUIRE(q && k_nib && codebooks && (!with_qjl || (k_qjl && k_norms)), OMNI_ERR_ARG, "omni_attn_weight_sums: NULL buffer");
-    OMNI_REQUIRE((((uintptr_t)q | (uintptr_t)k_nib) & 15) == 0 && ((uintptr_t)k_qjl & 7) == 0, OMNI_ERR_ARG, "omni_attn_weight_sums: misaligned buffer");
-    OMNI_REQUIRE(workspace && workspace_bytes >= omni_attn_weight_sums_workspace_bytes(B, Hq, Hkv, T, S) && ((uintptr_t)workspace & 15) == 0,
+    OMNI_REQUIRE(p.q && p.k_nib && p.codebooks && (!with_qjl || (p.k_qjl && p.k_norms)), OMNI_ERR_ARG, "omni_attn_weight_sums: NULL buffer");
+    OMNI_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.k_nib) & 15) == 0 && ((uintptr_t)p.k_qjl & 7) == 0, OMNI_ERR_ARG, "omni_attn_weight_sums: misaligned buffer");
+    OMNI_REQUIRE(p.workspace && p.workspace_bytes >= omni_attn_weight_sums_workspace_bytes(B, Hq, Hkv, T, S) && ((uintptr_t)p.workspace & 15) == 0,
                  OMNI_ERR_ARG, "omni_attn_weight_sums: workspace too small or misaligned");
     const DeviceTables* tab = tables_for_current_device();
     if (!tab) return OMNI_ERR_NOT_INIT;
     WeightArgs a{};
-    a.q = q; a.k_nib = k_nib; a.k_qjl = k_qjl; a.k_norms = k_norms; a.codebooks = codebooks; a.cb_per_head = cb_per_head;
-    a.user_ids = user_ids; a.user_id = user_id; a.seq_lens = seq_lens; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.T = T; a.S = S;
-    a.scale = scale; a.with_qjl = with_qjl; a.rotate_q = rotate_q; a.causal = causal; a.accumulate = accumulate;
-    a.g_rows = tab->rows; a.partial = reinterpret_cast<float2*>(workspace); a.sums = sums;
+    a.q = p.q; a.k_nib = p.k_nib; a.k_qjl = p.k_qjl; a.k_norms = p.k_norms; a.codebooks = p.codebooks; a.cb_per_head = p.cb_per_head;
+    a.user_ids = p.user_ids; a.user_id = p.user_id; a.seq_lens = p.seq_lens; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.T = T; a.S = S;
+    a.scale = p.scale; a.with_qjl = with_qjl; a.rotate_q = rotate_q; a.causal = p.causal; a.accumulate = p.accumulate;
+    a.g_rows = tab->rows; a.partial = reinterpret_cast<float2*>(p.workspace); a.sums = p.sums;
     OMNI_REQUIRE(S <= 0x7fffff00LL && B * Hkv <= 0x7fffffffLL && (int64_t)(Hq / Hkv) * T <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_attn_weight_sums: too many keys");
-    if (Hq / Hkv * (int64_t)T > kWsStepCols) return launch_weight_window(a, q_dtype, status_word, st);
+    if (Hq / Hkv * (int64_t)T > kWsStepCols) return launch_weight_window(a, q_dtype, p.status_word, st);
     switch (q_dtype) {
         case OMNI_F32:  return launch_weight_step<OMNI_F32, true>(a, st);
         case OMNI_BF16: return rotate_q ? launch_weight_step<OMNI_BF16, true>(a, st) : launch_weight_step<OMNI_BF16, false>(a, st);

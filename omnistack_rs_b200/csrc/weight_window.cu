@@ -571,8 +571,8 @@ size_t weight_window_workspace(int64_t B, int Hq, int Hkv, int T, int64_t S) {
 template <bool QLO>
 static int32_t launch_weight_window_t(const WeightArgs& a, unsigned grid, int32_t* status, cudaStream_t st) {
     const int cols = a.Hq / a.Hkv * a.T;
-    OMNI_CUDA(cudaFuncSetAttribute(weight_window_kernel<QLO, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWwSmem));
-    OMNI_CUDA(cudaFuncSetAttribute(weight_window_kernel<QLO, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWwSmem));
+    OMNI_ALLOW_SMEM((weight_window_kernel<QLO, 1>), kWwSmem);
+    OMNI_ALLOW_SMEM((weight_window_kernel<QLO, 2>), kWwSmem);
     for (int pass = 1; pass <= 2; ++pass) {
         for (int col0 = 0; col0 < cols; col0 += kWwTile) {
             if (pass == 1) OMNI_CUDA(launch_early(weight_window_kernel<QLO, 1>, dim3(grid), kWwThreads, kWwSmem, st, a, col0, status));

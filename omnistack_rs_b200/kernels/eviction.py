@@ -17,7 +17,8 @@ from .hadamard import HEAD_DIM
 from .quantize import _NBYTES_NIBBLE, _NBYTES_QJL, _prep_codebooks, _user_args
 
 
-# ``omni_evict_t`` of the C header, field by field
+# ``omni_weight_sums_t`` and ``omni_evict_t`` of the C header, field by field
+_WEIGHT_SUMS = struct.Struct("@10P2qQ10if")
 _EVICT = struct.Struct("@8P7P2P5q2i")
 
 
@@ -90,12 +91,12 @@ def attn_weight_sums(q: torch.Tensor, k_nibbles: torch.Tensor, k_qjl: torch.Tens
     sums = torch.empty(B, Hkv, S, dtype=torch.float32, device=dev) if into is None else into
     nbytes = lib.omni_attn_weight_sums_workspace_bytes(B, Hq, Hkv, T, S)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    call = _WEIGHT_SUMS.pack(q.data_ptr(), k_nibbles.data_ptr(), k_qjl.data_ptr(), k_norms.data_ptr(), cb.data_ptr(),
+                             0 if ids is None else ids.data_ptr(), 0 if lens is None else lens.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                             sums.data_ptr(), _lib.status_word(dev).data_ptr(), B, S, nbytes, _lib.DTYPE_CODE[q.dtype], per_head, uid, Hq, Hkv, T,
+                             bool(with_qjl), bool(rotate_q), bool(causal), into is not None, 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
     with _lib.on_device(dev):
-        _lib.check(lib.omni_attn_weight_sums(
-            _lib.ptr(q), _lib.DTYPE_CODE[q.dtype], _lib.ptr(k_nibbles), _lib.ptr(k_qjl), _lib.ptr(k_norms), _lib.ptr(cb), per_head,
-            _lib.ptr(ids), uid, _lib.ptr(lens), B, Hq, Hkv, T, S, float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale),
-            int(bool(with_qjl)), int(bool(rotate_q)), int(bool(causal)), int(into is not None), _lib.ptr(scratch), nbytes,
-            _lib.ptr(sums), _lib.ptr(_lib.status_word(dev)), _lib.stream_ptr(dev)))
+        _lib.check(lib.omni_attn_weight_sums(call, _lib.stream_ptr(dev)))
     return sums
 
 

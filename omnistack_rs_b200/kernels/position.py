@@ -24,6 +24,9 @@ def _place(x: torch.Tensor):
     """(tensor, address, strides of users, heads and tokens) of rows a kernel can read: ``x`` itself when its 128-element rows are
     contiguous and start on 16-byte boundaries, else a contiguous copy.  Strides of extents of one do not count and are 0."""
     n0, n1, n2, _ = x.shape
+    at = x.data_ptr()
+    if not at & 15 and x.is_contiguous():
+        return x, at, n1 * n2 * HEAD_DIM, n2 * HEAD_DIM, HEAD_DIM
     s0, s1, s2, s3 = x.stride()
     if n0 < 2:
         s0 = 0
@@ -31,7 +34,6 @@ def _place(x: torch.Tensor):
         s1 = 0
     if n2 < 2:
         s2 = 0
-    at = x.data_ptr()
     if s3 != 1 or at & 15 or (s0 | s1 | s2) & (3 if x.dtype is torch.float32 else 7):
         x = x.clone(memory_format=torch.contiguous_format)
         return x, x.data_ptr(), n1 * n2 * HEAD_DIM, n2 * HEAD_DIM, HEAD_DIM
@@ -73,14 +75,19 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     ``inv_freq``: float32 or float64 (P,), one frequency per pair, P <= 64; pair i turns by position * inv_freq[i], formed in
     float64.  The pairs are dims (i, i + P), or (2i, 2i + 1) with ``interleaved``; dims from 2P on are not rotated.
     ``eps=None`` leaves the norm (and the weights) out."""
-    if q.dim() != 4 or (k is not None and k.dim() != 4):
+    q_shape = q.shape
+    if len(q_shape) != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be (B, n_heads, T, 128)")
-    B, Hq, T, D = q.shape
+    B, Hq, T, D = q_shape
     if D != HEAD_DIM:
         raise ValueError(f"norm and rotation require last dim = {HEAD_DIM} (head_dim), got {D}")
-    if k is not None and (k.shape[0] != B or k.shape[2] != T or k.shape[3] != HEAD_DIM):
+    Hkv, k_at, k_strides, k_out, k_out_at = 0, 0, (0, 0, 0), None, 0
+    if k is not None:
+        k0, Hkv, k2, k3 = k.shape
+    if k is not None and (k0 != B or k2 != T or k3 != HEAD_DIM):
         raise ValueError(f"k must be ({B}, n_kv_heads, {T}, {HEAD_DIM}) like q, got {tuple(k.shape)}")
-    if q.dtype not in _lib.DTYPE_CODE:
+    code = _lib.DTYPE_CODE.get(q.dtype)
+    if code is None:
         raise TypeError(f"unsupported dtype {q.dtype}; use float32, bfloat16 or float16")
     if k is not None and k.dtype is not q.dtype:
         raise TypeError(f"q and k have different dtypes: {q.dtype} and {k.dtype}")
@@ -92,13 +99,14 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
     if axis_pairs is None:
-        axis_pairs, lead = (P,), ()
+        n_axes, ends, lead = 1, (P, 0, 0, 0), ()
     else:
         axis_pairs = tuple(int(n) for n in axis_pairs)
-        lead = (len(axis_pairs),)
+        n_axes, lead = len(axis_pairs), (len(axis_pairs),)
+        ends = tuple(sum(axis_pairs[:i + 1]) for i in range(n_axes)) + (0,) * (MAX_AXES - n_axes)
         if not 1 <= len(axis_pairs) <= MAX_AXES or min(axis_pairs) < 0 or sum(axis_pairs) != P:
             raise ValueError(f"axis_pairs must be 1 to {MAX_AXES} pair counts that add up to {P} (the length of inv_freq), got {axis_pairs}")
-    if tuple(positions.shape) not in (lead + (B, T), lead + (T,)):
+    if positions.shape != lead + (B, T) and positions.shape != lead + (T,):
         raise ValueError(f"positions must have shape {lead + (B, T)} or {lead + (T,)}, got {tuple(positions.shape)}")
     if eps is None and (q_weight is not None or k_weight is not None):
         raise ValueError("eps=None leaves the norm out, so it takes no weights")
@@ -108,9 +116,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     lib = _lib.load()
     q, q_at, *q_strides = _place(q)
     q_out = torch.empty(B, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
-    Hkv, k_at, k_strides, k_out, k_out_at = 0, 0, (0, 0, 0), None, 0
     if k is not None:
-        Hkv = k.shape[1]
         k, k_at, *k_strides = _place(k)
         k_out = torch.empty(B, Hkv, T, HEAD_DIM, dtype=q.dtype, device=dev)
         k_out_at = k_out.data_ptr()
@@ -121,11 +127,10 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if inv_freq.device != dev or not inv_freq.is_contiguous():
         inv_freq = inv_freq.to(dev).contiguous()
     ps = positions.stride()
-    ends = [sum(axis_pairs[:i + 1]) for i in range(len(axis_pairs))] + [0] * (MAX_AXES - len(axis_pairs))
     call = _NORM_ROPE.pack(
         q_at, k_at, q_out.data_ptr(), k_out_at, qw_at, kw_at, positions.data_ptr(), inv_freq.data_ptr(), *q_strides, *k_strides,
         ps[0] if lead else 0, ps[-2] if positions.dim() == len(lead) + 2 else 0, ps[-1], B, T, Hq, Hkv, qw_code, kw_code, *ends,
-        _lib.DTYPE_CODE[q.dtype], len(axis_pairs), P, positions.dtype is torch.int64, inv_freq.dtype is torch.float64, bool(interleaved),
+        code, n_axes, P, positions.dtype is torch.int64, inv_freq.dtype is torch.float64, bool(interleaved),
         eps is not None, 0.0 if eps is None else eps)
     with _lib.on_device(dev):
         _lib.check(lib.omni_qk_norm_rope(call, _lib.stream_ptr(dev)))

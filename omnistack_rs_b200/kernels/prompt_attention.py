@@ -16,12 +16,13 @@ from .hadamard import HEAD_DIM
 from .position import _place
 
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
-_STRIDES = struct.Struct("@3q")
+# ``omni_prompt_t`` of the C header, field by field
+_PROMPT = struct.Struct("@7P9q3q4if")
 
 
 def _tiles(x: torch.Tensor):
     """Rows a kernel can copy in boxes: tensor maps have no stride of 0, so rows shared by one are copied."""
-    if 0 in x.stride()[:3]:
+    if not x.is_contiguous() and 0 in x.stride()[:3]:
         x = x.contiguous()
     return _place(x)
 
@@ -42,22 +43,26 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens
 
     Scores, softmax statistics and sums are float32.  For bfloat16 and float16 the tensor cores multiply the weights, rounded
     to that type, with the values; float32 stays float32 throughout."""
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 4 or len(k_shape) != 4 or v.dim() != 4:
         raise ValueError("q, k and v must be (B, n_heads, T, 128)")
-    B, Hq, T, D = q.shape
+    B, Hq, T, D = q_shape
     if D != HEAD_DIM:
         raise ValueError(f"attention requires last dim = {HEAD_DIM} (head_dim), got {D}")
-    Hkv = k.shape[1]
-    if k.shape != (B, Hkv, T, HEAD_DIM) or v.shape != k.shape:
-        raise ValueError(f"k and v must be ({B}, n_kv_heads, {T}, {HEAD_DIM}) like q, got {tuple(k.shape)} and {tuple(v.shape)}")
+    Hkv = k_shape[1]
+    if k_shape[0] != B or k_shape[2] != T or k_shape[3] != HEAD_DIM or v.shape != k_shape:
+        raise ValueError(f"k and v must be ({B}, n_kv_heads, {T}, {HEAD_DIM}) like q, got {tuple(k_shape)} and {tuple(v.shape)}")
     if Hkv == 0 or Hq % Hkv or Hq == 0:
         raise ValueError(f"n_heads={Hq} is not a multiple of n_kv_heads={Hkv}")
-    if q.dtype not in _lib.DTYPE_CODE:
-        raise TypeError(f"unsupported dtype {q.dtype}; use float32, bfloat16 or float16")
-    if k.dtype is not q.dtype or v.dtype is not q.dtype:
-        raise TypeError(f"q, k and v have different dtypes: {q.dtype}, {k.dtype} and {v.dtype}")
+    dtype = q.dtype
+    code = _lib.DTYPE_CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}; use float32, bfloat16 or float16")
+    if k.dtype is not dtype or v.dtype is not dtype:
+        raise TypeError(f"q, k and v have different dtypes: {dtype}, {k.dtype} and {v.dtype}")
+    packed = cu_seqlens is not None
     lengths = None
-    if cu_seqlens is not None:
+    if packed:
         if seq_lens is not None:
             raise ValueError("give cu_seqlens (packed prompts) or seq_lens (padded ones), not both")
         if B != 1:
@@ -70,27 +75,28 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens
             raise ValueError(f"seq_lens must have shape ({B},), got {tuple(seq_lens.shape)}")
         lengths, name = seq_lens, "seq_lens"
     if lengths is not None:
-        if lengths.dtype not in (torch.int32, torch.int64):
+        if lengths.dtype is not torch.int32 and lengths.dtype is not torch.int64:
             raise TypeError(f"{name} must be int32 or int64, got {lengths.dtype}")
-        if lengths.device.type == "cpu" and lengths.numel():
+        if not lengths.is_cuda and lengths.numel():
             if int(lengths.min()) < 0 or int(lengths.max()) > T:
                 raise ValueError(f"{name} must lie in [0, {T}]")
-            if cu_seqlens is not None and bool((lengths[1:] < lengths[:-1]).any()):
+            if packed and bool((lengths[1:] < lengths[:-1]).any()):
                 raise ValueError("cu_seqlens must ascend")
     dev = _lib.require_cuda(q, k, v)
     lib = _lib.load()
+    n_seqs, cu_at, lens_at = B, 0, 0
     if lengths is not None:
         lengths = _lib.as_device(lengths, dev, torch.int32)
-    q, q_at, *q_strides = _tiles(q)
-    k, k_at, *k_strides = _tiles(k)
-    v, v_at, *v_strides = _tiles(v)
-    out = torch.empty(B, Hq, T, HEAD_DIM, dtype=q.dtype, device=dev)
-    packed = cu_seqlens is not None
-    lens_at = None if lengths is None else lengths.data_ptr()
+        if packed:
+            n_seqs, cu_at = lengths.numel() - 1, lengths.data_ptr()
+        else:
+            lens_at = lengths.data_ptr()
+    q, q_at, q0, q1, q2 = _tiles(q)
+    k, k_at, k0, k1, k2 = _tiles(k)
+    v, v_at, v0, v1, v2 = _tiles(v)
+    out = torch.empty(B, Hq, T, HEAD_DIM, dtype=dtype, device=dev)
+    call = _PROMPT.pack(q_at, k_at, v_at, out.data_ptr(), cu_at, lens_at, _lib.status_word(dev).data_ptr(), q0, q1, q2, k0, k1, k2, v0, v1, v2,
+                        n_seqs, B, T, code, Hq, Hkv, bool(causal), _SCALE if scale is None else scale)
     with _lib.on_device(dev):
-        _lib.check(lib.omni_prompt_attn(
-            q_at, k_at, v_at, _lib.DTYPE_CODE[q.dtype], _STRIDES.pack(*q_strides), _STRIDES.pack(*k_strides), _STRIDES.pack(*v_strides),
-            lens_at if packed else None, lengths.numel() - 1 if packed else B, None if packed else lens_at,
-            B, Hq, Hkv, T, _SCALE if scale is None else scale, bool(causal), out.data_ptr(), _lib.status_word(dev).data_ptr(),
-            _lib.stream_ptr(dev)))
+        _lib.check(lib.omni_prompt_attn(call, _lib.stream_ptr(dev)))
     return out

@@ -1,11 +1,9 @@
 """What the prompt-side and eviction operators refuse, checked before anything reaches a GPU."""
-import ctypes as C
-
 import pytest
 import torch
 
 from omnistack_rs_b200 import _lib, build
-from omnistack_rs_b200.kernels import eviction, position
+from omnistack_rs_b200.kernels import eviction, position, prompt_attention
 from omnistack_rs_b200.kernels.eviction import attn_weight_sums, evict_keys
 from omnistack_rs_b200.kernels.position import qk_norm_rope
 from omnistack_rs_b200.kernels.prompt_attention import prompt_attn
@@ -90,23 +88,22 @@ def test_evict_refusals(change, error, match):
 
 def test_c_entries_refuse_bad_arguments(lib):
     """Checks that need no device: they come before the first CUDA call of each entry."""
-    one = C.c_void_p(32)
     assert lib.omni_qk_norm_rope(None, None) == _lib.ERR_ARG
     def norm_rope(q=16, heads=1, axes=1, pairs=0, end=0, stride=128, dtype=1):
         return lib.omni_qk_norm_rope(position._NORM_ROPE.pack(q, 0, 16, 0, 0, 0, 16, 16, 0, 0, stride, 0, 0, 0, 0, 0, 0, 1, 1, heads, 0, 0, 0, end, 0, 0, 0,
                                                               dtype, axes, pairs, 0, 0, 0, 1, 1e-6), None)
     assert norm_rope(q=0) == norm_rope(q=8) == norm_rope(heads=-1) == norm_rope(pairs=65, end=65) == norm_rope(pairs=8) == _lib.ERR_ARG
     assert norm_rope(stride=132) == norm_rope(dtype=7) == _lib.ERR_ARG and norm_rope(axes=5) == _lib.ERR_UNSUPPORTED and norm_rope(heads=0) == _lib.OK
-    st = (C.c_int64 * 3)(0, 0, 128)
-    prompt = lambda q=one, dt=1, strides=st, n=1, B=1, Hq=2, Hkv=1, T=4, cu=None: lib.omni_prompt_attn(  # noqa: E731
-        q, one, one, dt, strides, st, st, cu, n, None, B, Hq, Hkv, T, 1.0, 1, one, None, None)
-    assert prompt(q=None) == prompt(q=C.c_void_p(8)) == prompt(dt=3) == prompt(Hq=3, Hkv=2) == prompt(n=2) == _lib.ERR_ARG
-    assert prompt(strides=(C.c_int64 * 3)(0, 0, 130)) == prompt(cu=one, B=2) == prompt(T=-1) == _lib.ERR_ARG
+    assert lib.omni_prompt_attn(None, None) == lib.omni_attn_weight_sums(None, None) == _lib.ERR_ARG
+    prompt = lambda q=32, out=32, dt=1, stride=128, n=1, B=1, Hq=2, Hkv=1, T=4, cu=0: lib.omni_prompt_attn(prompt_attention._PROMPT.pack(  # noqa: E731
+        q, 32, 32, out, cu, 0, 0, 0, 0, stride, 0, 0, 128, 0, 0, 128, n, B, T, dt, Hq, Hkv, 1, 1.0), None)
+    assert prompt(q=0) == prompt(q=8) == prompt(out=16) == prompt(dt=3) == prompt(Hq=3, Hkv=2) == prompt(n=2) == _lib.ERR_ARG
+    assert prompt(stride=130) == prompt(cu=32, B=2) == prompt(T=-1) == _lib.ERR_ARG
     assert prompt(T=1 << 31) == _lib.ERR_UNSUPPORTED and prompt(T=0) == _lib.OK
     assert lib.omni_attn_weight_sums_workspace_bytes(0, 4, 2, 1, 100) == 0
-    sums = lambda q=one, Hq=4, Hkv=2, S=64, ws=0: lib.omni_attn_weight_sums(  # noqa: E731
-        q, 1, one, one, one, one, 0, None, 0, None, 1, Hq, Hkv, 1, S, 1.0, 1, 0, 1, 0, one, ws, one, None, None)
-    assert sums(q=None) == sums(Hq=3) == sums(ws=0) == _lib.ERR_ARG and sums(S=0) == _lib.OK
+    sums = lambda q=16, Hq=4, Hkv=2, S=64, ws=0: lib.omni_attn_weight_sums(eviction._WEIGHT_SUMS.pack(  # noqa: E731
+        q, 16, 16, 16, 16, 0, 0, 16, 16, 0, 1, S, ws, 1, 0, 0, Hq, Hkv, 1, 1, 0, 1, 0, 1.0), None)
+    assert sums(q=0) == sums(Hq=3) == sums(ws=0) == _lib.ERR_ARG and sums(S=0) == _lib.OK
     assert sums(Hq=2048, Hkv=2048) == _lib.ERR_UNSUPPORTED
     assert lib.omni_evict_keys(None, None) == _lib.ERR_ARG
     evict = lambda capacity, nib=16, B=1: lib.omni_evict_keys(  # noqa: E731

@@ -253,7 +253,7 @@ extern "C" int32_t omni_evict_keys(const omni_evict_t* call, void* stream) {
     OMNI_REQUIRE(a.B >= 0 && a.H >= 0 && a.S >= 0, OMNI_ERR_ARG, "omni_evict_keys: negative extent");
     OMNI_REQUIRE(a.budget >= 1 && a.recent >= 0 && a.recent <= a.budget && a.capacity >= a.budget, OMNI_ERR_ARG,
                  "omni_evict_keys: need 0 <= recent <= budget <= capacity and budget >= 1");
-    OMNI_REQUIRE(a.S <= 0x7fffff00LL && a.budget <= 0x7fffff00LL && a.B * a.H <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_evict_keys: extent past 2^31");
+    OMNI_REQUIRE(a.S <= 0x7fff0000LL && a.budget <= 0x7fff0000LL && a.B * a.H <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_evict_keys: extent past 2^31");
     if (a.B == 0 || a.H == 0) return OMNI_OK;
     OMNI_REQUIRE((a.S == 0 || (a.sums && a.k_nib && a.k_qjl && a.k_norms && a.v_nib)) && a.sums_out && a.k_nib_out && a.k_qjl_out && a.k_norms_out &&
                  a.v_nib_out && a.index && a.new_lens, OMNI_ERR_ARG, "omni_evict_keys: NULL buffer");

@@ -203,6 +203,9 @@ class QuantizedKVCache:
                 _lib.ptr(self.v_norms), S, _lib.ptr(self.lens), _lib.ptr(self.lens32), int(self.pair_v), _lib.stream_ptr(dev)))
         return True
 
+    def _capturing(self) -> bool:
+        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompt_lens: Optional[torch.Tensor] = None, *,
                 causal: bool = True, scale: Optional[float] = None, rotate: bool = True) -> torch.Tensor:
         """Take in every user's prompt: ``prompt_attn`` of ``q`` (n_users, n_heads, T, 128) over ``k`` and ``v`` (n_users,
@@ -233,8 +236,11 @@ class QuantizedKVCache:
                 causal: bool = True) -> torch.Tensor:
         """Add the attention weight that every cached key receives from ``q`` (n_users, n_heads, T, 128), the queries of the last T
         tokens, to ``weight_sums`` (float32 (n_users, n_kv_heads, max_len), kept from the first call on), which decides what
-        :meth:`evict` keeps.  Arguments as in :meth:`attend`; returns ``weight_sums``."""
+        :meth:`evict` keeps.  Arguments as in :meth:`attend`; returns ``weight_sums``.  A CUDA graph may hold every call but the
+        first."""
         if self.weight_sums is None:
+            if self._capturing():                  # the zeros would be part of the graph, and every replay would start from them
+                raise RuntimeError("the first observe makes weight_sums: call it once before the capture")
             self.weight_sums = torch.zeros(self.n_users, self.n_kv_heads, self.max_len, dtype=torch.float32, device=self.device)
         return attn_weight_sums(q, self.k_nib, self.k_qjl, self.k_norms, self.codebooks, self.user_ids, scale, with_qjl,
                                 seq_lens=self.lens32, rotate_q=rotate_q, causal=causal, into=self.weight_sums)
@@ -244,7 +250,9 @@ class QuantizedKVCache:
         (without a call of :meth:`observe`, the first ones).  The kept rows move into new arrays of ``max_len`` rows (the cache's
         present capacity when ``None``; a smaller one gives memory back), their sums with them.  Returns the kept keys' old
         positions, int32 (n_users, n_kv_heads, budget), -1 behind a user's keys.  Calls captured on the old arrays
-        (``GraphedAttention``, ``HostDecodeStep``) have to be made anew."""
+        (``GraphedAttention``, ``HostDecodeStep``) have to be made anew, and the call itself takes no part in a capture."""
+        if self._capturing():                      # the new arrays would hold nothing until a replay, and every replay would move old rows
+            raise RuntimeError("evict replaces the cache's arrays: it cannot be captured (evict_keys can)")
         capacity = self.max_len if max_len is None else int(max_len)
         sums = self.weight_sums
         if sums is None:

@@ -96,3 +96,68 @@ def test_prefill_refusals_and_defaults():
     big = make_cache(False, True, max_len=10)
     with pytest.raises(ValueError, match="capacity"):
         big.prefill(x, x, x)
+
+
+@pytest.mark.parametrize("pair_v", [False, True])
+@pytest.mark.parametrize("T", [1, 33])
+def test_padding_of_a_prompt_reaches_nothing(pair_v, T):
+    """Rows behind a prompt may hold anything: the packed rows they leave behind the length are never attended to.  The prompt's own
+    rows beside infinities or NaN are computed again with unrounded weights, the others with weights rounded to bf16: half a step,
+    2^-8, of each weight and so at most of max |v| in the result, and each result is rounded once, 2^-8 of at most max |v| each."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = [torch.randn(3, h, 40, 128, generator=g, device=DEV, dtype=torch.bfloat16) for h in (4, 2, 2)]
+    lens = torch.tensor([40, 13, 0])
+    top = float(x[2].float().abs().max())
+    results = []
+    for fill in (0.0, float("nan"), float("inf")):
+        rows = [t.clone() for t in x]
+        for b, m in enumerate(lens.tolist()):
+            for t in rows:
+                t[b, :, m:] = fill
+        cache = make_cache(pair_v, True)
+        out = cache.prefill(*rows, lens)
+        q = torch.randn(3, 4, T, 128, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV, dtype=torch.bfloat16)
+        got = [out, cache.attend(q), cache.observe(q).clone()]
+        index = cache.evict(9, recent=2)
+        results.append(got + [index, cache.k_nib, cache.v_nib, cache.k_norms, cache.weight_sums, cache.attend(q)])
+    for got in results:
+        assert all(bool(torch.isfinite(t.float()).all()) for t in got)
+        assert all(torch.equal(a, b) for a, b in zip(got[1:], results[0][1:]))
+        assert float((got[0].float() - results[0][0].float()).abs().max()) <= 3 * 2 ** -8 * 1.001 * top
+        assert all(bool((got[0][b, :, m:] == 0).all()) for b, m in enumerate(lens.tolist()))
+    assert bool((results[0][0][2] == 0).all()) and bool((results[0][2][2] == 0).all())
+
+
+def test_empty_prompts():
+    cache = make_cache(True, True)
+    x = torch.randn(3, 2, 0, 128, device=DEV)
+    assert cache.prefill(x, x, x).shape == (3, 2, 0, 128) and cache.lens.tolist() == [0, 0, 0]
+    assert bool((cache.evict(4) == -1).all())
+    q = torch.randn(3, 4, 1, 128, device=DEV)
+    assert bool((cache.observe(q) == 0).all())
+
+
+def test_captures():
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(3, 2, 40, 128, generator=g, device=DEV, dtype=torch.bfloat16)
+    q = torch.randn(3, 4, 1, 128, generator=g, device=DEV, dtype=torch.bfloat16)
+    cache, plain = make_cache(True, False), make_cache(True, False)
+    for c in (cache, plain):
+        c.prefill(x, x, x)
+    plain.observe(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            cache.observe(q)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            cache.evict(8)
+    assert cache.weight_sums is None and cache.max_len == 160
+    cache.observe(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.observe(q)
+    for _ in range(3):
+        graph.replay()
+        plain.observe(q)
+    assert torch.equal(cache.weight_sums, plain.weight_sums)
+    assert torch.equal(cache.evict(8, recent=2), plain.evict(8, recent=2))

@@ -1,7 +1,7 @@
 // Key weights of many columns (a prompt's last tokens): tcgen05 products in two passes over the keys.
 //
 // Query columns are the rows of the product (128 at a time), keys its columns:  S[col, key] = Q'[col, :] . K'[key, :].  Q' is made
-// once by a launch of its own (rotation, scaling, G . q, fp16 values and remainders) and lives in tensor memory for a whole CTA, K' is dequantised tile by tile (128 keys) into shared memory, twice: values and what they
+// once by a launch of its own (rotation, scaling, G . q, fp16 values and remainders) and lives in tensor memory for a span, K' is dequantised tile by tile (128 keys) into shared memory, twice: values and what they
 // leave of the centroids, plus the signs.  Two accumulators, since a key's norm multiplies the sign product alone and would have to
 // be split as well to ride in it:   A = Qhi Khi + Qhi Klo (+ Qlo Khi),   B = Chi sign + Clo sign,   s = f_A A + f_B norm B.
 //
@@ -12,7 +12,8 @@
 // the columns: a halving exchange between the lanes of a warp, then the four warps' parts in order.
 //
 // Warps 0-7: scores, two threads per column with 64 of a tile's keys each.  Warps 8-15: dequantisation, two threads per key, up to
-// two buffers ahead of the products.  Warp 16 issues the products.  (One thread per column and key left each scheduler two warps,
+// two buffers ahead of the products; with a span's first tile they bring its columns (the score warps doing so between two spans had the
+// products wait: 210 us instead of 190 for 16 users x 8 heads x up to 8,192 keys x 128 columns).  Warp 16 issues the products.  (One thread per column and key left each scheduler two warps,
 // which issued an instruction every third cycle: 135 us for a pass of 16 users x 8,192 keys x 128 columns.)  Shared memory bounds
 // a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the products' reads of K', about 1,900 cycles against 1,536
 // of the tensor pipe.
@@ -39,7 +40,13 @@ constexpr uint32_t kWwLutBytes = 256 * 16 * 8;
 constexpr uint32_t kWwBuf = 2 * kWwBytesV + kWwBytesSign;           // values, remainders, signs
 constexpr uint32_t kWwOffLut = 2 * kWwBuf, kWwOffNorm = kWwOffLut + kWwLutBytes, kWwOffRed = kWwOffNorm + 4 * kWwTile * 4,
                    kWwOffBar = kWwOffRed + 4 * kWwTile * 4, kWwSmem = kWwOffBar + 128;
-constexpr uint32_t kWwColA = 0, kWwColB = 128, kWwColQhi = 256, kWwColQlo = 320, kWwColChi = 384, kWwColClo = 416, kWwTmemCols = 512;
+// Tensor memory: accumulators, then Q'.  Without remainders two sets of it fit, and the next head's columns are written while products
+// read this head's.
+constexpr uint32_t kWwColA = 0, kWwColB = 128, kWwColQ = 256, kWwTmemCols = 512;
+template <bool QLO> struct WwSet {
+    static constexpr uint32_t kQlo = 64, kChi = QLO ? 128 : 64, kClo = QLO ? 160 : 96;   // columns behind those of Q' values
+    static constexpr uint32_t kNext = QLO ? 0 : 128;                     // columns from one set to the other
+};
 constexpr uint32_t kWwWaitLimit = 1u << 22;
 
 __device__ __forceinline__ void ww_bar_init(uint32_t bar, uint32_t count) {
@@ -247,9 +254,8 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(ww_smem);
     float* norm_s = reinterpret_cast<float*>(ww_smem + kWwOffNorm);      // ring of four tiles' norms
     float* red_s = reinterpret_cast<float*>(ww_smem + kWwOffRed);
-    const uint32_t bar_full = base + kWwOffBar, bar_empty = bar_full + 16, bar_s = bar_empty + 16, bar_free = bar_s + 16, bar_q = bar_free + 16, tmem_at = bar_q + 8;
+    const uint32_t bar_full = base + kWwOffBar, bar_empty = bar_full + 16, bar_s = bar_empty + 16, bar_free = bar_s + 16, tmem_at = bar_free + 16;
     if (tid == 0) {
-        ww_bar_init(bar_q, 8);
         for (int i = 0; i < 2; ++i) {
             ww_bar_init(bar_full + 8 * i, 8);
             ww_bar_init(bar_empty + 8 * i, 1);
@@ -275,11 +281,12 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" :: "n"(kWwOtherRegs));
         // ---- products ---------------------------------------------------------------------------------------------------
-        int span_end = 0, spans = 0;
+        using Set = WwSet<QLO>;
+        int span_end = 0;
+        uint32_t tq = tmem + kWwColQ + Set::kNext;                       // this span's columns
         for (int t = 0; warp == 16 && ok && t < n_share; ++t) {
             if (t == span_end) {                                         // another head's columns
-                ok = ww_bar_wait(bar_q, spans++ & 1);
-                if (!ok) break;
+                tq = tmem + kWwColQ + (tq == tmem + kWwColQ ? Set::kNext : 0);
                 span_end += at.n_tiles - at.tile;
                 if (span_end < n_share) at.next_head(a);
             }
@@ -294,18 +301,18 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                     const uint32_t kx = kv + x * 8 * kWwSbo, sx = kv + 2 * kWwBytesV + x * 8 * kWwSboSign, da = tmem + kWwColA + 64 * x, db = tmem + kWwColB + 64 * x;
                     // the remainders' products first: added to an accumulator that already holds the values', each would cost it a rounding
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + kWwBytesV + ks * 2 * kWwLbo, kWwSbo, 64, ks > 0);
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tq + 8 * ks, kx + kWwBytesV + ks * 2 * kWwLbo, kWwSbo, 64, ks > 0);
                     if (QLO) {
 #pragma unroll
-                        for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQlo + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, 1);
+                        for (int ks = 0; ks < 8; ++ks) ww_mma(da, tq + Set::kQlo + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, 1);
                     }
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tmem + kWwColQhi + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, 1);
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(da, tq + 8 * ks, kx + ks * 2 * kWwLbo, kWwSbo, 64, 1);
                     if (a.with_qjl) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColClo + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, ks > 0);
+                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tq + Set::kClo + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, ks > 0);
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tmem + kWwColChi + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, 1);
+                        for (int ks = 0; ks < 4; ++ks) ww_mma(db, tq + Set::kChi + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, 64, 1);
                     }
                     if (x == 1) ww_commit(bar_empty + 8 * (t & 1));
                     ww_commit(bar_s + 8 * x);
@@ -335,7 +342,8 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             }
         };
         fetch();
-        bool new_table = true;
+        bool new_table = true, new_span = true;
+        uint32_t tq = t_lane + kWwColQ + WwSet<QLO>::kNext;
         for (int t = 0; t < n_share; ++t) {
             if (new_table) {                                             // no lookup of the previous table is still to come
                 asm volatile("bar.sync 2, 256;\n" ::: "memory");
@@ -344,6 +352,35 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             }
             if (ok && t > 1) ok = ww_bar_wait(bar_empty + 8 * (t & 1), ((t >> 1) - 1) & 1);
             // (a warp whose wait ran out stays for the barriers of the others and leaves behind the loop)
+            if (new_span) {
+                // Q' of another head's columns into tensor memory, half of each part per thread: it comes with the span's first tile.  Two
+                // sets: that wait was for the second tile back, so no product reads the set of the span before the last one any more.
+                tq = t_lane + kWwColQ + (tq == t_lane + kWwColQ ? WwSet<QLO>::kNext : 0);
+                if (QLO && ok && t > 0) ok = ww_bar_wait(bar_empty + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
+                if (ok) {
+                    ww_fence_after();
+                    const int64_t bh = (int64_t)at.b * a.Hkv + at.h;
+                    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(a.prepared) + (bh * ((cols + kWwTile - 1) / kWwTile) + col0 / kWwTile) * kWwPrepBytes) + row;
+                    const bool col_on = col0 + row < cols;
+                    // four pieces at a time: 64 values, their remainders, 32 values of G . q, their remainders (more registers would spill)
+#pragma unroll 1
+                    for (int part = 0; part < 6; ++part) {
+                        const bool of_q = part < 4;
+                        if (of_q ? !QLO && part > 1 : !a.with_qjl) continue;
+                        const uint4* from = src + (size_t)(of_q ? 16 * (part >> 1) + 8 * half + 4 * (part & 1) : 32 + 8 * (part - 4) + 4 * half) * kWwTile;
+                        uint32_t v[16];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint4 x4 = col_on ? from[i * kWwTile] : make_uint4(0u, 0u, 0u, 0u);
+                            v[4 * i] = x4.x; v[4 * i + 1] = x4.y; v[4 * i + 2] = x4.z; v[4 * i + 3] = x4.w;
+                        }
+                        ww_st16(tq + (of_q ? WwSet<QLO>::kQlo * (part >> 1) + 32 * half + 16 * (part & 1)
+                                           : (part == 4 ? WwSet<QLO>::kChi : WwSet<QLO>::kClo) + 16 * half), v);
+                    }
+                    ww_wait_st();
+                    ww_fence_before();
+                }
+            }
             const uint32_t kv = base + (t & 1) * kWwBuf;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {                                // sixteen lookups, then their eight stores
@@ -370,7 +407,8 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             if (half == 0) norm_s[(t & 3) * kWwTile + x] = norm * norm_mul;
             if (t + 1 < n_share) {
                 const int h = at.h;
-                if (++at.tile == at.n_tiles) at.next_head(a);
+                new_span = ++at.tile == at.n_tiles;
+                if (new_span) at.next_head(a);
                 new_table = a.cb_per_head && at.h != h;
                 fetch();
             }
@@ -391,37 +429,6 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             float* sums = a.sums + bh * a.S;
             const unsigned char* prep = reinterpret_cast<const unsigned char*>(a.prepared) + (bh * ((cols + kWwTile - 1) / kWwTile) + col0 / kWwTile) * kWwPrepBytes;
             const float f = col_on ? reinterpret_cast<const float*>(prep + (size_t)kWwPrepRows * kWwTile * 16)[row] : 1.f;
-            // Q' of the columns into tensor memory, half of each part per thread, once no product of the previous span reads it
-            if (ok && done > 0) ok = ww_bar_wait(bar_empty + 8 * ((done - 1) & 1), ((done - 1) >> 1) & 1);
-            ww_fence_after();
-            {
-                const uint4* src = reinterpret_cast<const uint4*>(prep) + row;
-                auto piece = [&](int r, uint32_t* dst) {
-                    const uint4 x = col_on ? src[(size_t)r * kWwTile] : make_uint4(0u, 0u, 0u, 0u);
-                    dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w;
-                };
-                uint32_t v[32], r[32], p[16], o[16];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) piece(8 * half + i, v + 4 * i);
-                if (QLO) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) piece(16 + 8 * half + i, r + 4 * i);
-                }
-                if (a.with_qjl) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { piece(32 + 4 * half + i, p + 4 * i); piece(40 + 4 * half + i, o + 4 * i); }
-                }
-                ww_st32(t_lane + kWwColQhi + 32 * half, v);
-                if (QLO) ww_st32(t_lane + kWwColQlo + 32 * half, r);
-                if (a.with_qjl) {
-                    ww_st16(t_lane + kWwColChi + 16 * half, p);
-                    ww_st16(t_lane + kWwColClo + 16 * half, o);
-                }
-                ww_wait_st();
-                ww_fence_before();
-                __syncwarp();
-                if (lane == 0) ww_bar_arrive(bar_q);
-            }
             const int last = col_on ? (a.causal ? len - a.T + col % a.T : len - 1) : -1;    // newest key of the column
             const int open_to = a.causal ? len - a.T : len - 1;          // newest key that every column sees
             float m = -INFINITY, l = 0.f, top_all = 0.f, inv = 0.f;          // pass 2: the column's maximum and reciprocal sum
@@ -430,10 +437,17 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                 const int64_t first = ((int64_t)a.tiles_before[at.b]) * a.Hkv + (int64_t)at.h * at.n_tiles;
                 const int64_t c0 = ws_cta_of(first, gridDim.x, all), c1 = ws_cta_of(first + at.n_tiles - 1, gridDim.x, all);
                 const float2* p = a.partial + (bh + c0) * cols + col;
-                for (int64_t i = 0; i <= c1 - c0; ++i) m = fmaxf(m, p[i * cols].x);
-                const float ref = m == -INFINITY ? 0.f : m;
-                for (int64_t i = 0; i <= c1 - c0; ++i) l += p[i * cols].y * exp2f(p[i * cols].x - ref);
-                top_all = ref;
+                for (int64_t i = 0; i <= c1 - c0; i += 4) {              // seldom more than three
+                    float2 e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[k] = i + k <= c1 - c0 ? p[(i + k) * cols] : make_float2(-INFINITY, 0.f);
+                    const float top = fmaxf(fmaxf(fmaxf(m, e[0].x), fmaxf(e[1].x, e[2].x)), e[3].x), ref = top == -INFINITY ? 0.f : top;
+                    l *= exp2f(m - ref);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) l += e[k].y * exp2f(e[k].x - ref);
+                    m = top;
+                }
+                top_all = m == -INFINITY ? 0.f : m;
                 inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;         // no open key: its scores are -inf
             }
             for (int t = done; t < done + n_span; ++t) {

@@ -20,11 +20,7 @@ namespace omni {
 constexpr int kWmWarps = 8;
 constexpr int kWmLutBytes = 256 * 32 * 8;
 
-__device__ __forceinline__ void wm_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// ... into a fresh accumulator
+// wm_mma into a fresh accumulator
 __device__ __forceinline__ void wm_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
@@ -56,93 +52,16 @@ __global__ void __launch_bounds__(kWmPrepWarps * 32) weight_fragments_kernel(con
     for (int x = 8; x >= 1; x >>= 1) cb_top = fmaxf(cb_top, __shfl_xor_sync(kFullMask, cb_top, x));
     const float cb_mul = ws_pow2(cb_top);
 
-    // ---- query fragments: lane (g, c) has dims 32c .. 32c + 31 of column g --------------------------------------------
     uint32_t qv[8][2], qr[QLO ? 8 : 1][2];
-    float q_mul;
-    {
-        float q[32];
-        const int64_t qrow = g < cols ? (b * a.Hq + (int64_t)h * G + g / a.T) * a.T + g % a.T : 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (g < cols) load8<DT>(a.q, qrow * kHeadDim + 32 * c + 8 * i, v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) q[8 * i + k] = v[k];
-        }
-        if (a.rotate_q) {                                            // Walsh-Hadamard over 4 lanes x 32 elements, stages in order
-#pragma unroll
-            for (int s = 1; s < 32; s <<= 1) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if ((i & s) == 0) {
-                        const float x = q[i], y = q[i | s];
-                        q[i] = __fadd_rn(x, y);
-                        q[i | s] = __fsub_rn(x, y);
-                    }
-                }
-            }
-#pragma unroll
-            for (int s = 1; s < 4; s <<= 1) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float o = __shfl_xor_sync(kFullMask, q[i], s);
-                    q[i] = (c & s) ? __fsub_rn(o, q[i]) : __fadd_rn(q[i], o);
-                }
-            }
-            const float s = __uint_as_float(OMNI_WHT_SCALE_BITS);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) q[i] = __fmul_rn(q[i], s);
-        }
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(q[i]));
-        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
-        q_mul = ws_pow2(top);
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float u = q[4 * ks + 2 * x] * q_mul, v = q[4 * ks + 2 * x + 1] * q_mul;
-                qv[ks][x] = ws_half2(u, v);
-                if (QLO) qr[ks][x] = ws_rest2(u, v, qv[ks][x]);
-            }
-        }
-    }
-    // ---- G . q of the head's 64 projections (G is +-1: exact), sixteen at a time, handed over through shared memory -----------
+    float p[16];
+    const float q_mul = ws_columns8<DT, QLO>(a, b, h, g < cols ? g : -1, 1.f, c_s[warp], lane, qv, qr, p);
+    // ---- G . q of the head's 64 projections -------------------------------------------------------------------------------------
     uint32_t pv[4][2], pr[4][2];
     float p_mul = 1.f;
     if (a.with_qjl) {
-        const int32_t uid = a.user_ids ? __ldg(a.user_ids + b) : a.user_id;
-        const uint32_t* gr = a.g_rows + (size_t)seed_of(uid, h) * kQjlDim * 4 + g * 4 + c;
-        uint32_t gw[4][2];
+        float top = 0.f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) { gw[t][0] = __ldg(gr + 64 * t); gw[t][1] = __ldg(gr + 64 * t + 32); }
-        float (*cw)[kQjlDim + 4] = c_s[warp];
-        __syncwarp();
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                const uint32_t a0 = ws_signs2(gw[t][0] >> (4 * ks)), a1 = ws_signs2(gw[t][1] >> (4 * ks));
-                const uint32_t a2 = ws_signs2(gw[t][0] >> (4 * ks + 2)), a3 = ws_signs2(gw[t][1] >> (4 * ks + 2));
-                wm_mma(d, a0, a1, a2, a3, qv[ks][0], qv[ks][1]);
-                if (QLO) wm_mma(d, a0, a1, a2, a3, qr[ks][0], qr[ks][1]);
-            }
-            cw[2 * c][16 * t + g] = d[0];
-            cw[2 * c + 1][16 * t + g] = d[1];
-            cw[2 * c][16 * t + g + 8] = d[2];
-            cw[2 * c + 1][16 * t + g + 8] = d[3];
-        }
-        __syncwarp();
-        float p[16], top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(&cw[g][16 * c + i]);
-            p[i] = v.x; p[i + 1] = v.y; p[i + 2] = v.z; p[i + 3] = v.w;
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(p[i]));
         top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
         top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
         p_mul = ws_pow2(top);

@@ -55,6 +55,100 @@ __device__ __forceinline__ uint32_t ws_signs2(uint32_t bits) {
     return 0xBC00BC00u ^ (((bits & 1u) << 15) | ((bits & 2u) << 30));
 }
 
+__device__ __forceinline__ void wm_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight columns of one head by a warp: lane (g, c) = (lane / 4, lane % 4) has dims 32c .. 32c + 31 of its column `col` (of the head's;
+// -1: zeros), rotated where asked and scaled by the power of two returned, which takes the sign of `sign`: qv[ks] holds dims 32c + 4ks .. + 3 as
+// fp16, qr what those leave (QLO).  p: projections 16c .. 16c + 15 of G . q (G is +-1: exact products), handed over through `hand`.
+template <int DT, bool QLO>
+__device__ __forceinline__ float ws_columns8(const WeightArgs& a, int64_t b, int h, int col, float sign, float (*hand)[kQjlDim + 4], int lane,
+                                             uint32_t (&qv)[8][2], uint32_t (&qr)[QLO ? 8 : 1][2], float (&p)[16]) {
+    const int g = lane >> 2, c = lane & 3, G = a.Hq / a.Hkv;
+    float q[32];
+    const int64_t qrow = col >= 0 ? (b * a.Hq + (int64_t)h * G + col / a.T) * a.T + col % a.T : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (col >= 0) load8<DT>(a.q, qrow * kHeadDim + 32 * c + 8 * i, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[8 * i + k] = v[k];
+    }
+    uint32_t gw[4][2];
+    if (a.with_qjl) {
+        const int32_t uid = a.user_ids ? __ldg(a.user_ids + b) : a.user_id;
+        const uint32_t* gr = a.g_rows + (size_t)seed_of(uid, h) * kQjlDim * 4 + g * 4 + c;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) { gw[t][0] = __ldg(gr + 64 * t); gw[t][1] = __ldg(gr + 64 * t + 32); }
+    }
+    if (a.rotate_q) {                                                // Walsh-Hadamard over 4 lanes x 32 elements, stages in order
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                if ((i & s) == 0) {
+                    const float x = q[i], y = q[i | s];
+                    q[i] = __fadd_rn(x, y);
+                    q[i | s] = __fsub_rn(x, y);
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 1; s < 4; s <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float o = __shfl_xor_sync(kFullMask, q[i], s);
+                q[i] = (c & s) ? __fsub_rn(o, q[i]) : __fadd_rn(q[i], o);
+            }
+        }
+        const float s = __uint_as_float(OMNI_WHT_SCALE_BITS);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) q[i] = __fmul_rn(q[i], s);
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(q[i]));
+    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+    const float q_mul = copysignf(ws_pow2(top), sign);
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const float u = q[4 * ks + 2 * x] * q_mul, v = q[4 * ks + 2 * x + 1] * q_mul;
+            qv[ks][x] = ws_half2(u, v);
+            if (QLO) qr[ks][x] = ws_rest2(u, v, qv[ks][x]);
+        }
+    }
+    if (a.with_qjl) {                                                // sixteen projections at a time
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                const uint32_t a0 = ws_signs2(gw[t][0] >> (4 * ks)), a1 = ws_signs2(gw[t][1] >> (4 * ks));
+                const uint32_t a2 = ws_signs2(gw[t][0] >> (4 * ks + 2)), a3 = ws_signs2(gw[t][1] >> (4 * ks + 2));
+                wm_mma(d, a0, a1, a2, a3, qv[ks][0], qv[ks][1]);
+                if (QLO) wm_mma(d, a0, a1, a2, a3, qr[ks][0], qr[ks][1]);
+            }
+            hand[2 * c][16 * t + g] = d[0];
+            hand[2 * c + 1][16 * t + g] = d[1];
+            hand[2 * c][16 * t + g + 8] = d[2];
+            hand[2 * c + 1][16 * t + g + 8] = d[3];
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&hand[g][16 * c + i]);
+            p[i] = v.x; p[i + 1] = v.y; p[i + 2] = v.z; p[i + 3] = v.w;
+        }
+    }
+    return q_mul;
+}
+
 // Centroid table of a head in shared memory: the entry of a code byte holds the fp16 values of both centroids and what they
 // leave, 8 bytes in COPIES copies side by side.  An 8-byte load is served in two half-warps, so sixteen copies (128 bytes per entry,
 // 32 KiB) keep the lanes in banks of their own; thirty-two (256 bytes, 64 KiB) let one byte permutation make a lane's address.

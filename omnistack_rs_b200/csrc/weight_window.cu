@@ -9,14 +9,15 @@
 // them.  A run of tiles of one head inside a share is a span; span (head, CTA) is number head + CTA, which no other span has.
 // Pass 1: thread = column, running maximum and sum over a span's keys, one pair per (span, column) into the workspace.
 // Pass 2: the same scores again (cheaper than 4 bytes per key and column written and read), weights 2^(s - max) / sum, and their sum over
-// the columns: a halving exchange between the lanes of a warp, then the four warps' parts in order.
+// the columns.  There a thread reads four columns of 16 keys (the 16-row form of the tensor-memory load), so that most of the sum is its
+// own: eight lanes trade halves, then the four warps' parts in order (one column of 64 keys per thread: 62 instead of 14 exchanges).
 //
 // Warps 0-7: scores, two threads per column with 64 of a tile's keys each.  Warps 8-15: dequantisation, two threads per key, up to
 // two buffers ahead of the products; with a span's first tile they bring its columns (the score warps doing so between two spans had the
 // products wait: 210 us instead of 190 for 16 users x 8 heads x up to 8,192 keys x 128 columns).  Warp 16 issues the products.  (One thread per column and key left each scheduler two warps,
 // which issued an instruction every third cycle: 135 us for a pass of 16 users x 8,192 keys x 128 columns.)  Shared memory bounds
 // a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the products' reads of K', about 1,900 cycles against 1,536
-// of the tensor pipe.
+// of the tensor pipe; measured, a tile takes 3,200 and the call 171 us, 18.7 of which its products would need alone.
 #include "weight_sums.cuh"
 
 namespace omni {
@@ -39,7 +40,7 @@ constexpr uint32_t kWwBytesV = 128 * 128 * 2, kWwBytesSign = 128 * 64 * 2;
 constexpr uint32_t kWwLutBytes = 256 * 16 * 8;
 constexpr uint32_t kWwBuf = 2 * kWwBytesV + kWwBytesSign;           // values, remainders, signs
 constexpr uint32_t kWwOffLut = 2 * kWwBuf, kWwOffNorm = kWwOffLut + kWwLutBytes, kWwOffRed = kWwOffNorm + 4 * kWwTile * 4,
-                   kWwOffBar = kWwOffRed + 4 * kWwTile * 4, kWwSmem = kWwOffBar + 128;
+                   kWwOffBar = kWwOffRed + 2 * 4 * kWwTile * 4, kWwSmem = kWwOffBar + 128;
 // Tensor memory: accumulators, then Q'.  Without remainders two sets of it fit, and the next head's columns are written while products
 // read this head's.
 constexpr uint32_t kWwColA = 0, kWwColB = 128, kWwColQ = 256, kWwTmemCols = 512;
@@ -94,6 +95,16 @@ __device__ __forceinline__ void ww_ld32(uint32_t taddr, uint32_t* v) {
                    "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(taddr) : "memory");
 }
+// 16 rows x 64 columns: v[4 i ..] holds columns 8 i + 2 (lane % 4) and the next one of rows lane / 4 and lane / 4 + 8
+__device__ __forceinline__ void ww_ld16x64(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void ww_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
                  "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
@@ -140,76 +151,53 @@ __device__ __forceinline__ uint2 ww_lut(uint32_t lut_lane, uint32_t w, int byte)
     return v;
 }
 
-// A warp per column: rotation, power-of-two scaling, G . q, and all of it as fp16 values and remainders.
-constexpr int kWpWarps = 8;
-template <int DT>
+// Eight columns per warp: rotation, power-of-two scaling, G . q, and all of it as fp16 values and remainders.  (A column per warp with
+// sums in fp32 and pieces of 16 bytes every 2 KiB: 25 us for 16,384 columns; four columns: 18 us.)
+constexpr int kWpWarps = 4, kWpCols = 8;
+template <int DT, bool QLO>
 __global__ void __launch_bounds__(kWpWarps * 32) weight_prepare_kernel(const __grid_constant__ WeightArgs a, int64_t col_groups) {
-    __shared__ __align__(16) float q_s[kWpWarps][kHeadDim];
-    __shared__ uint4 g_s[kQjlDim];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ __align__(16) float hand_s[kWpWarps][kWpCols][kQjlDim + 4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     follow_me_early();
     if (blockIdx.x == gridDim.x - 1) {
         ws_tiles_before<kWpWarps>(a, tid);
         return;
     }
     const int64_t bh = blockIdx.x / col_groups, b = bh / a.Hkv;
-    const int h = (int)(bh % a.Hkv), G = a.Hq / a.Hkv, cols = G * a.T;
-    const int col = (int)(blockIdx.x % col_groups) * kWpWarps + warp;
-    if (tid < kQjlDim && a.with_qjl) {
-        const int32_t uid = a.user_ids ? __ldg(a.user_ids + b) : a.user_id;
-        g_s[tid] = __ldg(reinterpret_cast<const uint4*>(a.g_rows + ((size_t)seed_of(uid, h) * kQjlDim + tid) * 4));
-    }
-    float q[4] = {0.f, 0.f, 0.f, 0.f};
-    if (col < cols) Elem<DT>::load4(a.q, ((b * a.Hq + (int64_t)h * G + col / a.T) * a.T + col % a.T) * kHeadDim + 4 * lane, q);
-    if (a.rotate_q) wht128_warp(q, lane);
-    float top = fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3])));
+    const int h = (int)(bh % a.Hkv), cols = a.Hq / a.Hkv * a.T;
+    const int col = ((int)(blockIdx.x % col_groups) * kWpWarps + warp) * kWpCols + g;
+    if (col - g >= cols) return;
+    float cb_top = fabsf(__ldg(a.codebooks + (a.cb_per_head ? h * 16 : 0) + (lane & 15)));
 #pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, x));
+    for (int x = 8; x >= 1; x >>= 1) cb_top = fmaxf(cb_top, __shfl_xor_sync(kFullMask, cb_top, x));
+    uint32_t qv[8][2], qr[QLO ? 8 : 1][2];
+    float p[16];
     // a negative scale goes into the queries, so that the largest product is the largest score
-    const float q_mul = copysignf(ws_pow2(top), a.scale);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { q[k] *= q_mul; q_s[warp][4 * lane + k] = q[k]; }
-    __syncthreads();
+    const float q_mul = ws_columns8<DT, QLO>(a, b, h, col < cols ? col : -1, a.scale, hand_s[warp], lane, qv, qr, p);
     if (col >= cols) return;
     unsigned char* out = reinterpret_cast<unsigned char*>(a.prepared) + (bh * ((cols + kWwTile - 1) / kWwTile) + col / kWwTile) * kWwPrepBytes;
-    const int c = col % kWwTile;
-    {
-        const uint32_t v0 = ws_half2(q[0], q[1]), v1 = ws_half2(q[2], q[3]);
-        const int piece = lane >> 1, at = (lane & 1) * 8;                 // two lanes fill a piece of eight halves
-        *reinterpret_cast<uint2*>(out + ((size_t)piece * kWwTile + c) * 16 + at) = make_uint2(v0, v1);
-        *reinterpret_cast<uint2*>(out + ((size_t)(16 + piece) * kWwTile + c) * 16 + at) = make_uint2(ws_rest2(q[0], q[1], v0), ws_rest2(q[2], q[3], v1));
+    uint4* piece = reinterpret_cast<uint4*>(out) + col % kWwTile;         // a warp's stores fill whole sectors: eight columns side by side
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        piece[(4 * c + i) * kWwTile] = make_uint4(qv[2 * i][0], qv[2 * i][1], qv[2 * i + 1][0], qv[2 * i + 1][1]);
+        if constexpr (QLO) piece[(16 + 4 * c + i) * kWwTile] = make_uint4(qr[2 * i][0], qr[2 * i][1], qr[2 * i + 1][0], qr[2 * i + 1][1]);
     }
-    if (a.with_qjl) {                                                    // projections 2 lane and 2 lane + 1
-        float p[2] = {0.f, 0.f};
-        const uint4 ga = g_s[2 * lane], gb = g_s[2 * lane + 1];
-        const uint32_t wa[4] = {ga.x, ga.y, ga.z, ga.w}, wb[4] = {gb.x, gb.y, gb.z, gb.w};
+    if (a.with_qjl) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int i = 0; i < 2; ++i) {
+            uint32_t v[4], r[4];
 #pragma unroll
-            for (int d = 0; d < 32; d += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(&q_s[warp][32 * w + d]);
-                const float e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    p[0] += __uint_as_float(__float_as_uint(e[k]) ^ (((~wa[w] >> (d + k)) & 1u) << 31));
-                    p[1] += __uint_as_float(__float_as_uint(e[k]) ^ (((~wb[w] >> (d + k)) & 1u) << 31));
-                }
+            for (int k = 0; k < 4; ++k) {
+                const float x = p[8 * i + 2 * k] * kWwProjMul, y = p[8 * i + 2 * k + 1] * kWwProjMul;
+                v[k] = ws_half2(x, y);
+                r[k] = ws_rest2(x, y, v[k]);
             }
+            piece[(32 + 2 * c + i) * kWwTile] = make_uint4(v[0], v[1], v[2], v[3]);
+            piece[(40 + 2 * c + i) * kWwTile] = make_uint4(r[0], r[1], r[2], r[3]);
         }
-        const float x = p[0] * kWwProjMul, y = p[1] * kWwProjMul;
-        const uint32_t v = ws_half2(x, y);
-        const int piece = 32 + (lane >> 2), at = (lane & 3) * 4;
-        *reinterpret_cast<uint32_t*>(out + ((size_t)piece * kWwTile + c) * 16 + at) = v;
-        *reinterpret_cast<uint32_t*>(out + ((size_t)(8 + piece) * kWwTile + c) * 16 + at) = ws_rest2(x, y, v);
     }
-    if (lane == 0) {
-        float cb_top = 0.f;
-        const float* cb = a.codebooks + (a.cb_per_head ? h * 16 : 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) cb_top = fmaxf(cb_top, fabsf(__ldg(cb + i)));
-        // never zero: zero times a masked score's -inf is NaN
-        reinterpret_cast<float*>(out + (size_t)kWwPrepRows * kWwTile * 16)[c] = fmaxf(a.scale * kWsLog2e / q_mul / ws_pow2(cb_top), 1e-30f);
-    }
+    // never zero: zero times a masked score's -inf is NaN
+    if (c == 0) reinterpret_cast<float*>(out + (size_t)kWwPrepRows * kWwTile * 16)[col % kWwTile] = fmaxf(a.scale * kWsLog2e / q_mul / ws_pow2(cb_top), 1e-30f);
 }
 
 // Position in the row of tiles: user, kv head, tile of that head.  Users without keys have no place in it.
@@ -345,22 +333,34 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
         bool new_table = true, new_span = true;
         uint32_t tq = t_lane + kWwColQ + WwSet<QLO>::kNext;
         for (int t = 0; t < n_share; ++t) {
-            if (new_table) {                                             // no lookup of the previous table is still to come
+            // the next tile's rows are requested first: their way from DRAM takes a third of a tile's time
+            const bool table_now = new_table, span_now = new_span;
+            const int h_now = at.h;
+            const int64_t bh_now = (int64_t)at.b * a.Hkv + at.h;
+            const uint4 nib_now[2] = {nib[0], nib[1]};
+            const uint32_t sign_now = sign;
+            const float norm_now = norm;
+            if (t + 1 < n_share) {
+                new_span = ++at.tile == at.n_tiles;
+                if (new_span) at.next_head(a);
+                new_table = a.cb_per_head && at.h != h_now;
+                fetch();
+            }
+            if (table_now) {                                             // no lookup of the previous table is still to come
                 asm volatile("bar.sync 2, 256;\n" ::: "memory");
-                norm_mul = kQjlCoef / kWwProjMul * ws_build_lut<16>(ww_smem + kWwOffLut, a.codebooks + (a.cb_per_head ? at.h * 16 : 0), tid - 256);
+                norm_mul = kQjlCoef / kWwProjMul * ws_build_lut<16>(ww_smem + kWwOffLut, a.codebooks + (a.cb_per_head ? h_now * 16 : 0), tid - 256);
                 asm volatile("bar.sync 2, 256;\n" ::: "memory");
             }
             if (ok && t > 1) ok = ww_bar_wait(bar_empty + 8 * (t & 1), ((t >> 1) - 1) & 1);
             // (a warp whose wait ran out stays for the barriers of the others and leaves behind the loop)
-            if (new_span) {
+            if (span_now) {
                 // Q' of another head's columns into tensor memory, half of each part per thread: it comes with the span's first tile.  Two
                 // sets: that wait was for the second tile back, so no product reads the set of the span before the last one any more.
                 tq = t_lane + kWwColQ + (tq == t_lane + kWwColQ ? WwSet<QLO>::kNext : 0);
                 if (QLO && ok && t > 0) ok = ww_bar_wait(bar_empty + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1);
                 if (ok) {
                     ww_fence_after();
-                    const int64_t bh = (int64_t)at.b * a.Hkv + at.h;
-                    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(a.prepared) + (bh * ((cols + kWwTile - 1) / kWwTile) + col0 / kWwTile) * kWwPrepBytes) + row;
+                    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(a.prepared) + (bh_now * ((cols + kWwTile - 1) / kWwTile) + col0 / kWwTile) * kWwPrepBytes) + row;
                     const bool col_on = col0 + row < cols;
                     // four pieces at a time: 64 values, their remainders, 32 values of G . q, their remainders (more registers would spill)
 #pragma unroll 1
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             const uint32_t kv = base + (t & 1) * kWwBuf;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {                                // sixteen lookups, then their eight stores
-                const uint32_t w[4] = {nib[i].x, nib[i].y, nib[i].z, nib[i].w};
+                const uint32_t w[4] = {nib_now[i].x, nib_now[i].y, nib_now[i].z, nib_now[i].w};
                 uint2 v[4][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -400,18 +400,11 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             if (a.with_qjl) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t bits = sign >> (8 * i);
+                    const uint32_t bits = sign_now >> (8 * i);
                     ww_sts16(kv + sign_at + (uint32_t)i * kWwLbo, ws_signs2(bits), ws_signs2(bits >> 2), ws_signs2(bits >> 4), ws_signs2(bits >> 6));
                 }
             }
-            if (half == 0) norm_s[(t & 3) * kWwTile + x] = norm * norm_mul;
-            if (t + 1 < n_share) {
-                const int h = at.h;
-                new_span = ++at.tile == at.n_tiles;
-                if (new_span) at.next_head(a);
-                new_table = a.cb_per_head && at.h != h;
-                fetch();
-            }
+            if (half == 0) norm_s[(t & 3) * kWwTile + x] = norm_now * norm_mul;
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) ww_bar_arrive(bar_full + 8 * (t & 1));
@@ -450,10 +443,94 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                 top_all = m == -INFINITY ? 0.f : m;
                 inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;         // no open key: its scores are -inf
             }
+            // pass 2: a thread has four columns, rows lane / 4 + 8 r of its warp's 32
+            uint64_t f4[PASS == 2 ? 4 : 1], top4[PASS == 2 ? 4 : 1], inv4[PASS == 2 ? 4 : 1];
+            int last4[PASS == 2 ? 4 : 1];
+            if constexpr (PASS == 2) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int from = 8 * r + (lane >> 2);
+                    const float fr = __shfl_sync(kFullMask, f, from), tr = -__shfl_sync(kFullMask, top_all, from), ir = __shfl_sync(kFullMask, inv, from);
+                    f4[r] = ww_pack2(fr, fr); top4[r] = ww_pack2(tr, tr); inv4[r] = ww_pack2(ir, ir);
+                    last4[r] = __shfl_sync(kFullMask, last, from);
+                }
+            }
             for (int t = done; t < done + n_span; ++t) {
                 // after a wait that ran out the warp still goes through the barriers it shares with the others, storing nothing
                 if (ok) ok = ww_bar_wait(bar_s + 8 * half, t & 1);
                 ww_fence_after();
+                const int k0 = (at.tile + t - done) * kWwTile;
+                const bool masked = k0 + kWwTile - 1 > open_to || k0 + kWwTile > len || cols - col0 < kWwTile;
+                if constexpr (PASS == 2) {
+                    // keys 8 i + 2 (lane % 4) and the next one of the half's 64: weights summed over the thread's four columns
+                    uint64_t sum[8];
+                    const float* nrm = norm_s + (t & 3) * kWwTile + 64 * half + 2 * (lane & 3);
+#pragma unroll
+                    for (int rb = 0; rb < 2; ++rb) {
+                        const uint32_t at16 = t_lane + ((uint32_t)(16 * rb) << 16) + 64 * half;
+                        uint32_t s[32], v[32];                           // products of the values, then the scores / f; of the signs
+                        ww_ld16x64(at16 + kWwColA, s);
+                        if (a.with_qjl) ww_ld16x64(at16 + kWwColB, v);
+                        ww_wait_ld();
+                        if (rb == 1) {
+                            ww_fence_before();
+                            __syncwarp();
+                            if (lane == 0) ww_bar_arrive(bar_free + 8 * half);   // the accumulators may be overwritten
+                        }
+                        if (a.with_qjl) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float2 n2 = *reinterpret_cast<const float2*>(nrm + 8 * i);
+#pragma unroll
+                                for (int r = 0; r < 4; r += 2) {
+                                    const float2 y = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(v[4 * i + r]), __uint_as_float(v[4 * i + r + 1])), ww_pack2(n2.x, n2.y),
+                                                                        ww_pack2(__uint_as_float(s[4 * i + r]), __uint_as_float(s[4 * i + r + 1]))));
+                                    s[4 * i + r] = __float_as_uint(y.x);
+                                    s[4 * i + r + 1] = __float_as_uint(y.y);
+                                }
+                            }
+                        }
+                        if (masked) {
+                            const int l0 = (last4[2 * rb] < len - 1 ? last4[2 * rb] : len - 1) - k0 - 64 * half - 2 * (lane & 3);
+                            const int l1 = (last4[2 * rb + 1] < len - 1 ? last4[2 * rb + 1] : len - 1) - k0 - 64 * half - 2 * (lane & 3);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) s[i] = 8 * (i >> 2) + (i & 1) <= ((i & 2) ? l1 : l0) ? s[i] : 0xff800000u;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[4 * i + 2 * r]), __uint_as_float(s[4 * i + 2 * r + 1])), f4[2 * rb + r], top4[2 * rb + r]));
+                                sum[i] = ww_fma2(ww_pack2(ws_ex2(e.x), ws_ex2(e.y)), inv4[2 * rb + r], rb + r ? sum[i] : ww_pack2(0.f, 0.f));
+                            }
+                        }
+                    }
+                    // and over the eight lanes with other columns: they trade halves of their keys until each has the totals of two
+#pragma unroll
+                    for (int n = 4, x = 16; n >= 1; n >>= 1, x >>= 1) {
+                        const bool up = (lane & x) != 0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (i < n) {
+                                const float2 mine = ww_unpack2(up ? sum[i + n] : sum[i]), other = ww_unpack2(up ? sum[i] : sum[i + n]);
+                                sum[i] = ww_pack2(mine.x + __shfl_xor_sync(kFullMask, other.x, x), mine.y + __shfl_xor_sync(kFullMask, other.y, x));
+                            }
+                        }
+                    }
+                    // two of [four warps of a half][128 keys], so one barrier per tile; the halves do not wait for one another
+                    float* red = red_s + (t & 1) * 4 * kWwTile + 64 * half;
+                    *reinterpret_cast<float2*>(red + (warp & 3) * kWwTile + 2 * lane) = ww_unpack2(sum[0]);
+                    asm volatile("bar.sync %0, 128;\n" :: "r"(3 + half) : "memory");
+                    if (row < 64) {
+                        const float total = (red[row] + red[kWwTile + row]) + (red[2 * kWwTile + row] + red[3 * kWwTile + row]);
+                        const int key = k0 + 64 * half + row;
+                        if (ok && key < len) {
+                            if (a.accumulate || col0 > 0) sums[key] += total;
+                            else sums[key] = total;
+                        }
+                    }
+                    continue;
+                }
                 uint32_t s[64];                                          // products of the values, then the scores / f
                 ww_ld32(t_lane + kWwColA + 64 * half, s);
                 ww_ld32(t_lane + kWwColA + 64 * half + 32, s + 32);
@@ -489,62 +566,27 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                     __syncwarp();
                     if (lane == 0) ww_bar_arrive(bar_free + 8 * half);
                 }
-                const int k0 = (at.tile + t - done) * kWwTile;
-                if (k0 + kWwTile - 1 > open_to || k0 + kWwTile > len || cols - col0 < kWwTile) {
+                if (masked) {
                     const int lim = (last < len - 1 ? last : len - 1) - k0 - 64 * half;
 #pragma unroll
                     for (int i = 0; i < 64; ++i) s[i] = i <= lim ? s[i] : 0xff800000u;
                 }
-                if (PASS == 1) {
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    const float m_new = fmaxf(m, top * f);
-                    const float ref = m_new == -INFINITY ? 0.f : m_new;
-                    const uint64_t f2 = ww_pack2(f, f), r2 = ww_pack2(-ref, -ref);
-                    uint64_t sum[2] = {ww_pack2(0.f, 0.f), ww_pack2(0.f, 0.f)};
+                for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const float m_new = fmaxf(m, top * f);
+                const float ref = m_new == -INFINITY ? 0.f : m_new;
+                const uint64_t f2 = ww_pack2(f, f), r2 = ww_pack2(-ref, -ref);
+                uint64_t sum[2] = {ww_pack2(0.f, 0.f), ww_pack2(0.f, 0.f)};
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
-                        const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, r2));
-                        sum[(i >> 1) & 1] = ww_add2(sum[(i >> 1) & 1], ww_pack2(ws_ex2(e.x), ws_ex2(e.y)));
-                    }
-                    const float2 total = ww_unpack2(ww_add2(sum[0], sum[1]));
-                    l = fmaf(l, ws_ex2(m - ref), total.x + total.y);
-                    m = m_new;
-                } else {
-                    float p[64];
-                    const uint64_t f2 = ww_pack2(f, f), r2 = ww_pack2(-top_all, -top_all);
-#pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
-                        const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, r2));
-                        p[i] = ws_ex2(e.x) * inv;
-                        p[i + 1] = ws_ex2(e.y) * inv;
-                    }
-                    // sum over the warp's 32 columns: lanes trade halves of their keys until each has the totals of two
-#pragma unroll
-                    for (int n = 32, x = 16; n >= 2; n >>= 1, x >>= 1) {
-                        const bool up = (lane & x) != 0;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (i < n) {
-                                const float mine = up ? p[i + n] : p[i], other = up ? p[i] : p[i + n];
-                                p[i] = mine + __shfl_xor_sync(kFullMask, other, x);
-                            }
-                        }
-                    }
-                    float* red = red_s + 64 * half;                          // [four warps of a half][128 keys]
-                    *reinterpret_cast<float2*>(red + (warp & 3) * kWwTile + 2 * lane) = make_float2(p[0], p[1]);
-                    asm volatile("bar.sync 1, 256;\n" ::: "memory");
-                    if (tid < kWwTile) {
-                        const float total = (red_s[tid] + red_s[kWwTile + tid]) + (red_s[2 * kWwTile + tid] + red_s[3 * kWwTile + tid]);
-                        if (ok && k0 + tid < len) {
-                            if (a.accumulate || col0 > 0) sums[k0 + tid] += total;
-                            else sums[k0 + tid] = total;
-                        }
-                    }
-                    asm volatile("bar.sync 1, 256;\n" ::: "memory");
+                for (int i = 0; i < 64; i += 2) {
+                    const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, r2));
+                    sum[(i >> 1) & 1] = ww_add2(sum[(i >> 1) & 1], ww_pack2(ws_ex2(e.x), ws_ex2(e.y)));
                 }
+                const float2 total = ww_unpack2(ww_add2(sum[0], sum[1]));
+                l = fmaf(l, ws_ex2(m - ref), total.x + total.y);
+                m = m_new;
             }
             if (PASS == 1) {                                             // the column's halves
                 float2* hand = reinterpret_cast<float2*>(red_s);
@@ -597,7 +639,7 @@ static int32_t launch_weight_window_t(const WeightArgs& a, unsigned grid, int32_
 }
 
 int32_t launch_weight_window(WeightArgs a, int q_dtype, int32_t* status, cudaStream_t st) {
-    const int64_t heads = a.B * a.Hkv, cols = (int64_t)(a.Hq / a.Hkv) * a.T, col_groups = (cols + kWpWarps - 1) / kWpWarps;
+    const int64_t heads = a.B * a.Hkv, cols = (int64_t)(a.Hq / a.Hkv) * a.T, col_groups = (cols + kWpWarps * kWpCols - 1) / (kWpWarps * kWpCols);
     const int64_t ctas = ww_ctas(heads, a.S);
     OMNI_REQUIRE(heads * col_groups < 0x7fffffffLL && a.B * ((a.S + kWwTile - 1) / kWwTile) <= 0x7fffffffLL, OMNI_ERR_UNSUPPORTED, "omni_attn_weight_sums: too many keys");
     unsigned char* ws = reinterpret_cast<unsigned char*>(a.partial);     // prepared columns, tiles in front of every user, the spans' partial states
@@ -606,14 +648,17 @@ int32_t launch_weight_window(WeightArgs a, int q_dtype, int32_t* status, cudaStr
     a.tiles_before = reinterpret_cast<int32_t*>(ws);
     a.partial = reinterpret_cast<float2*>(ws + ws_before_bytes(a.B));
     const unsigned grid = (unsigned)(heads * col_groups) + 1;
+    const bool qlo = q_dtype == OMNI_F32 || a.rotate_q;                  // a query of a 16-bit type, not rotated, is exact in its fp16 values
     switch (q_dtype) {
-        case OMNI_F32:  weight_prepare_kernel<OMNI_F32><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;
-        case OMNI_BF16: weight_prepare_kernel<OMNI_BF16><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;
-        default:        weight_prepare_kernel<OMNI_F16><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;
+        case OMNI_F32:  weight_prepare_kernel<OMNI_F32, true><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups); break;
+        case OMNI_BF16: if (qlo) weight_prepare_kernel<OMNI_BF16, true><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups);
+                        else weight_prepare_kernel<OMNI_BF16, false><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups);
+                        break;
+        default:        if (qlo) weight_prepare_kernel<OMNI_F16, true><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups);
+                        else weight_prepare_kernel<OMNI_F16, false><<<grid, kWpWarps * 32, 0, st>>>(a, col_groups);
     }
     OMNI_CUDA(cudaGetLastError());
-    // a query of a 16-bit type, not rotated, is exact in its fp16 values
-    return q_dtype == OMNI_F32 || a.rotate_q ? launch_weight_window_t<true>(a, (unsigned)ctas, status, st) : launch_weight_window_t<false>(a, (unsigned)ctas, status, st);
+    return qlo ? launch_weight_window_t<true>(a, (unsigned)ctas, status, st) : launch_weight_window_t<false>(a, (unsigned)ctas, status, st);
 }
 
 }  // namespace omni

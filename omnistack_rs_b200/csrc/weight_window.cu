@@ -1,8 +1,8 @@
 // Key weights of many columns (a prompt's last tokens): tcgen05 products in two passes over the keys.
 //
 // Query columns are the rows of the product (128 at a time), keys its columns:  S[col, key] = Q'[col, :] . K'[key, :].  Q' is made
-// once by a launch of its own (rotation, scaling, G . q, fp16 values and remainders) and lives in tensor memory for a span, K' is dequantised tile by tile (128 keys) into shared memory, twice: values and what they
-// leave of the centroids, plus the signs.  Two accumulators, since a key's norm multiplies the sign product alone and would have to
+// once by a launch of its own (rotation, scaling, G . q, fp16 values and remainders) and lives in tensor memory for a span, K' is
+// dequantised tile by tile (128 keys) into shared memory, twice: values and what they leave of the centroids, plus the signs.  Two accumulators, since a key's norm multiplies the sign product alone and would have to
 // be split as well to ride in it:   A = Qhi Khi + Qhi Klo (+ Qlo Khi),   B = Chi sign + Clo sign,   s = f_A A + f_B norm B.
 //
 // The tiles of all (user, head) lie in one row, cut into equal shares, one per CTA: lengths differ, and only the device knows
@@ -14,10 +14,10 @@
 //
 // Warps 0-7: scores, two threads per column with 64 of a tile's keys each.  Warps 8-15: dequantisation, two threads per key, up to
 // two buffers ahead of the products; with a span's first tile they bring its columns (the score warps doing so between two spans had the
-// products wait: 210 us instead of 190 for 16 users x 8 heads x up to 8,192 keys x 128 columns).  Warp 16 issues the products.  (One thread per column and key left each scheduler two warps,
-// which issued an instruction every third cycle: 135 us for a pass of 16 users x 8,192 keys x 128 columns.)  Shared memory bounds
+// products wait: 210 us instead of 190 for 16 users x 8 heads x up to 8,192 keys x 128 columns).  Warp 16 issues the
+// products.  (One thread per column and key left each scheduler two warps, which issued an instruction every third cycle: 135 us for a pass of 16 users x 8,192 keys x 128 columns.)  Shared memory bounds
 // a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the products' reads of K', about 1,900 cycles against 1,536
-// of the tensor pipe; measured, a tile takes 3,200 and the call 171 us, 18.7 of which its products would need alone.
+// of the tensor pipe; measured, a tile takes 2,400 in pass 1 and 3,200 in pass 2, and the call 156 us, 18.7 of which its products would need alone.
 #include "weight_sums.cuh"
 
 namespace omni {
@@ -247,8 +247,11 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
         for (int i = 0; i < 2; ++i) {
             ww_bar_init(bar_full + 8 * i, 8);
             ww_bar_init(bar_empty + 8 * i, 1);
-            ww_bar_init(bar_s + 8 * i, 1);                               // scores of keys 0-63 and 64-127 of a tile: by halves, so that the
-            ww_bar_init(bar_free + 8 * i, 4);                            // products of one go on while the other's are taken out
+            // The products of one part of a tile go on while the other's are taken out.  Pass 1: values, then signs, of all keys (128 keys per
+            // instruction; 64 take longer by a third: 171 us for the call instead of 156).  Pass 2: both, of keys 0-63 and then of 64-127, since its
+            // four columns' factors leave no registers to keep a tile's values until the signs are there.
+            ww_bar_init(bar_s + 8 * i, 1);
+            ww_bar_init(bar_free + 8 * i, PASS == 1 ? 8 : 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -280,8 +283,42 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             }
             const uint32_t kv = base + (t & 1) * kWwBuf;
             ok = ww_bar_wait(bar_full + 8 * (t & 1), (t >> 1) & 1);
+            if constexpr (PASS == 1) {                                   // all keys, values and then signs
+                if (ok && t > 0) ok = ww_bar_wait(bar_free, (t - 1) & 1);
+                if (!ok) break;
+                ww_fence_after();
+                const bool one = ww_elect();
+                if (one) {
+                    // the remainders' products first: added to an accumulator that already holds the values', each would cost it a rounding
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tq + 8 * ks, kv + kWwBytesV + ks * 2 * kWwLbo, kWwSbo, kWwTile, ks > 0);
+                    if (QLO) {
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tq + Set::kQlo + 8 * ks, kv + ks * 2 * kWwLbo, kWwSbo, kWwTile, 1);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) ww_mma(tmem + kWwColA, tq + 8 * ks, kv + ks * 2 * kWwLbo, kWwSbo, kWwTile, 1);
+                    if (!a.with_qjl) ww_commit(bar_empty + 8 * (t & 1));
+                    ww_commit(bar_s);
+                }
+                __syncwarp();
+                if (!a.with_qjl) continue;
+                if (t > 0) ok = ww_bar_wait(bar_free + 8, (t - 1) & 1);
+                if (!ok) break;
+                ww_fence_after();
+                if (one) {
+                    const uint32_t sx = kv + 2 * kWwBytesV;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) ww_mma(tmem + kWwColB, tq + Set::kClo + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, kWwTile, ks > 0);
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) ww_mma(tmem + kWwColB, tq + Set::kChi + 8 * ks, sx + ks * 2 * kWwLbo, kWwSboSign, kWwTile, 1);
+                    ww_commit(bar_empty + 8 * (t & 1));
+                    ww_commit(bar_s + 8);
+                }
+                __syncwarp();
+            }
 #pragma unroll 1
-            for (int x = 0; ok && x < 2; ++x) {
+            for (int x = PASS == 1 ? 2 : 0; ok && x < 2; ++x) {
                 if (t > 0) ok = ww_bar_wait(bar_free + 8 * x, (t - 1) & 1);
                 if (!ok) break;
                 ww_fence_after();
@@ -457,7 +494,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             }
             for (int t = done; t < done + n_span; ++t) {
                 // after a wait that ran out the warp still goes through the barriers it shares with the others, storing nothing
-                if (ok) ok = ww_bar_wait(bar_s + 8 * half, t & 1);
+                if (ok) ok = ww_bar_wait(bar_s + (PASS == 1 ? 0 : 8 * half), t & 1);
                 ww_fence_after();
                 const int k0 = (at.tile + t - done) * kWwTile;
                 const bool masked = k0 + kWwTile - 1 > open_to || k0 + kWwTile > len || cols - col0 < kWwTile;
@@ -534,7 +571,13 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                 uint32_t s[64];                                          // products of the values, then the scores / f
                 ww_ld32(t_lane + kWwColA + 64 * half, s);
                 ww_ld32(t_lane + kWwColA + 64 * half + 32, s + 32);
+                ww_wait_ld();
+                ww_fence_before();
+                __syncwarp();
+                if (lane == 0) ww_bar_arrive(bar_free);                  // the accumulator may be overwritten
                 if (a.with_qjl) {
+                    if (ok) ok = ww_bar_wait(bar_s + 8, t & 1);
+                    ww_fence_after();
                     const float* nrm = norm_s + (t & 3) * kWwTile + 64 * half;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -544,7 +587,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                         if (j == 1) {
                             ww_fence_before();
                             __syncwarp();
-                            if (lane == 0) ww_bar_arrive(bar_free + 8 * half);   // the accumulators may be overwritten
+                            if (lane == 0) ww_bar_arrive(bar_free + 8);
                         }
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
@@ -560,11 +603,6 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                             }
                         }
                     }
-                } else {
-                    ww_wait_ld();
-                    ww_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ww_bar_arrive(bar_free + 8 * half);
                 }
                 if (masked) {
                     const int lim = (last < len - 1 ? last : len - 1) - k0 - 64 * half;

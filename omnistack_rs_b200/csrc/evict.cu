@@ -7,6 +7,10 @@
 //
 // Gather.  A warp moves a group of eight kept rows.  Rows are moved, never recomputed, so the new cache holds the same bits;
 // V's pair layout mixes the nibbles of two keys per row, which the lanes take apart for the old pairs and join for the new.
+//
+// 64 users x 8 heads, up to 8,192 keys to 1,024: 65 us, selection 18 (shared-memory atomics and three passes over the keys) and gather 42
+// (5.2 TB/s of sectors: kept rows lie apart, and a sector of signs or norms holds neighbours that go).  The selecting CTA moving its rows
+// itself saves a launch and takes 76 us, too few warps to cover the rows' way.
 #include "common.cuh"
 
 namespace omni {

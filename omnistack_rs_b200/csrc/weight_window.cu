@@ -2,8 +2,9 @@
 //
 // Query columns are the rows of the product (128 at a time), keys its columns:  S[col, key] = Q'[col, :] . K'[key, :].  Q' is made
 // once by a launch of its own (rotation, scaling, G . q, fp16 values and remainders) and lives in tensor memory for a span, K' is
-// dequantised tile by tile (128 keys) into shared memory, twice: values and what they leave of the centroids, plus the signs.  Two accumulators, since a key's norm multiplies the sign product alone and would have to
-// be split as well to ride in it:   A = Qhi Khi + Qhi Klo (+ Qlo Khi),   B = Chi sign + Clo sign,   s = f_A A + f_B norm B.
+// dequantised tile by tile (128 keys) into shared memory, twice: values and what they leave of the centroids, plus the signs.  Two
+// accumulators, since a key's norm multiplies the sign product alone and would have to be split as well to ride in it:
+//   A = Qhi Khi + Qhi Klo (+ Qlo Khi),   B = Chi sign + Clo sign,   s = f_A A + f_B norm B.
 //
 // The tiles of all (user, head) lie in one row, cut into equal shares, one per CTA: lengths differ, and only the device knows
 // them.  A run of tiles of one head inside a share is a span; span (head, CTA) is number head + CTA, which no other span has.
@@ -12,12 +13,14 @@
 // the columns.  There a thread reads four columns of 16 keys (the 16-row form of the tensor-memory load), so that most of the sum is its
 // own: eight lanes trade halves, then the four warps' parts in order (one column of 64 keys per thread: 62 instead of 14 exchanges).
 //
-// Warps 0-7: scores, two threads per column with 64 of a tile's keys each.  Warps 8-15: dequantisation, two threads per key, up to
-// two buffers ahead of the products; with a span's first tile they bring its columns (the score warps doing so between two spans had the
-// products wait: 210 us instead of 190 for 16 users x 8 heads x up to 8,192 keys x 128 columns).  Warp 16 issues the
-// products.  (One thread per column and key left each scheduler two warps, which issued an instruction every third cycle: 135 us for a pass of 16 users x 8,192 keys x 128 columns.)  Shared memory bounds
-// a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the products' reads of K', about 1,900 cycles against 1,536
-// of the tensor pipe; measured, a tile takes 2,400 in pass 1 and 3,200 in pass 2, and the call 156 us, 18.7 of which its products would need alone.
+// Warps 0-7: scores, two threads per column with 64 of a tile's keys each.  (One thread per column and key left each scheduler two
+// warps, which issued an instruction every third cycle: 135 us for a pass of 16 users x 8,192 keys x 128 columns.)  Warps 8-15:
+// dequantisation, two threads per key, up to two buffers ahead of the products; with a span's first tile they bring its columns (the
+// score warps doing so between two spans had the products wait: 210 us instead of 190 for 16 users x 8 heads x up to 8,192 keys x 128
+// columns).  Warp 16 issues the products.
+// Shared memory bounds a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the products' reads of K', about 1,900 cycles
+// against 1,536 of the tensor pipe.  Measured, a tile takes 2,400 cycles in pass 1 and 3,200 in pass 2, and the call 156 us, 18.7 of which
+// its products would need alone.
 #include "weight_sums.cuh"
 
 namespace omni {

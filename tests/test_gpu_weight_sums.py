@@ -131,3 +131,30 @@ def test_graph_replay():
     lens.copy_(torch.tensor([1, 700, 0, 64], dtype=torch.int32))
     graph.replay()
     assert torch.equal(out, attn_weight_sums(*dev, seq_lens=lens))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,per_head", [(1, True), (12, False), (70, True)])
+def test_many_short_caches_per_cta(dtype, T, per_head):
+    """More tiles than CTAs, so that a CTA walks over several heads and users, some of them empty, and changes columns and centroid
+    tables on its way; 140 columns take two rounds."""
+    from omnistack_rs_b200.kernels.eviction import attn_weight_sums
+    B, H, S = 44, 4, 300
+    nib, qjl, norms, cb = packed(B, H, S, seed=31)
+    if not per_head:
+        cb = cb[0]
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(0, S + 1, (B,), generator=g).tolist()
+    lens[:9] = [300, 0, 1, 128, 0, 0, 129, 256, 2]
+    q = torch.randn(B, 2 * H, T, 128, generator=g).to(dtype)
+    ids = torch.arange(B, dtype=torch.int32) * 37
+    dev = [x.to(DEV) for x in (q, nib, qjl, norms, cb)]
+    seq = torch.tensor(lens, device=DEV)
+    for with_qjl in (True, False):
+        got = attn_weight_sums(*dev, user_id=ids.to(DEV), with_qjl=with_qjl, seq_lens=seq)
+        check(got, q, (nib, qjl, norms), cb if per_head else cb.expand(H, 16), ids, lens, with_qjl, True)
+        assert torch.equal(got, attn_weight_sums(*dev, user_id=ids.to(DEV), with_qjl=with_qjl, seq_lens=seq))
+        if T < 70:                                                               # one round: a single addition
+            into = torch.full((B, H, S), 3.0, device=DEV)
+            attn_weight_sums(*dev, user_id=ids.to(DEV), with_qjl=with_qjl, seq_lens=seq, into=into)
+            assert torch.equal(into, 3 + got)

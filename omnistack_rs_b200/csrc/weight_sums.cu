@@ -289,8 +289,9 @@ __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_
     const int tid = threadIdx.x;
     const int64_t bh = blockIdx.x / segments, s0 = blockIdx.x % segments * (kWfKeys * kWfThreads);
     const int64_t b = bh / a.Hkv, h = bh % a.Hkv;
-    const int len = ws_len(a, b), cols = a.Hq / a.Hkv * a.T;
+    const int cols = a.Hq / a.Hkv * a.T;
     after_predecessor();
+    const int len = ws_len(a, b);
     float2 v[kWfKeys][kWsStepCols / 2];                                  // the scores, requested before the normalisers are known
 #pragma unroll
     for (int k = 0; k < kWfKeys; ++k) {

@@ -18,16 +18,19 @@ struct WeightArgs {
     const uint32_t* g_rows;
     float2* partial;                               // per span and column (and warp): maximum (base 2) and sum
     float* scores;                                 // warp-level kernel: [B * Hkv][S][columns, rounded up to even]
-    int32_t* tiles_before;                         // [B + 1] tiles of one kv head in front of every user
+    int32_t* tiles_before;                         // [B + 1] tiles of one kv head in front of every user, then the [B] lengths they belong to
     void* prepared;                                // the columns, ready for registers or tensor memory
     float* sums;
 };
 
-__device__ __forceinline__ int ws_len(const WeightArgs& a, int64_t b) {
+__device__ __forceinline__ int ws_len_given(const WeightArgs& a, int64_t b) {
     if (!a.seq_lens) return (int)a.S;
     const int64_t n = __ldg(a.seq_lens + b);
     return (int)(n < 0 ? 0 : (n > a.S ? a.S : n));
 }
+// The length as the call's first launch read it: every later one walks over the same tiles, whatever is written to seq_lens meanwhile
+// (a share that ends elsewhere than its tiles would walk on past the last user).  Behind that launch only.
+__device__ __forceinline__ int ws_len(const WeightArgs& a, int64_t b) { return a.tiles_before[a.B + 1 + b]; }
 __device__ __forceinline__ float ws_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -180,7 +183,8 @@ __device__ __forceinline__ void ws_tiles_before(const WeightArgs& a, int tid) {
     int before = 0;
     for (int64_t b0 = 0; b0 <= a.B; b0 += WARPS * 32) {
         const int64_t b = b0 + tid;
-        const int n = b < a.B ? (ws_len(a, b) + kWsTile - 1) / kWsTile : 0;
+        const int len = b < a.B ? ws_len_given(a, b) : 0, n = (len + kWsTile - 1) / kWsTile;
+        if (b < a.B) a.tiles_before[a.B + 1 + b] = len;
         int upto = n;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -216,7 +220,7 @@ __device__ __forceinline__ int ws_user_of(const WeightArgs& a, int64_t x, int64_
 __device__ __forceinline__ int64_t ws_sharers(int64_t ctas, int64_t all) { return ctas < all ? ctas : all; }
 // The CTA of `ctas` launched ones whose share of `all` tiles holds tile x.
 __device__ __forceinline__ int64_t ws_cta_of(int64_t x, int64_t ctas, int64_t all) { return ((x + 1) * ws_sharers(ctas, all) + all - 1) / all - 1; }
-__host__ __device__ __forceinline__ size_t ws_before_bytes(int64_t B) { return ((size_t)(B + 1) * 4 + 15) & ~(size_t)15; }
+__host__ __device__ __forceinline__ size_t ws_before_bytes(int64_t B) { return ((size_t)(2 * B + 1) * 4 + 15) & ~(size_t)15; }
 
 // tcgen05 kernel for more columns (weight_window.cu)
 int32_t launch_weight_window(WeightArgs a, int q_dtype, int32_t* status, cudaStream_t st);

@@ -434,6 +434,11 @@ typedef struct omni_evict_t {
 } omni_evict_t;
 int32_t omni_evict_keys(const omni_evict_t* call, void* stream);
 
+/* Sums of keys that an append is about to write: sums[b,h,lens[b]] .. sums[b,h,lens[b] + T - 1] become zero (fp32 [B][H][S], device
+ * int64 lens; positions outside [0, S) are left out).  Cleared when the keys come, not when they go: whoever sets lens back
+ * leaves no trace of it but the lengths. */
+int32_t omni_clear_new_sums(float* sums, const int64_t* lens, int64_t B, int32_t H, int64_t S, int64_t T, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

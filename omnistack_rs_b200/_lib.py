@@ -65,6 +65,7 @@ SIGNATURES = {
     "omni_attn_weight_sums_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64]),
     "omni_attn_weight_sums": (_i32, [_vp, _vp]),
     "omni_evict_keys": (_i32, [_vp, _vp]),
+    "omni_clear_new_sums": (_i32, [_vp, _vp, _i64, _i32, _i64, _i64, _vp]),
 }
 
 _lock = threading.Lock()

@@ -247,6 +247,14 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
     }
 }
 
+// sums of the T keys per (user, head) that come next
+__global__ void clear_new_sums_kernel(float* sums, const int64_t* lens, int64_t n, int H, int64_t S, int64_t T) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t bh = i / T, s = __ldg(lens + bh / H) + i % T;
+        if (s >= 0 && s < S) sums[bh * S + s] = 0.f;
+    }
+}
+
 }  // namespace omni
 
 using namespace omni;
@@ -274,4 +282,13 @@ extern "C" int32_t omni_evict_keys(const omni_evict_t* call, void* stream) {
     OMNI_CUDA(cudaGetLastError());
     return check_cuda(launch_early(evict_gather_kernel, dim3((unsigned)((n_groups + kGatherWarps - 1) / kGatherWarps)), kGatherWarps * 32, 0, st, a, groups_per_head, n_groups),
                       "evict_gather_kernel launch");
+}
+
+extern "C" int32_t omni_clear_new_sums(float* sums, const int64_t* lens, int64_t B, int32_t H, int64_t S, int64_t T, void* stream) {
+    OMNI_REQUIRE(B >= 0 && H >= 0 && S >= 0 && T >= 0, OMNI_ERR_ARG, "omni_clear_new_sums: negative extent");
+    if (B == 0 || H == 0 || S == 0 || T == 0) return OMNI_OK;
+    OMNI_REQUIRE(sums && lens, OMNI_ERR_ARG, "omni_clear_new_sums: NULL buffer");
+    const int64_t n = B * H * T, blocks = (n + 255) / 256;
+    clear_new_sums_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, (cudaStream_t)stream>>>(sums, lens, n, H, S, T);
+    return check_cuda(cudaGetLastError(), "clear_new_sums_kernel launch");
 }

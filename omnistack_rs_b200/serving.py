@@ -157,6 +157,7 @@ class QuantizedKVCache:
             return
         if int(self.lens.max()) + T > self.max_len:
             raise ValueError("append would run past the cache capacity")
+        self._forget_sums(T)
         rotate_quantize_append(k_new, self.k_nib, self.k_qjl, self.k_norms, self.lens, self.codebooks,
                                self.user_ids, rotate=rotate)
         rotate_quantize_append(v_new, self.v_nib, self.v_qjl, self.v_norms, self.lens, self.codebooks,
@@ -190,6 +191,7 @@ class QuantizedKVCache:
         lo, hi = _lib.index_range(self.lens)
         if hi + T > self.max_len or lo < 0:
             raise ValueError("append would run past the cache capacity")
+        self._forget_sums(T)
         lib = _lib.ensure_init(dev)
         k_new, v_new = _codec_rows(k_new), _codec_rows(v_new)
         cb, per_head = _prep_codebooks(self.codebooks, H, dev)
@@ -202,6 +204,17 @@ class QuantizedKVCache:
                 _lib.ptr(self.k_nib), _lib.ptr(self.k_qjl), _lib.ptr(self.k_norms), _lib.ptr(self.v_nib), _lib.ptr(self.v_qjl),
                 _lib.ptr(self.v_norms), S, _lib.ptr(self.lens), _lib.ptr(self.lens32), int(self.pair_v), _lib.stream_ptr(dev)))
         return True
+
+    def _forget_sums(self, T: int) -> None:
+        """No weight has reached the T keys that every user is about to get, whatever stood in their rows before: ``lens`` may
+        have been set back, for another continuation or another prompt."""
+        if self.weight_sums is None or T == 0 or self.n_users == 0:
+            return
+        dev = self.weight_sums.device
+        lens = _lib.as_device(self.lens, dev, torch.int64)
+        with _lib.on_device(dev):
+            _lib.check(_lib.load().omni_clear_new_sums(_lib.ptr(self.weight_sums), _lib.ptr(lens), self.n_users, self.n_kv_heads, self.max_len, T,
+                                                       _lib.stream_ptr(dev)))
 
     def _capturing(self) -> bool:
         return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
@@ -235,9 +248,9 @@ class QuantizedKVCache:
     def observe(self, q: torch.Tensor, scale: Optional[float] = None, with_qjl: bool = True, rotate_q: bool = False,
                 causal: bool = True) -> torch.Tensor:
         """Add the attention weight that every cached key receives from ``q`` (n_users, n_heads, T, 128), the queries of the last T
-        tokens, to ``weight_sums`` (float32 (n_users, n_kv_heads, max_len), kept from the first call on), which decides what
-        :meth:`evict` keeps.  Arguments as in :meth:`attend`; returns ``weight_sums``.  A CUDA graph may hold every call but the
-        first."""
+        tokens, to ``weight_sums`` (float32 (n_users, n_kv_heads, max_len), kept from the first call on; new keys begin with
+        zero), which decides what :meth:`evict` keeps.  Arguments as in :meth:`attend`; returns ``weight_sums``.  A CUDA graph may
+        hold every call but the first."""
         if self.weight_sums is None:
             if self._capturing():                  # the zeros would be part of the graph, and every replay would start from them
                 raise RuntimeError("the first observe makes weight_sums: call it once before the capture")

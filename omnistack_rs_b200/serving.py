@@ -223,21 +223,23 @@ class QuantizedKVCache:
                 causal: bool = True, scale: Optional[float] = None, rotate: bool = True) -> torch.Tensor:
         """Take in every user's prompt: ``prompt_attn`` of ``q`` (n_users, n_heads, T, 128) over ``k`` and ``v`` (n_users,
         n_kv_heads, T, 128) in full precision, and the keys and values packed into the (empty) cache.  ``prompt_lens`` (n_users,):
-        user b's prompt is its first ``prompt_lens[b]`` rows; the others are neither attended to nor kept.  Returns the
-        attention's result, zeros in the rows behind a prompt."""
-        T = k.shape[2]
+        user b's prompt is its first ``prompt_lens[b]`` rows; the others are neither attended to nor kept (the longest prompt has to
+        fit the cache, its padding need not).  Returns the attention's result, zeros in the rows behind a prompt."""
+        T = longest = k.shape[2]
         lens = None
         if prompt_lens is not None:
             if prompt_lens.shape != (self.n_users,):
                 raise ValueError(f"prompt_lens must have shape ({self.n_users},), got {tuple(prompt_lens.shape)}")
             lens = prompt_lens.to(device=self.device, dtype=torch.int64)
-            lo, hi = _lib.index_range(lens) if self.n_users else (0, 0)
-            if lo < 0 or hi > T:
+            lo, longest = _lib.index_range(lens) if self.n_users else (0, 0)
+            if lo < 0 or longest > T:
                 raise ValueError(f"prompt_lens must lie in [0, {T}]")
+        if longest > self.max_len:
+            raise ValueError("prefill would run past the cache capacity")
         if self.n_users and _lib.index_range(self.lens) != (0, 0):
             raise ValueError("prefill takes whole prompts: the cache already holds keys")
         out = prompt_attn(q, k, v, seq_lens=lens, causal=causal, scale=scale)
-        self.append(k, v, rotate=rotate)
+        self.append(k[:, :, :longest], v[:, :, :longest], rotate=rotate)           # rows behind the longest prompt are nobody's
         if lens is not None:
             if self.pair_v:                        # groups that are not complete below the prompt's length go back to single rows
                 pair_v_rows(self.v_nib, lens, self.lens)

@@ -87,3 +87,28 @@ def test_clearing_stays_inside_the_rows():
     assert torch.equal(guard.cpu(), want)
     assert lib.omni_clear_new_sums(None, lens.data_ptr(), B, H, S, T, None) == _lib.ERR_ARG
     assert lib.omni_clear_new_sums(None, None, B, -1, S, T, None) == _lib.ERR_ARG and lib.omni_clear_new_sums(None, None, B, H, S, 0, None) == _lib.OK
+
+
+@pytest.mark.parametrize("pair_v", [False, True])
+def test_prompts_that_fit_although_their_padding_does_not(pair_v):
+    """What counts is the longest prompt, not the padded length; what does not fit is refused before anything is done."""
+    x = [rows(h, MAX + 40, h, torch.float16) for h in (HQ, H, H)]
+    lens = torch.tensor([MAX, 13, 0])
+    cache, narrow = make_cache(pair_v), make_cache(pair_v)
+    out = cache.prefill(*x, lens)
+    want = narrow.prefill(*[t[:, :, :MAX] for t in x], lens)
+    assert out.shape == x[0].shape and torch.equal(out[:, :, :MAX], want) and bool((out[:, :, MAX:] == 0).all())
+    assert cache.lens.tolist() == lens.tolist() == cache.lens32.tolist()
+    for b, n in enumerate(lens.tolist()):
+        for name in ("k_nib", "k_qjl", "k_norms", "v_nib", "v_qjl", "v_norms"):
+            assert torch.equal(getattr(cache, name)[b, :, :n], getattr(narrow, name)[b, :, :n]), name
+    q = rows(HQ, 1, 9)
+    assert torch.equal(cache.attend(q), narrow.attend(q))
+    over = make_cache(pair_v)
+    with pytest.raises(ValueError, match="capacity"):
+        over.prefill(*x, torch.tensor([1, MAX + 1, 0]))
+    with pytest.raises(ValueError, match="capacity"):
+        over.prefill(*x)
+    assert over.lens.tolist() == [0, 0, 0] and bool((over.k_nib == 0).all())
+    none = over.prefill(*x, torch.zeros(N, dtype=torch.int64))            # prompts without a token
+    assert bool((none == 0).all()) and over.lens.tolist() == [0, 0, 0]

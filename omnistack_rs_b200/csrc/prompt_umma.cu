@@ -19,8 +19,8 @@
 // measured burst rate of a plain matrix product and 87 % of its sustained one.  A quarter of the exponentials as a polynomial on the
 // FP32 units (1.84 ms) or a third (1.90 ms) gained nothing.
 //
-// A zero weight times an infinite or NaN value of a masked key would be NaN.  Rows that come out NaN are therefore formed
-// again from global memory over their own keys alone (prompt_row_again), which settles NaN that belong there too.
+// A zero weight times an infinite or NaN value of a masked key is NaN.  Rows that come out NaN although no score of theirs is, in dims
+// that the values they see do not account for (prompt_unexplained), are formed again from global memory over their own keys alone.
 #include "prompt.cuh"
 #include <cuda.h>
 #include <mutex>
@@ -162,35 +162,213 @@ template <int DT> __device__ __forceinline__ uint32_t pu_pack(float lo, float hi
     return r;
 }
 
-// One output row over its own keys alone, by a warp (lane l has dims 4l .. 4l + 3), fp32 throughout.
+// D += A B of one warp: 16 rows x 16 x 8 columns
 template <int DT>
-__device__ __forceinline__ void prompt_row_again(const PromptArgs& a, int64_t b, int64_t row0, int t, int newest, int head, int lane) {
-    const int hkv = head / (a.Hq / a.Hkv);
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-    Elem<DT>::load4(a.q, b * a.qs[0] + (int64_t)head * a.qs[1] + (row0 + t) * a.qs[2] + 4 * lane, q);
-    const int64_t kb = b * a.ks[0] + (int64_t)hkv * a.ks[1] + row0 * a.ks[2] + 4 * lane;
-    const int64_t vb = b * a.vs[0] + (int64_t)hkv * a.vs[1] + row0 * a.vs[2] + 4 * lane;
-    const float c = a.scale * kPuLog2e;
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j <= newest; ++j) {
-        float k[4], v[4];
-        Elem<DT>::load4(a.k, kb + (int64_t)j * a.ks[2], k);
-        Elem<DT>::load4(a.v, vb + (int64_t)j * a.vs[2], v);
-        float s = fmaf(q[0], k[0], fmaf(q[1], k[1], fmaf(q[2], k[2], q[3] * k[3])));
+__device__ __forceinline__ void pu_warp_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (DT == OMNI_BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int DT> __device__ __forceinline__ float2 pu_unpack(uint32_t w) {
+    if constexpr (DT == OMNI_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Output rows of one kv head over their own keys alone, by a warp.  Lane l brings a row: token t of query head `head`, keys 0 .. lim, wanted
+// where bit l of `again` is set.  Sixteen rows at a time: lane (g, c) = (lane / 4, lane % 4) holds dims 32 c .. 32 c + 31 of rows g and g + 8.
+// Keys that all wanted rows see go through warp-level products, sixteen at a time, with the weights rounded to the type as everywhere; the
+// others, fewer than 16 + 127, one by one, skipped where they are masked.
+// 4,096 tokens of 8 heads, 64 us: 385 us with a NaN value at token 2,000 in a tile of earlier rows (21 ms with a row and a key at a time).
+template <int DT>
+__device__ __forceinline__ void prompt_rows_again(const PromptArgs& a, int64_t b, int64_t row0, int hkv, int t, int lim, int head, uint32_t again, int lane) {
+    constexpr float kBias = DT == OMNI_F16 ? 14.f : 0.f;                 // fp16 weights end at 2^-24
+    constexpr float kLeast = DT == OMNI_F16 ? 5.9604644775390625e-8f : 1.17549435e-38f;        // a visible infinity times a weight is not NaN
+    using E = typename Elem<DT>::T;
+    const int g = lane >> 2, c = lane & 3;
+    const E* kp = reinterpret_cast<const E*>(a.k) + b * a.ks[0] + (int64_t)hkv * a.ks[1] + row0 * a.ks[2];
+    const E* vp = reinterpret_cast<const E*>(a.v) + b * a.vs[0] + (int64_t)hkv * a.vs[1] + row0 * a.vs[2];
+    const float scale = a.scale * kPuLog2e;
+    auto load8w = [](const E* p, uint32_t* w) {                          // eight elements
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    };
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 16) {
+        const uint32_t wanted = (again >> r0) & 0xffffu;
+        if (!wanted) continue;
+        const bool mine = (lane & 16) == r0 && ((again >> lane) & 1);
+        const int n_common = __reduce_min_sync(kFullMask, mine ? lim : 0x7ffffffe) + 1, last = __reduce_max_sync(kFullMask, mine ? lim : -1);
+        bool on[2];
+        int64_t out_at[2];
+        int lims[2];
+        uint32_t q[2][16];
 #pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(kFullMask, s, x);
-        s *= c;
-        const float m_new = fmaxf(m, s);
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = exp2f(m - ref), p = exp2f(s - ref);
-        m = m_new;
-        l = fmaf(l, alpha, p);
+        for (int r = 0; r < 2; ++r) {
+            const int from = r0 + g + 8 * r;
+            const int tr = __shfl_sync(kFullMask, t, from), hr = __shfl_sync(kFullMask, head, from);
+            lims[r] = __shfl_sync(kFullMask, lim, from);
+            on[r] = (again >> from) & 1;
+            out_at[r] = ((b * a.Hq + hr) * a.T + row0 + tr) * kHeadDim + 32 * c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = fmaf(o[i], alpha, p * v[i]);
+            for (int i = 0; i < 16; ++i) q[r][i] = 0u;
+            if (on[r]) {
+                const E* qp = reinterpret_cast<const E*>(a.q) + b * a.qs[0] + (int64_t)hr * a.qs[1] + (row0 + tr) * a.qs[2] + 32 * c;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) load8w(qp + 8 * i, q[r] + 4 * i);
+            }
+        }
+        float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};        // o[i]: dims 32 c + i and 32 c + 16 + i of row g, then of row g + 8
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        auto raise = [&](int r, float top) {                             // the row's new reference
+            const float m_new = fmaxf(m[r], top), alpha = exp2f(m[r] - (m_new == -INFINITY ? 0.f : m_new));
+            m[r] = m_new;
+            l[r] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { o[i][2 * r] *= alpha; o[i][2 * r + 1] *= alpha; }
+        };
+        int j0 = 0;
+#pragma unroll 1
+        for (; j0 + 16 <= n_common; j0 += 16) {
+            uint32_t k[2][16], v[4][8];                                  // keys g and g + 8, this lane's dims; keys 2c, 2c + 1, 2c + 8, 2c + 9, dims 16 g ..
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) load8w(kp + (int64_t)(j0 + g + 8 * i) * a.ks[2] + 32 * c + 8 * x, k[i] + 4 * x);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) load8w(vp + (int64_t)(j0 + 2 * c + (i & 1) + 8 * (i >> 1)) * a.vs[2] + 16 * g + 8 * x, v[i] + 4 * x);
+            }
+            float s[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) pu_warp_mma<DT>(s[i], q[0][2 * ks], q[1][2 * ks], q[0][2 * ks + 1], q[1][2 * ks + 1], k[i][2 * ks], k[i][2 * ks + 1]);
+            }
+            uint32_t p[2][2];                                            // [row][keys 2c and 2c + 1, then 2c + 8 and 2c + 9]
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float x[4] = {s[0][2 * r] * scale, s[0][2 * r + 1] * scale, s[1][2 * r] * scale, s[1][2 * r + 1] * scale};
+                float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+                if (__any_sync(kFullMask, top > m[r])) raise(r, top);
+                const float ref = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool seen = x[i] > -INFINITY;
+                    x[i] = exp2f(x[i] - ref + kBias);
+                    l[r] += x[i];
+                    if (seen) x[i] = fmaxf(x[i], kLeast);
+                }
+                p[r][0] = pu_pack<DT>(x[0], x[1]);
+                p[r][1] = pu_pack<DT>(x[2], x[3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t half = (i & 1) ? 0x7632u : 0x5410u;
+                pu_warp_mma<DT>(o[i], p[0][0], p[1][0], p[0][1], p[1][1], __byte_perm(v[0][i >> 1], v[1][i >> 1], half), __byte_perm(v[2][i >> 1], v[3][i >> 1], half));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(kFullMask, l[r], 1);
+            l[r] += __shfl_xor_sync(kFullMask, l[r], 2);
+        }
+#pragma unroll 1
+        for (; j0 <= last; ++j0) {
+            uint32_t k[16], v[16];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                load8w(kp + (int64_t)j0 * a.ks[2] + 32 * c + 8 * x, k + 4 * x);
+                load8w(vp + (int64_t)j0 * a.vs[2] + 32 * c + 8 * x, v + 4 * x);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 x = pu_unpack<DT>(q[r][i]), y = pu_unpack<DT>(k[i]);
+                    s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+                }
+                s += __shfl_xor_sync(kFullMask, s, 1);
+                s += __shfl_xor_sync(kFullMask, s, 2);
+                s = j0 <= lims[r] ? s * scale : -INFINITY;
+                if (__any_sync(kFullMask, s > m[r])) raise(r, s);
+                const float e = exp2f(s - (m[r] == -INFINITY ? 0.f : m[r]) + kBias);
+                l[r] += e;
+                if (j0 <= lims[r]) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 y = pu_unpack<DT>(v[i]);            // dims 32 c + 2 i, + 1
+                        float& u = o[(2 * i) & 15][2 * r + (i >> 3)];
+                        float& w = o[(2 * i + 1) & 15][2 * r + (i >> 3)];
+                        u = fmaf(e, y.x, u);
+                        w = fmaf(e, y.y, w);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (!on[r]) continue;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                float y[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) y[x] = o[(i + x) & 15][2 * r + (i >> 4)] / l[r];
+                Elem<DT>::store4(a.out, out_at[r] + i, y);
+            }
+        }
     }
+}
+
+// Of the rows `again` (one per lane) whose sums over the values came out NaN in the dims `dims` (bit i of word w: dim 32 w + i), those that
+// the values 0 .. first, which all of them see, do not account for: a NaN there, or infinities of both signs, whatever the weights.
+template <int DT>
+__device__ __forceinline__ uint32_t prompt_unexplained(const PromptArgs& a, int64_t b, int64_t row0, int hkv, int first, uint32_t again,
+                                                       const uint32_t (&dims)[4], int lane) {
+    constexpr uint32_t kExp = DT == OMNI_BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = DT == OMNI_BF16 ? 0x00800080u : 0x04000400u;
+    using E = typename Elem<DT>::T;
+    const int half = lane >> 4, d = lane & 15;                           // dims 8 d .. 8 d + 7 of every other key
+    const E* vp = reinterpret_cast<const E*>(a.v) + b * a.vs[0] + (int64_t)hkv * a.vs[1] + row0 * a.vs[2] + 8 * d;
+    uint32_t is_nan = 0, up = 0, down = 0;                               // bit i: dim 8 d + i
+#pragma unroll 1
+    for (int j0 = 0; j0 <= first && again; j0 += 32) {
+        uint4 v[16];
+        uint32_t hit = 0;                                                // an exponent of ones carries into its sign's place
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] /= l;
-    Elem<DT>::store4(a.out, ((b * a.Hq + head) * a.T + row0 + t) * kHeadDim + 4 * lane, o);
+        for (int i = 0; i < 16; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(vp + (int64_t)(j0 + 2 * i + half < first ? j0 + 2 * i + half : first) * a.vs[2]));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) hit |= ((v[i].x & kExp) + kOne) | ((v[i].y & kExp) + kOne) | ((v[i].z & kExp) + kOne) | ((v[i].w & kExp) + kOne);
+        if (!__any_sync(kFullMask, (hit & 0x80008000u) != 0)) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const float2 y = pu_unpack<DT>(w[x]);
+                is_nan |= (y.x != y.x ? 1u << (2 * x) : 0u) | (y.y != y.y ? 2u << (2 * x) : 0u);
+                up |= (y.x == INFINITY ? 1u << (2 * x) : 0u) | (y.y == INFINITY ? 2u << (2 * x) : 0u);
+                down |= (y.x == -INFINITY ? 1u << (2 * x) : 0u) | (y.y == -INFINITY ? 2u << (2 * x) : 0u);
+            }
+        }
+        is_nan |= __shfl_xor_sync(kFullMask, is_nan, 16);                // the other keys
+        up |= __shfl_xor_sync(kFullMask, up, 16);
+        down |= __shfl_xor_sync(kFullMask, down, 16);
+        const uint32_t known = (is_nan | (up & down)) << (8 * (lane & 3));
+        uint32_t left = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) left |= dims[w] & ~__reduce_or_sync(kFullMask, d >> 2 == w ? known : 0u);
+        again &= __ballot_sync(kFullMask, left != 0);
+    }
+    return again;
 }
 
 // A work item: two tiles (32-bit: a prompt's rows and a call's slots are).
@@ -477,7 +655,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                     for (int k = 0; k < 4; ++k) mx[k] = pu_max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-                const bool raise = top > m + kSlack;
+                const bool raise = top > m + kSlack;                         // never while every score so far is -inf
                 if (__any_sync(kFullMask, raise)) {
                     const float m_new = raise ? top : m;
                     const float alpha = raise ? pu_ex2(m - m_new) : 1.f;
@@ -495,7 +673,8 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                         }
                     }
                 }
-                const uint64_t c2 = pu_pair(c, c), neg2 = pu_pair(kBias - m, kBias - m);
+                const float shift = kBias - (m == -INFINITY ? 0.f : m);      // scores of -inf then weigh zero
+                const uint64_t c2 = pu_pair(c, c), neg2 = pu_pair(shift, shift);
                 uint64_t sum[2] = {pu_pair(0.f, 0.f), pu_pair(0.f, 0.f)};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -543,13 +722,24 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                     pu_store32(dst + 4 * i + 2, r + 8);
                 }
             }
-            uint32_t again = __ballot_sync(kFullMask, live && bad);
-            while (again) {
-                const int src = __ffs(again) - 1;
-                again &= again - 1;
-                prompt_row_again<DT>(a, it.b, it.row0, __shfl_sync(kFullMask, t, src), __shfl_sync(kFullMask, lim, src),
-                                     it.head0 + __shfl_sync(kFullMask, g, src), lane);
+            // A sum l that is NaN comes from the row's own scores (masked ones are -inf before their use), one of zero from scores that are
+            // all -inf: such rows are NaN, and done.  What is left has NaN among its values, visible or masked.
+            uint32_t again = __ballot_sync(kFullMask, live && bad && l > 0.f);
+            if (again) {
+                uint32_t dims[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t o[32];
+                    pu_ld32(t_o + 32 * i, o);
+                    pu_wait_ld();
+                    dims[i] = 0;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) dims[i] |= __uint_as_float(o[k]) != __uint_as_float(o[k]) ? 1u << k : 0u;
+                }
+                const int first = __reduce_min_sync(kFullMask, (again >> lane) & 1 ? lim : 0x7fffffff);
+                again = prompt_unexplained<DT>(a, it.b, it.row0, it.hkv, first, again, dims, lane);
             }
+            if (again) prompt_rows_again<DT>(a, it.b, it.row0, it.hkv, t, lim, it.head0 + g, again, lane);
         }
     }
     if (!ok && a.status) atomicExch(a.status, OMNI_STATUS_WAIT_EXPIRED);

@@ -42,8 +42,8 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens
     the keys and values behind a query's own position (infinities and NaN included).
 
     Scores, softmax statistics and sums are float32.  For bfloat16 and float16 the tensor cores multiply the weights, rounded
-    to that type, with the values; float32 stays float32 throughout.  A row that shares a tile with infinities or NaN it must not
-    see is computed again without the tensor cores, its weights unrounded, and may differ by that rounding."""
+    to that type, with the values; float32 stays float32 throughout.  A row that shares a tile with values that are
+    infinite or NaN and that it must not see is formed again over its own keys, and may differ by the rounding of the weights."""
     q_shape, k_shape = q.shape, k.shape
     if len(q_shape) != 4 or len(k_shape) != 4 or v.dim() != 4:
         raise ValueError("q, k and v must be (B, n_heads, T, 128)")

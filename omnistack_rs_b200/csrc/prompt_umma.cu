@@ -44,6 +44,10 @@ constexpr uint32_t kPuSmem = kPuOffItem + kPuItems * 32 + 16 + 1024;   // items,
 constexpr uint32_t kPuColS = 0, kPuColO = 256, kPuTmemCols = 512;
 constexpr uint32_t kPuWaitLimit = 1u << 26;        // waits may last as long as a CTA's item does (rows formed again take milliseconds)
 constexpr float kPuLog2e = 1.4426950408889634f;
+// Past 2^22 a step of fp32 is half a power of two or more.  The roundings of the reference, of its bias and of the slack's comparison add up to a
+// whole power there, and an fp16 weight of 2^(8 + 7) would not hold twice that.  Rows that get there are formed again (prompt_rows_again
+// subtracts before it adds a bias); a second form of the loop below that does so costs every call 2 %.
+constexpr float kPuFar = 4194304.f;
 
 // ---- PTX wrappers --------------------------------------------------------------------------------
 __device__ __forceinline__ void pu_bar_init(uint32_t bar, uint32_t count) {
@@ -635,6 +639,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             const int lim = live ? (a.causal ? t : it.len - 1) : it.len - 1;
             const int n_free = a.causal ? it.t0 + x * tt + 1 : it.len;       // keys below this are open to every row of the tile
             float m = -INFINITY, l = 0.f;                                    // m: in units of c * score
+            bool far = false;                                                // m has been past kPuFar
             for (int j = 0; j < n_mine; ++j) {
                 ok = pu_bar_wait_warp(bar_s + 8 * x, done & 1);
                 if (!ok) break;
@@ -660,6 +665,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                     const float m_new = raise ? top : m;
                     const float alpha = raise ? pu_ex2(m - m_new) : 1.f;
                     m = m_new;
+                    far = far || (raise && fabsf(m) > kPuFar);
                     l *= alpha;
                     if (j > 0) {
 #pragma unroll 1
@@ -724,7 +730,8 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             }
             // A sum l that is NaN comes from the row's own scores (masked ones are -inf before their use), one of zero from scores that are
             // all -inf: such rows are NaN, and done.  What is left has NaN among its values, visible or masked.
-            uint32_t again = __ballot_sync(kFullMask, live && bad && l > 0.f);
+            far = far && live && m < INFINITY;                               // (an infinite score makes its row NaN)
+            uint32_t again = __ballot_sync(kFullMask, live && bad && !far && l > 0.f);
             if (again) {
                 uint32_t dims[4];
 #pragma unroll
@@ -739,6 +746,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
                 const int first = __reduce_min_sync(kFullMask, (again >> lane) & 1 ? lim : 0x7fffffff);
                 again = prompt_unexplained<DT>(a, it.b, it.row0, it.hkv, first, again, dims, lane);
             }
+            again |= __ballot_sync(kFullMask, far);
             if (again) prompt_rows_again<DT>(a, it.b, it.row0, it.hkv, t, lim, it.head0 + g, again, lane);
         }
     }

@@ -385,7 +385,7 @@ int32_t omni_qk_norm_rope(const omni_norm_rope_t* call, void* stream);
  *   out          contiguous [B][Hq][T][128] of `dtype`, on a 32-byte boundary
  * Values of masked keys never reach a row, whatever they hold (infinities and NaN included).  Scores, softmax statistics and
  * sums are fp32; for bf16 and fp16 the weights are rounded to that type for the second product.
- *   status_word  device int32 or NULL, as in omni_qattn_decode */
+ *   status_word  device int32 or NULL, as in omni_qattn_decode: a CTA that gave up leaves zeros in the rows of its work */
 typedef struct omni_prompt_t {
     const void* q; const void* k; const void* v; void* out;
     const int32_t* cu_seqlens; const int32_t* seq_lens; int32_t* status_word;

@@ -42,7 +42,9 @@ constexpr uint32_t kPuOffCu = kPuOffBar + 256;
 constexpr uint32_t kPuOffItem = kPuOffCu + kPuCu * 4;           // item: batch, first row, length, first token, kv head, first query head, valid
 constexpr uint32_t kPuSmem = kPuOffItem + kPuItems * 32 + 16 + 1024;   // items, a stolen CTA's handle, and room to start on a 1,024-byte boundary
 constexpr uint32_t kPuColS = 0, kPuColO = 256, kPuTmemCols = 512;
-constexpr uint32_t kPuWaitLimit = 1u << 26;        // waits may last as long as a CTA's item does (rows formed again take milliseconds)
+// A poll that fails lasts 4 us, so a wait runs out after 4 s (and one for the next item after 16 s: it outlasts the waits of the warp that
+// publishes it).  Waits last as long as a CTA's item does; rows formed again over a million keys take a tenth of a second.
+constexpr uint32_t kPuWaitLimit = 1u << 20, kPuItemWaitLimit = 1u << 22;
 constexpr float kPuLog2e = 1.4426950408889634f;
 // Past 2^22 a step of fp32 is half a power of two or more.  The roundings of the reference, of its bias and of the slack's comparison add up to a
 // whole power there, and an fp16 weight of 2^(8 + 7) would not hold twice that.  Rows that get there are formed again (prompt_rows_again
@@ -59,8 +61,8 @@ __device__ __forceinline__ void pu_bar_arrive(uint32_t bar) {
 __device__ __forceinline__ void pu_bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("{\n .reg .b64 t;\n mbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n}\n" :: "r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool pu_bar_wait(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kPuWaitLimit; ++i) {
+__device__ __forceinline__ bool pu_bar_wait(uint32_t bar, uint32_t parity, uint32_t limit = kPuWaitLimit) {
+    for (uint32_t i = 0; i < limit; ++i) {
         uint32_t ok;
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
@@ -69,7 +71,9 @@ __device__ __forceinline__ bool pu_bar_wait(uint32_t bar, uint32_t parity) {
     return false;
 }
 // by all lanes of a warp, with one answer
-__device__ __forceinline__ bool pu_bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(kFullMask, pu_bar_wait(bar, parity)); }
+__device__ __forceinline__ bool pu_bar_wait_warp(uint32_t bar, uint32_t parity, uint32_t limit = kPuWaitLimit) {
+    return __all_sync(kFullMask, pu_bar_wait(bar, parity, limit));
+}
 __device__ __forceinline__ void pu_tma_load(uint32_t dst, const CUtensorMap* map, int d, int t, int h, int b, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
                  :: "r"(dst), "l"(map), "r"(d), "r"(t), "r"(h), "r"(b), "r"(bar) : "memory");
@@ -375,6 +379,13 @@ __device__ __forceinline__ uint32_t prompt_unexplained(const PromptArgs& a, int6
     return again;
 }
 
+// Zeros in a row whose work is given up.
+template <int DT>
+__device__ __forceinline__ void prompt_leave_row(const PromptArgs& a, int64_t b, int64_t row, int head, int at, int step) {
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = at; i < kHeadDim / 4; i += step) Elem<DT>::store4(a.out, ((b * a.Hq + head) * a.T + row) * kHeadDim + 4 * i, zero);
+}
+
 // A work item: two tiles (32-bit: a prompt's rows and a call's slots are).
 struct PuItem {
     int b, row0, len, t0, hkv, head0, slot;
@@ -441,7 +452,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
     PuItem it;
     auto next_item = [&](int k) {
         const int at = k % kPuItems;
-        ok = pu_bar_wait_warp(bar_item + 8 * at, (k / kPuItems) & 1);
+        ok = pu_bar_wait_warp(bar_item + 8 * at, (k / kPuItems) & 1, kPuItemWaitLimit);
         if (!ok) return false;
         uint32_t v[7];
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(items + 32 * at) : "memory");
@@ -468,12 +479,20 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             for (int k = 0;; ++k) {
                 const int at = k % kPuItems;
                 if (k >= kPuItems) ok = pu_bar_wait_warp(bar_taken + 8 * at, (k / kPuItems - 1) & 1);
-                if (!ok) break;
                 const int64_t slot = (int64_t)gridDim.x - 1 - bx;        // a prompt's last tiles have the most keys: first
                 PromptTile w{};
                 if (valid) w = prompt_tile(near, slot, lane);
+                const uint32_t hkv = by / a.n_hg, head0 = hkv * (uint32_t)(a.Hq / a.Hkv) + by % a.n_hg * a.gp;
+                if (!ok) {                                               // an item that no other CTA will take up: zeros
+                    if (valid) {
+                        prompt_zero_rows<DT>(a, w, slot, (int)head0, lane, 32);
+                        for (int r = 0; r < a.tpt * a.gp; ++r)
+                            if (w.t0 + r % a.tpt < w.len)
+                                prompt_leave_row<DT>(a, w.b, w.row0 + w.t0 + r % a.tpt, (int)head0 + r / a.tpt, lane, 32);
+                    }
+                    break;
+                }
                 if (lane == 0) {
-                    const uint32_t hkv = by / a.n_hg, head0 = hkv * (uint32_t)(a.Hq / a.Hkv) + by % a.n_hg * a.gp;
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" :: "r"(items + 32 * at), "r"((uint32_t)w.b), "r"((uint32_t)w.row0), "r"(w.len), "r"(w.t0) : "memory");
                     asm volatile("st.shared.v2.u32 [%0+16], {%1,%2};\n st.shared.u32 [%0+24], %3;\n" :: "r"(items + 32 * at), "r"(hkv), "r"(head0),
                                  "r"(valid ? (uint32_t)slot : 0xffffffffu) : "memory");
@@ -630,7 +649,9 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
         const int g = row / tt, t_in = row % tt;
         const float c = a.scale * kPuLog2e;
         uint32_t done = 0, used = 0;                                     // blocks and items of this tile so far
-        for (int k = 0; next_item(k); ++k) {
+        bool left = false;                                               // a wait ran out in the middle of an item
+        int k = 0;
+        for (; next_item(k); ++k) {
             const int n_mine = x ? it.n[1] : it.n[0];
             if (n_mine == 0) continue;
             const int t = it.t0 + x * tt + t_in;
@@ -705,7 +726,7 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             // ---- result rows ---------------------------------------------------------------------------------------------
             if (ok) ok = pu_bar_wait_warp(bar_o + 8 * x, used & 1);
             ++used;
-            if (!ok) break;
+            if (!ok) { left = true; break; }
             pu_fence_after();
             const float inv = 1.f / l;
             uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) +
@@ -748,6 +769,13 @@ prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__
             }
             again |= __ballot_sync(kFullMask, far);
             if (again) prompt_rows_again<DT>(a, it.b, it.row0, it.hkv, t, lim, it.head0 + g, again, lane);
+        }
+        if (left) {                                                      // zeros for its rows and those of the items still to come
+            do {
+                const int t = it.t0 + x * tt + t_in;
+                if (g < a.gp && t < it.len) prompt_leave_row<DT>(a, it.b, (int64_t)it.row0 + t, it.head0 + g, 0, 1);
+            } while (next_item(++k));
+            ok = false;
         }
     }
     if (!ok && a.status) atomicExch(a.status, OMNI_STATUS_WAIT_EXPIRED);

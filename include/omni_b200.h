@@ -405,7 +405,7 @@ int32_t omni_prompt_attn(const omni_prompt_t* call, void* stream);
  *                behind the length stay as they are
  * Cache arguments as in omni_qattn_decode ([B][Hkv][S] rows, contiguous).  Sums are formed in a fixed order: the same call
  * gives the same bits.  `workspace`: omni_attn_weight_sums_workspace_bytes(...) bytes of device scratch.
- *   status_word  device int32 or NULL, as in omni_qattn_decode */
+ *   status_word  device int32 or NULL, as in omni_qattn_decode: columns that were given up add nothing */
 size_t  omni_attn_weight_sums_workspace_bytes(int64_t B, int32_t Hq, int32_t Hkv, int32_t T, int64_t S);
 typedef struct omni_weight_sums_t {
     const void* q; const uint8_t* k_nib; const uint8_t* k_qjl; const float* k_norms; const float* codebooks;

@@ -480,8 +480,8 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                     for (int k = 0; k < 4; ++k) l += e[k].y * exp2f(e[k].x - ref);
                     m = top;
                 }
-                top_all = m == -INFINITY ? 0.f : m;
-                inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;         // no open key: its scores are -inf
+                top_all = m == -INFINITY ? INFINITY : m;                  // no open key, or given up in pass 1: every weight is zero
+                inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
             }
             // pass 2: a thread has four columns, rows lane / 4 + 8 r of its warp's 32
             uint64_t f4[PASS == 2 ? 4 : 1], top4[PASS == 2 ? 4 : 1], inv4[PASS == 2 ? 4 : 1];
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                 }
             }
             for (int t = done; t < done + n_span; ++t) {
-                // after a wait that ran out the warp still goes through the barriers it shares with the others, storing nothing
+                // after a wait that ran out the warp still goes through the barriers it shares with the others; its columns add nothing
                 if (ok) ok = ww_bar_wait(bar_s + (PASS == 1 ? 0 : 8 * half), t & 1);
                 ww_fence_after();
                 const int k0 = (at.tile + t - done) * kWwTile;
@@ -559,12 +559,12 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                     }
                     // two of [four warps of a half][128 keys], so one barrier per tile; the halves do not wait for one another
                     float* red = red_s + (t & 1) * 4 * kWwTile + 64 * half;
-                    *reinterpret_cast<float2*>(red + (warp & 3) * kWwTile + 2 * lane) = ww_unpack2(sum[0]);
+                    *reinterpret_cast<float2*>(red + (warp & 3) * kWwTile + 2 * lane) = ok ? ww_unpack2(sum[0]) : make_float2(0.f, 0.f);
                     asm volatile("bar.sync %0, 128;\n" :: "r"(3 + half) : "memory");
                     if (row < 64) {
                         const float total = (red[row] + red[kWwTile + row]) + (red[2 * kWwTile + row] + red[3 * kWwTile + row]);
                         const int key = k0 + 64 * half + row;
-                        if (ok && key < len) {
+                        if (key < len) {
                             if (a.accumulate || col0 > 0) sums[key] += total;
                             else sums[key] = total;
                         }
@@ -631,9 +631,10 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             }
             if (PASS == 1) {                                             // the column's halves
                 float2* hand = reinterpret_cast<float2*>(red_s);
+                if (!ok) { m = -INFINITY; l = 0.f; }                     // given up: a state that pass 2 ignores, not what the memory held
                 if (half == 1) hand[row] = make_float2(m, l);
                 asm volatile("bar.sync 1, 256;\n" ::: "memory");
-                if (half == 0 && ok && col_on) {
+                if (half == 0 && col_on) {
                     const float2 o = hand[row];
                     const float top = fmaxf(m, o.x), ref = top == -INFINITY ? 0.f : top;
                     a.partial[(bh + blockIdx.x) * cols + col] = make_float2(top, l * ws_ex2(m - ref) + o.y * ws_ex2(o.x - ref));

@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
     const int len = clamp_len(a.seq_lens, b, a.S);
     const int64_t new_len = len < a.budget ? len : a.budget;
     const int64_t src0 = bh * a.S, dst0 = bh * a.capacity;
-    after_predecessor();
+    after_predecessor();                                         // the lengths above are older than the selection
     // old position of row r of the group in lane r (-1: no key)
     int from = -1;
     if (lane < 8 && row0 + lane < new_len) from = a.index[bh * a.budget + row0 + lane];
@@ -280,6 +280,8 @@ extern "C" int32_t omni_evict_keys(const omni_evict_t* call, void* stream) {
     OMNI_ALLOW_SMEM((evict_select_kernel), kSelKeyBytes);
     evict_select_kernel<<<(unsigned)(a.B * a.H), kSelThreads, kSelKeyBytes, st>>>(a);
     OMNI_CUDA(cudaGetLastError());
+    // The selection lets nobody start early (waiting CTAs take up its places: 9 us); behind its last CTA the gap to the gather is still shorter
+    // this way: 12.4 us for 5 users x 2,047 keys against 12.5, and 1 us of host time.
     return check_cuda(launch_early(evict_gather_kernel, dim3((unsigned)((n_groups + kGatherWarps - 1) / kGatherWarps)), kGatherWarps * 32, 0, st, a, groups_per_head, n_groups),
                       "evict_gather_kernel launch");
 }

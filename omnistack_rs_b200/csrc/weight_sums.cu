@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_
     const int64_t bh = blockIdx.x / segments, s0 = blockIdx.x % segments * (kWfKeys * kWfThreads);
     const int64_t b = bh / a.Hkv, h = bh % a.Hkv;
     const int cols = a.Hq / a.Hkv * a.T;
+    const bool ordered = a.causal && a.T > 1;                            // a column may see fewer keys than there are
     after_predecessor();
     const int len = ws_len(a, b);
     float2 v[kWfKeys][kWsStepCols / 2];                                  // the scores, requested before the normalisers are known
@@ -332,6 +333,12 @@ __global__ void __launch_bounds__(kWfThreads) weight_finish_kernel(const __grid_
             for (int i = 0; i < kWsStepCols / 2; ++i) {
                 if (2 * i < cols) total = fmaf(ws_ex2(v[k][i].x - norm[2 * i].x), norm[2 * i].y, total);
                 if (2 * i + 1 < cols) total = fmaf(ws_ex2(v[k][i].y - norm[2 * i + 1].x), norm[2 * i + 1].y, total);
+            }
+            if (ordered && total != total) {                             // keys behind a column's token add nothing, not zero times a NaN query's normaliser
+                total = 0.f;
+#pragma unroll
+                for (int i = 0; i < kWsStepCols; ++i)
+                    if (i < cols && s <= len - a.T + i % a.T) total = fmaf(ws_ex2(((i & 1) ? v[k][i / 2].y : v[k][i / 2].x) - norm[i].x), norm[i].y, total);
             }
         }
         float* d = a.sums + bh * a.S + s;

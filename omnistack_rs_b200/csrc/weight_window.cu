@@ -530,18 +530,24 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                                 }
                             }
                         }
+                        uint64_t n2[2] = {inv4[2 * rb], inv4[2 * rb + 1]};
                         if (masked) {
                             const int l0 = (last4[2 * rb] < len - 1 ? last4[2 * rb] : len - 1) - k0 - 64 * half - 2 * (lane & 3);
                             const int l1 = (last4[2 * rb + 1] < len - 1 ? last4[2 * rb + 1] : len - 1) - k0 - 64 * half - 2 * (lane & 3);
+                            // a NaN column's normaliser goes into the scores that it sees: a masked key's zero times it would be NaN
+                            const float z0 = ww_unpack2(n2[0]).x, z1 = ww_unpack2(n2[1]).x;
+                            n2[0] = z0 == z0 ? n2[0] : 0;
+                            n2[1] = z1 == z1 ? n2[1] : 0;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = 8 * (i >> 2) + (i & 1) <= ((i & 2) ? l1 : l0) ? s[i] : 0xff800000u;
+                            for (int i = 0; i < 32; ++i)
+                                s[i] = 8 * (i >> 2) + (i & 1) <= ((i & 2) ? l1 : l0) ? __float_as_uint(__uint_as_float(s[i]) + ((i & 2) ? z1 - z1 : z0 - z0)) : 0xff800000u;
                         }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 const float2 e = ww_unpack2(ww_fma2(ww_pack2(__uint_as_float(s[4 * i + 2 * r]), __uint_as_float(s[4 * i + 2 * r + 1])), f4[2 * rb + r], top4[2 * rb + r]));
-                                sum[i] = ww_fma2(ww_pack2(ws_ex2(e.x), ws_ex2(e.y)), inv4[2 * rb + r], rb + r ? sum[i] : ww_pack2(0.f, 0.f));
+                                sum[i] = ww_fma2(ww_pack2(ws_ex2(e.x), ws_ex2(e.y)), n2[r], rb + r ? sum[i] : ww_pack2(0.f, 0.f));
                             }
                         }
                     }

@@ -199,8 +199,8 @@ __global__ void __launch_bounds__(kWpWarps * 32) weight_prepare_kernel(const __g
             piece[(40 + 2 * c + i) * kWwTile] = make_uint4(r[0], r[1], r[2], r[3]);
         }
     }
-    // never zero: zero times a masked score's -inf is NaN
-    if (c == 0) reinterpret_cast<float*>(out + (size_t)kWwPrepRows * kWwTile * 16)[col % kWwTile] = fmaxf(a.scale * kWsLog2e / q_mul / ws_pow2(cb_top), 1e-30f);
+    // never zero, as zero times a masked score's -inf is NaN; the factor of tiny queries and centroids is below 1e-37
+    if (c == 0) reinterpret_cast<float*>(out + (size_t)kWwPrepRows * kWwTile * 16)[col % kWwTile] = fmaxf(a.scale * kWsLog2e / q_mul / ws_pow2(cb_top), 1.401298464e-45f);
 }
 
 // Position in the row of tiles: user, kv head, tile of that head.  Users without keys have no place in it.

@@ -1,4 +1,4 @@
-"""``attn_weight_sums`` where a query is NaN."""
+"""``attn_weight_sums`` where a query is NaN, and where queries, centroids and norms are of sizes far apart."""
 import pytest
 import torch
 
@@ -40,3 +40,15 @@ def test_a_nan_query_reaches_the_keys_it_sees(dtype, G, T):
     assert torch.equal(torch.isnan(into), torch.isnan(got)) and bool((into[1, 0, lens[1]:] == 1).all())
     every = attn_weight_sums(q, *rows, seq_lens=seq, causal=False)       # without the causal order it reaches all keys of its head
     assert bool(torch.isnan(every[1, 0, :130]).all()) and bool(torch.isfinite(every[1, 1]).all()) and bool((every[1, 0, 130:] == 0).all())
+
+
+@pytest.mark.parametrize("T", [1, 12])
+@pytest.mark.parametrize("q_size,cb_size,norm_size", [(1e-15, 1e-15, 1e8), (1e-15, 1e-15, 1e10), (1e-12, 1e-20, 1e11), (1e15, 1e-16, 1e-16), (1e-16, 1e15, 1e15)])
+def test_sizes_far_apart(T, q_size, cb_size, norm_size):
+    from omnistack_rs_b200.kernels.eviction import attn_weight_sums
+    nib, qjl, norms, cb = packed(2, 2, 300, 3)
+    norms, cb = norms * norm_size, cb * cb_size
+    q = torch.randn(2, 4, T, 128, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV) * q_size
+    keys = dense.dequantized_keys(nib, qjl, norms, cb, [0, 0], True)
+    got = attn_weight_sums(q, nib, qjl, norms, cb, seq_lens=torch.tensor([300, 77], device=DEV))
+    dense.check_weights(got, q, keys, [300, 77], True, SCALE)

@@ -217,6 +217,15 @@ def status_word(device: torch.device) -> torch.Tensor:
     return _status_words[idx]
 
 
+def status_ptr(device: torch.device) -> int:
+    """Address of the device's status word; 0, so that a call reports nothing, where the word would have to be made inside a capture:
+    it would belong to the graph, and every replay would clear what other calls have reported."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if idx not in _status_words and torch.cuda.is_current_stream_capturing():
+        return 0
+    return status_word(device).data_ptr()
+
+
 def check_device_status(device: torch.device) -> None:
     """Synchronises the device and raises if a kernel reported an expired wait (RuntimeError) or an
     adapter index past the adapter count (IndexError) since the last check."""

@@ -93,7 +93,7 @@ def attn_weight_sums(q: torch.Tensor, k_nibbles: torch.Tensor, k_qjl: torch.Tens
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     call = _WEIGHT_SUMS.pack(q.data_ptr(), k_nibbles.data_ptr(), k_qjl.data_ptr(), k_norms.data_ptr(), cb.data_ptr(),
                              0 if ids is None else ids.data_ptr(), 0 if lens is None else lens.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
-                             sums.data_ptr(), _lib.status_word(dev).data_ptr(), B, S, nbytes, _lib.DTYPE_CODE[q.dtype], per_head, uid, Hq, Hkv, T,
+                             sums.data_ptr(), _lib.status_ptr(dev), B, S, nbytes, _lib.DTYPE_CODE[q.dtype], per_head, uid, Hq, Hkv, T,
                              bool(with_qjl), bool(rotate_q), bool(causal), into is not None, 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
     with _lib.on_device(dev):
         _lib.check(lib.omni_attn_weight_sums(call, _lib.stream_ptr(dev)))

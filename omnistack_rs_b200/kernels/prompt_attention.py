@@ -96,7 +96,7 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens
     k, k_at, k0, k1, k2 = _tiles(k)
     v, v_at, v0, v1, v2 = _tiles(v)
     out = torch.empty(B, Hq, T, HEAD_DIM, dtype=dtype, device=dev)
-    call = _PROMPT.pack(q_at, k_at, v_at, out.data_ptr(), cu_at, lens_at, _lib.status_word(dev).data_ptr(), q0, q1, q2, k0, k1, k2, v0, v1, v2,
+    call = _PROMPT.pack(q_at, k_at, v_at, out.data_ptr(), cu_at, lens_at, _lib.status_ptr(dev), q0, q1, q2, k0, k1, k2, v0, v1, v2,
                         n_seqs, B, T, code, Hq, Hkv, bool(causal), _SCALE if scale is None else scale)
     with _lib.on_device(dev):
         _lib.check(lib.omni_prompt_attn(call, _lib.stream_ptr(dev)))

@@ -15,9 +15,12 @@
 // do it themselves: S_t of a block is issued behind P_t V of the block before, so its arrival says that O_t is complete.
 //
 // What bounds it: the chain of one tile, scores (512 cycles) - softmax (about 1,900) - product (512), two tiles deep, and on long prompts
-// the board's power: 16,384 tokens of 32 heads in fp16 take 1.80 ms, 1,220 TFLOP/s at about 1.62 GHz under the 1,000 W cap, 75 % of the
-// measured burst rate of a plain matrix product and 87 % of its sustained one.  A quarter of the exponentials as a polynomial on the
-// FP32 units (1.84 ms) or a third (1.90 ms) gained nothing.
+// the board's power: 16,384 tokens of 32 heads in fp16 take 1.82 to 1.99 ms on different boards, 1,100 to 1,210 TFLOP/s at about 1.62 GHz
+// under the 1,000 W cap, 68 to 74 % of the measured burst rate of a plain matrix product and 79 to 86 % of its sustained one.  A quarter of the
+// exponentials as a polynomial on the FP32 units (1.84 ms against 1.80 on one board) or a third (1.90 ms) gained nothing.
+//
+// The tensor pipe takes both operands in 16 bits, so weights are rounded to the type (their sum is not): relative to 64 bits a ragged bf16
+// batch is off by 2.1e-3 and 16,384 fp16 tokens by 2.7e-4, of which 1.6e-3 and 2.1e-4 are the rounding of the result alone.
 //
 // A zero weight times an infinite or NaN value of a masked key is NaN.  Rows that come out NaN although no score of theirs is, in dims
 // that the values they see do not account for (prompt_unexplained), are formed again from global memory over their own keys alone.

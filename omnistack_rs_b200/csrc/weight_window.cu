@@ -19,7 +19,7 @@
 // score warps doing so between two spans had the products wait: 210 us instead of 190 for 16 users x 8 heads x up to 8,192 keys x 128
 // columns).  Warp 16 issues the products.
 // Shared memory bounds a tile: 64 lookups of 8 bytes and 40 stores of 16 bytes per key, and the products' reads of K', about 1,900 cycles
-// against 1,536 of the tensor pipe.  Measured, a tile takes 2,400 cycles in pass 1 and 3,200 in pass 2, and the call 156 us, 18.7 of which
+// against 1,536 of the tensor pipe.  Measured, a tile takes 2,400 cycles in pass 1 and 3,200 in pass 2, and the call 150 us, 18.7 of which
 // its products would need alone.
 #include "weight_sums.cuh"
 
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
             ww_bar_init(bar_full + 8 * i, 8);
             ww_bar_init(bar_empty + 8 * i, 1);
             // The products of one part of a tile go on while the other's are taken out.  Pass 1: values, then signs, of all keys (128 keys per
-            // instruction; 64 take longer by a third: 171 us for the call instead of 156).  Pass 2: both, of keys 0-63 and then of 64-127, since its
+            // instruction; 64 take longer by a third: 171 us for the call instead of 156, when this was measured).  Pass 2: both, of keys 0-63 and then of 64-127, since its
             // four columns' factors leave no registers to keep a tile's values until the signs are there.
             ww_bar_init(bar_s + 8 * i, 1);
             ww_bar_init(bar_free + 8 * i, PASS == 1 ? 8 : 4);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kWwThreads, 1) weight_window_kernel(const __gr
                     ww_fence_after();
                     const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(a.prepared) + (bh_now * ((cols + kWwTile - 1) / kWwTile) + col0 / kWwTile) * kWwPrepBytes) + row;
                     const bool col_on = col0 + row < cols;
-                    // four pieces at a time: 64 values, their remainders, 32 values of G . q, their remainders (more registers would spill)
+                    // four pieces at a time: 64 values, their remainders, 32 values of G . q, their remainders (the warp has 72 registers)
 #pragma unroll 1
                     for (int part = 0; part < 6; ++part) {
                         const bool of_q = part < 4;

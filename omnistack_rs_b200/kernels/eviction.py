@@ -61,8 +61,9 @@ def attn_weight_sums(q: torch.Tensor, k_nibbles: torch.Tensor, k_qjl: torch.Tens
 
     ``causal``: the T tokens are the last ones of the cache, so token t sees the keys up to ``len - T + t`` (the window of a
     prompt's last tokens; one token sees everything); ``False``: every token sees all keys below the length.  A token without
-    keys adds nothing.  Without ``into`` the result is a new tensor, zeros at and behind the length; with it the weights are
-    added to ``into`` in place (entries at and behind the length stay as they are) and ``into`` is returned."""
+    keys adds nothing; a NaN query reaches the keys its token sees, and no others.  Without ``into`` the result is a new tensor, zeros at and behind the length; with it the weights are
+    added to ``into`` in place (entries at and behind the length stay as they are) and ``into`` is returned.  ``q`` and the
+    nibble rows start on 16-byte boundaries, sign bytes on 8 (``ValueError``); arrays that are not contiguous are copied."""
     if q.dim() != 4 or k_nibbles.dim() != 4:
         raise ValueError("q must be (B, n_heads, T, 128) and k_nibbles (B, n_kv_heads, S, 64)")
     B, Hq, T, D = q.shape
@@ -109,7 +110,7 @@ def evict_keys(sums: torch.Tensor, k_nibbles: torch.Tensor, k_qjl: torch.Tensor,
 
     The kept rows leave in their order, bit for bit, in new arrays of ``capacity`` rows per head (``budget`` when ``None``),
     zeros behind the new length; the arrays given are not changed.  ``index`` (B, n_kv_heads, budget) int32 holds the old
-    positions, -1 behind the new length, and ``seq_lens`` the new lengths, int32.  ``v_paired``: V's nibble rows are in a
+    positions, -1 behind the new length, and ``seq_lens`` the new lengths, int32.  Alignment as in :func:`attn_weight_sums`.  ``v_paired``: V's nibble rows are in a
     resident cache's pair layout for the old lengths, and are again for the new ones."""
     if k_nibbles.dim() != 4:
         raise ValueError("k_nibbles must be (B, n_kv_heads, S, 64)")

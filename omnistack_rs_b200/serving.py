@@ -208,13 +208,15 @@ class QuantizedKVCache:
     def _forget_sums(self, T: int) -> None:
         """No weight has reached the T keys that every user is about to get, whatever stood in their rows before: ``lens`` may
         have been set back, for another continuation or another prompt."""
-        if self.weight_sums is None or T == 0 or self.n_users == 0:
+        sums = self.weight_sums
+        if sums is None or T == 0:
             return
-        dev = self.weight_sums.device
+        if sums.shape != (self.n_users, self.n_kv_heads, self.max_len) or sums.dtype is not torch.float32 or not sums.is_contiguous():
+            raise ValueError(f"weight_sums must be contiguous float32 {(self.n_users, self.n_kv_heads, self.max_len)}, got {tuple(sums.shape)} {sums.dtype}")
+        dev = _lib.require_cuda(sums)
         lens = _lib.as_device(self.lens, dev, torch.int64)
         with _lib.on_device(dev):
-            _lib.check(_lib.load().omni_clear_new_sums(_lib.ptr(self.weight_sums), _lib.ptr(lens), self.n_users, self.n_kv_heads, self.max_len, T,
-                                                       _lib.stream_ptr(dev)))
+            _lib.check(_lib.load().omni_clear_new_sums(_lib.ptr(sums), _lib.ptr(lens), *sums.shape, T, _lib.stream_ptr(dev)))
 
     def _capturing(self) -> bool:
         return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()

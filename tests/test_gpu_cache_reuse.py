@@ -112,3 +112,20 @@ def test_prompts_that_fit_although_their_padding_does_not(pair_v):
     assert over.lens.tolist() == [0, 0, 0] and bool((over.k_nib == 0).all())
     none = over.prefill(*x, torch.zeros(N, dtype=torch.int64))            # prompts without a token
     assert bool((none == 0).all()) and over.lens.tolist() == [0, 0, 0]
+
+
+def test_sums_that_are_not_the_cache_s_own_kind():
+    """A user may bring sums of their own, from a file for instance: of the cache's shape, on its device."""
+    cache = make_cache()
+    x = rows(H, 5, 1)
+    cache.append(x, x)
+    good = torch.ones(N, H, MAX, device=DEV)
+    for bad, error in ((good.cpu(), RuntimeError), (good[:, :, :50], ValueError), (good.double(), ValueError), (good.transpose(0, 1).contiguous().transpose(0, 1), ValueError)):
+        cache.weight_sums = bad
+        with pytest.raises(error):
+            cache.append(x, x)
+        assert cache.lens.tolist() == [5] * N
+    cache.weight_sums = good
+    cache.append(x, x)
+    assert cache.lens.tolist() == [10] * N
+    assert bool((good[:, :, 5:10] == 0).all()) and bool((good[:, :, :5] == 1).all()) and bool((good[:, :, 10:] == 1).all())

@@ -11,7 +11,8 @@
 // weights multiplied in:   out_e = rsqrt(..) (x_e A_e + x_partner(e) B_e),   A_e = w_e cos, B_e = -+ w_partner(e) sin.
 // The rows' factor being common, partners trade the rows' raw words (4 shuffles instead of 8 for a 16-bit type).
 // 8 x 2,048 tokens of 40 heads in bf16: 71 us, 4.7 TB/s of the 6.5 a plain copy reaches (118 us with the angles and weights apart and no
-// rows requested ahead; six CTAs per SM leave 80 registers, of which up to 120 bytes per thread spill); a decode step of 64 users 5.5 us, launch, positions, angles and rows one after the other.
+// rows requested ahead; six CTAs per SM leave 80 registers, and up to 120 bytes per thread spill); a decode step of 64 users 5.5 us, launch,
+// positions, angles and rows one after the other.
 #include "common.cuh"
 
 namespace omni {

@@ -5,8 +5,8 @@
 // One pass over the keys with the running maximum m and sum of each row.  64 x 64 tiles of scores on the FP32 units (two products per
 // instruction): 256 threads, 4 x 4 scores and 4 x 8 outputs each; K and V share one buffer so that two CTAs fit an SM.  4 prompts of up
 // to 611 tokens and 8 heads take 152 us (189 with one product per instruction), 1,500 tokens run at 33 TFLOP/s: bound by the loads
-// between the phases of a tile, which only the other CTA covers (and whose 128 registers spill 68 to 76 bytes per thread).  Tiles of 32 rows (three CTAs per SM) win below 100 tokens (18 us
-// against 23) and lose above (180 us).
+// between the phases of a tile, which only the other CTA covers (two CTAs leave 128 registers, and 68 to 76 bytes per thread spill).
+// Tiles of 32 rows (three CTAs per SM) win below 100 tokens (18 us against 23) and lose above (180 us).
 #include "prompt.cuh"
 
 namespace omni {
